@@ -446,6 +446,87 @@ MSX_API int msx_cg_context_solve(msx_cg_context *ctx, const float *b,
 MSX_API int msx_cg_context_destroy(msx_cg_context *ctx);
 
 /* ------------------------------------------------------------------------ */
+/* Distillation against a teacher's stored top logits. No counterpart in the  */
+/* reference.                                                                */
+/* ------------------------------------------------------------------------ */
+/* The teacher is a CSR matrix (n_rows tokens x n_cols vocabulary) of logits;
+ * `logits` are the student's, dense with stride 1 along the vocabulary and
+ * `logits_stride` elements between rows, of the same value dtype. With p =
+ * softmax of a row's stored entries / temperature and q = softmax of the
+ * student's whole row / temperature,
+ *   loss = temperature^2 sum_e p_e (log p_e - log q_e)       (float32, per row)
+ *   grad = cotangent * temperature * (q - p)                 (value dtype).
+ * A row without entries has loss 0 and gradient 0, a row whose cotangent is 0
+ * gradient 0. Entries of one column add up. An entry outside [0, n_cols) makes
+ * its row's loss NaN and is left out of the gradient.
+ * forward: `stats` (4 floats a row, for the backward call) may be null.
+ * backward: from the forward's stats. forward_backward: both in one pass.
+ * `cotangent` (float32, per row) may be null: ones. `grad` is contiguous. */
+MSX_API int msx_csr_distill_forward(int value_dtype, int index_dtype,
+                                    const void *data, const void *indices,
+                                    const void *indptr, int64_t nnz,
+                                    const void *logits, int64_t logits_stride,
+                                    int64_t n_rows, int64_t n_cols,
+                                    float temperature, float *loss,
+                                    float *stats, void *stream);
+MSX_API int msx_csr_distill_backward(int value_dtype, int index_dtype,
+                                     const void *data, const void *indices,
+                                     const void *indptr, int64_t nnz,
+                                     const void *logits, int64_t logits_stride,
+                                     int64_t n_rows, int64_t n_cols,
+                                     float temperature, const float *stats,
+                                     const float *cotangent, void *grad,
+                                     void *stream);
+MSX_API int msx_csr_distill_forward_backward(
+    int value_dtype, int index_dtype, const void *data, const void *indices,
+    const void *indptr, int64_t nnz, const void *logits, int64_t logits_stride,
+    int64_t n_rows, int64_t n_cols, float temperature, const float *cotangent,
+    float *loss, void *grad, void *stream);
+
+/* ------------------------------------------------------------------------ */
+/* Windowed attention with sink keys. No counterpart in the reference.        */
+/* ------------------------------------------------------------------------ */
+/* softmax(scale Q K^T) V over the keys that a query sees: query position p
+ * sees key j of its sequence iff j <= p and (p - j < window or j lies among the
+ * sequence's first `sinks` keys). A query that sees nothing has output and
+ * gradient 0. q (batch, q_len, q_heads, dim) and k, v (batch, k_len, k_heads,
+ * dim) have stride 1 along dim and the given strides (elements) along batch,
+ * tokens and heads, q_strides[3] etc.; query head h reads key head
+ * h / (q_heads / k_heads). dim is at most 256.
+ * Without indptr a batch entry is one sequence and query i is at position i +
+ * k_len - q_len. With indptr (n_seq + 1 boundaries on the device, batch 1,
+ * q_len = k_len) sequences lie one after another along the tokens; tokens
+ * outside all of them see nothing and get zeros.
+ * out, grad_out, dq are contiguous like q; dk, dv like k. lse: float (batch,
+ * q_heads, q_len), written by forward (null: not wanted), read by backward;
+ * delta: float workspace of the same size. backward reads forward's out. */
+MSX_API int msx_window_attention_forward(
+    int value_dtype, const void *q, const int64_t *q_strides, const void *k,
+    const int64_t *k_strides, const void *v, const int64_t *v_strides,
+    int64_t batch, int64_t q_len, int64_t k_len, int64_t q_heads,
+    int64_t k_heads, int64_t dim, int64_t window, int64_t sinks, float scale,
+    int index_dtype, const void *indptr, int64_t n_seq, void *out, float *lse,
+    void *stream);
+MSX_API int msx_window_attention_backward(
+    int value_dtype, const void *q, const int64_t *q_strides, const void *k,
+    const int64_t *k_strides, const void *v, const int64_t *v_strides,
+    int64_t batch, int64_t q_len, int64_t k_len, int64_t q_heads,
+    int64_t k_heads, int64_t dim, int64_t window, int64_t sinks, float scale,
+    int index_dtype, const void *indptr, int64_t n_seq, const void *out,
+    const float *lse, const void *grad_out, float *delta, void *dq, void *dk,
+    void *dv, void *stream);
+/* One query for each batch entry, at the end of that entry's cache: q (batch,
+ * q_heads, dim) with strides {batch, heads}; caches (batch, max_len, k_heads,
+ * dim) of which entry b holds lengths[b] tokens (device array of index_dtype;
+ * clamped to [0, max_len]; 0 gives zeros). out is contiguous like q. */
+MSX_API int msx_window_attention_decode(
+    int value_dtype, const void *q, const int64_t *q_strides,
+    const void *k_cache, const int64_t *k_strides, const void *v_cache,
+    const int64_t *v_strides, int64_t batch, int64_t max_len, int64_t q_heads,
+    int64_t k_heads, int64_t dim, int64_t window, int64_t sinks, float scale,
+    int index_dtype, const void *lengths, void *out, void *stream);
+
+/* ------------------------------------------------------------------------ */
 /* DLPack entry points: the same operations with every array passed as a     */
 /* DLTensor (borrowed; outputs caller-allocated). They check what the raw    */
 /* entry points cannot: device (CUDA, the current device), dtype codes,      */

@@ -582,6 +582,152 @@ int msx_csr_diagonal(int value_dtype, int index_dtype, const void *data, const v
   });
 }
 
+// ---- distillation against a CSR matrix of teacher logits -------------------------
+static void distill_checked(int value_dtype, int index_dtype, const DistillCall &c, void *stream) {
+  require(c.rows >= 0 && c.vocab >= 0 && c.nnz >= 0, MSX_ERR_INVALID, "csr_distillation sizes must be non-negative.");
+  require(c.ld >= c.vocab, MSX_ERR_INVALID, "csr_distillation logits rows must not overlap.");
+  require(std::isfinite(c.temperature) && c.temperature > 0.f, MSX_ERR_INVALID,
+          "csr_distillation temperature must be positive and finite.");
+  dispatch_value(value_dtype, [](auto) {});
+  dispatch_index(index_dtype, [](auto) {});
+  check_ptr(c.t_data, c.nnz, "csr_distillation data");
+  check_ptr(c.t_indices, c.nnz, "csr_distillation indices");
+  check_ptr(c.t_indptr, c.rows + 1, "csr_distillation indptr");
+  check_ptr(c.logits, c.rows * c.vocab, "csr_distillation logits");
+  distill_run(value_dtype, index_dtype, c, as_stream(stream));
+}
+
+int msx_csr_distill_forward(int value_dtype, int index_dtype, const void *data, const void *indices,
+                            const void *indptr, int64_t nnz, const void *logits, int64_t logits_stride,
+                            int64_t n_rows, int64_t n_cols, float temperature, float *loss, float *stats,
+                            void *stream) {
+  return guarded([&] {
+    check_ptr(loss, n_rows, "csr_distillation loss");
+    distill_checked(value_dtype, index_dtype,
+                    DistillCall{logits, logits_stride, data, indices, indptr, nnz, n_rows, n_cols, temperature,
+                                nullptr, loss, stats, nullptr},
+                    stream);
+  });
+}
+
+int msx_csr_distill_backward(int value_dtype, int index_dtype, const void *data, const void *indices,
+                             const void *indptr, int64_t nnz, const void *logits, int64_t logits_stride,
+                             int64_t n_rows, int64_t n_cols, float temperature, const float *stats,
+                             const float *cotangent, void *grad, void *stream) {
+  return guarded([&] {
+    check_ptr(stats, n_rows, "csr_distillation stats");
+    check_ptr(grad, n_rows * n_cols, "csr_distillation grad");
+    distill_checked(value_dtype, index_dtype,
+                    DistillCall{logits, logits_stride, data, indices, indptr, nnz, n_rows, n_cols, temperature,
+                                cotangent, nullptr, const_cast<float *>(stats), grad},
+                    stream);
+  });
+}
+
+int msx_csr_distill_forward_backward(int value_dtype, int index_dtype, const void *data, const void *indices,
+                                     const void *indptr, int64_t nnz, const void *logits, int64_t logits_stride,
+                                     int64_t n_rows, int64_t n_cols, float temperature, const float *cotangent,
+                                     float *loss, void *grad, void *stream) {
+  return guarded([&] {
+    check_ptr(loss, n_rows, "csr_distillation loss");
+    check_ptr(grad, n_rows * n_cols, "csr_distillation grad");
+    distill_checked(value_dtype, index_dtype,
+                    DistillCall{logits, logits_stride, data, indices, indptr, nnz, n_rows, n_cols, temperature,
+                                cotangent, loss, nullptr, grad},
+                    stream);
+  });
+}
+
+// ---- windowed attention ------------------------------------------------------------
+static WindowCall window_checked(int value_dtype, const void *q, const int64_t *qs, const void *k, const int64_t *ks,
+                                 const void *v, const int64_t *vs, int64_t batch, int64_t q_len, int64_t k_len,
+                                 int64_t q_heads, int64_t k_heads, int64_t dim, int64_t window, int64_t sinks,
+                                 float scale, int index_dtype) {
+  require(batch >= 0 && q_len >= 0 && k_len >= 0, MSX_ERR_INVALID, "window_attention sizes must be non-negative.");
+  require(k_heads > 0 && q_heads > 0 && q_heads % k_heads == 0, MSX_ERR_INVALID,
+          "window_attention query heads must be a multiple of key heads.");
+  require(dim > 0 && dim <= 256, MSX_ERR_INVALID, "window_attention head size must be between 1 and 256.");
+  require(window >= 0 && sinks >= 0, MSX_ERR_INVALID, "window_attention window and sinks must be non-negative.");
+  require(std::isfinite(scale), MSX_ERR_INVALID, "window_attention scale must be finite.");
+  require(batch <= 65535 && q_heads <= 65535 && q_len <= (1 << 30) && k_len <= (1 << 30), MSX_ERR_OVERFLOW,
+          "window_attention takes at most 65535 sequences and heads and 2^30 tokens.");
+  dispatch_value(value_dtype, [](auto) {});
+  dispatch_index(index_dtype, [](auto) {});
+  require(qs && ks && vs, MSX_ERR_INVALID, "window_attention strides must not be null.");
+  check_ptr(q, batch * q_len, "window_attention q");
+  check_ptr(k, batch * k_len, "window_attention k");
+  check_ptr(v, batch * k_len, "window_attention v");
+  WindowCall c{};
+  c.q = WindowTensor{q, qs[0], qs[1], qs[2]};
+  c.k = WindowTensor{k, ks[0], ks[1], ks[2]};
+  c.v = WindowTensor{v, vs[0], vs[1], vs[2]};
+  c.batch = batch, c.q_len = q_len, c.k_len = k_len;
+  c.q_heads = (int)q_heads, c.k_heads = (int)k_heads, c.dim = (int)dim;
+  c.window = window, c.sinks = sinks, c.scale = scale;
+  c.indptr_dtype = index_dtype;
+  return c;
+}
+
+static void window_packed(WindowCall &c, const void *indptr, int64_t n_seq) {
+  if (indptr == nullptr) return;
+  require(c.batch == 1 && c.q_len == c.k_len && n_seq >= 0, MSX_ERR_INVALID,
+          "window_attention with indptr needs batch 1 and as many queries as keys.");
+  c.indptr = indptr, c.n_seq = n_seq;
+}
+
+int msx_window_attention_forward(int value_dtype, const void *q, const int64_t *q_strides, const void *k,
+                                 const int64_t *k_strides, const void *v, const int64_t *v_strides, int64_t batch,
+                                 int64_t q_len, int64_t k_len, int64_t q_heads, int64_t k_heads, int64_t dim,
+                                 int64_t window, int64_t sinks, float scale, int index_dtype, const void *indptr,
+                                 int64_t n_seq, void *out, float *lse, void *stream) {
+  return guarded([&] {
+    WindowCall c = window_checked(value_dtype, q, q_strides, k, k_strides, v, v_strides, batch, q_len, k_len, q_heads,
+                                  k_heads, dim, window, sinks, scale, index_dtype);
+    window_packed(c, indptr, n_seq);
+    check_ptr(out, batch * q_len, "window_attention out");
+    c.out = out, c.lse = lse;
+    window_forward_run(value_dtype, c, as_stream(stream));
+  });
+}
+
+int msx_window_attention_backward(int value_dtype, const void *q, const int64_t *q_strides, const void *k,
+                                  const int64_t *k_strides, const void *v, const int64_t *v_strides, int64_t batch,
+                                  int64_t q_len, int64_t k_len, int64_t q_heads, int64_t k_heads, int64_t dim,
+                                  int64_t window, int64_t sinks, float scale, int index_dtype, const void *indptr,
+                                  int64_t n_seq, const void *out, const float *lse, const void *grad_out,
+                                  float *delta, void *dq, void *dk, void *dv, void *stream) {
+  return guarded([&] {
+    WindowCall c = window_checked(value_dtype, q, q_strides, k, k_strides, v, v_strides, batch, q_len, k_len, q_heads,
+                                  k_heads, dim, window, sinks, scale, index_dtype);
+    window_packed(c, indptr, n_seq);
+    check_ptr(out, batch * q_len, "window_attention out");
+    check_ptr(lse, batch * q_len, "window_attention lse");
+    check_ptr(grad_out, batch * q_len, "window_attention grad_out");
+    check_ptr(delta, batch * q_len, "window_attention delta");
+    require((dk == nullptr) == (dv == nullptr), MSX_ERR_INVALID, "window_attention dk and dv come together.");
+    c.out = const_cast<void *>(out), c.lse = const_cast<float *>(lse), c.grad_out = grad_out, c.delta = delta;
+    c.dq = dq, c.dk = dk, c.dv = dv;
+    window_backward_run(value_dtype, c, as_stream(stream));
+  });
+}
+
+int msx_window_attention_decode(int value_dtype, const void *q, const int64_t *q_strides, const void *k_cache,
+                                const int64_t *k_strides, const void *v_cache, const int64_t *v_strides, int64_t batch,
+                                int64_t max_len, int64_t q_heads, int64_t k_heads, int64_t dim, int64_t window,
+                                int64_t sinks, float scale, int index_dtype, const void *lengths, void *out,
+                                void *stream) {
+  return guarded([&] {
+    require(q_strides != nullptr, MSX_ERR_INVALID, "window_attention strides must not be null.");
+    const int64_t qs[3] = {q_strides[0], 0, q_strides[1]};
+    WindowCall c = window_checked(value_dtype, q, qs, k_cache, k_strides, v_cache, v_strides, batch, 1, max_len,
+                                  q_heads, k_heads, dim, window, sinks, scale, index_dtype);
+    check_ptr(lengths, batch, "window_attention lengths");
+    check_ptr(out, batch, "window_attention out");
+    c.lengths = lengths, c.out = out;
+    window_decode_run(value_dtype, c, as_stream(stream));
+  });
+}
+
 // ---- multi-GPU (NCCL) ---------------------------------------------------------
 int msx_dist_unique_id(void *out, int64_t size) {
   return guarded([&] {

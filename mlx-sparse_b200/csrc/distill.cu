@@ -1,0 +1,552 @@
+// Distillation against a teacher's stored top logits (a CSR matrix, tokens x
+// vocabulary), forward, backward, and both in one pass over the logits.
+//
+// For a row with teacher entries t_e at columns c_e and student logits z:
+//   p_e  = softmax_e(t_e / T)               over the row's stored entries
+//   q_j  = softmax_j(z_j / T)               over the whole vocabulary
+//   loss = T^2 sum_e p_e (log p_e - log q_{c_e})
+//   dloss/dz_j = T (q_j - sum_{e: c_e = j} p_e)
+// A row without entries has loss 0 and gradient 0 whatever its logits hold.
+// Entries that share a column are terms of their own; their p add up in the
+// gradient. Everything is computed in base 2 (c = log2(e) / T) and in fp32;
+// the gradient is rounded once, to the logits' type.
+//
+// Bound: HBM. Forward reads the logits once, the backward pass reads them
+// again and writes the gradient; the one-pass form keeps a row's logits in
+// shared memory (spread over a cluster when one SM's is too small) between
+// the sum of the exponentials and the gradient, so it reads once and writes
+// once, two thirds of the bytes of the two passes.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "ops.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace msx {
+namespace {
+
+constexpr float kNegInf = -INFINITY;
+
+// Per-row softmax statistics kept for the backward pass.
+struct RowStats {
+  float z_max, z_inv;  // c max_j z_j and 1 / sum_j 2^(c z_j - z_max)
+  float t_max, t_inv;  // the same of the teacher's entries
+};
+
+constexpr int kMaxKept = 200 * 1024;  // shared memory of a slice, at most
+
+struct DistillArgs {
+  const void *logits;
+  int64_t ld;  // elements between rows of the logits
+  const void *t_data, *t_idx, *t_ptr;
+  int64_t nnz, rows, vocab;
+  float c, temperature;
+  const float *cot;  // null: ones
+  float *loss;
+  RowStats *stats;
+  void *grad;  // contiguous (rows, vocab)
+  int64_t slice;  // columns of a row for each CTA of its cluster
+  int n_slices;
+};
+
+// ex2.approx: at most 2 ulp, results below 2^-126 flushed to zero; the
+// probabilities lost there are below fp32's smallest normal number.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T> struct Vec;  // 16 bytes of T
+template <> struct Vec<float> {
+  static constexpr int n = 4;
+  __device__ static void unpack(const uint4 &v, float *f) {
+    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+  }
+  __device__ static uint4 pack(const float *f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+template <> struct Vec<__half> {
+  static constexpr int n = 8;
+  __device__ static void unpack(const uint4 &v, float *f) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+      f[2 * i] = p.x, f[2 * i + 1] = p.y;
+    }
+  }
+  __device__ static uint4 pack(const float *f) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <> struct Vec<__nv_bfloat16> {
+  static constexpr int n = 8;
+  __device__ static void unpack(const uint4 &v, float *f) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  __device__ static uint4 pack(const float *f) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// Running maximum m of the logits and sum of 2^((z - m) c). A sum that is still
+// empty has m = -inf and sum 0; a NaN ends up in the sum.
+struct MaxSum {
+  float m = kNegInf, s = 0.f;
+  __device__ static float base(float m, float c) { return m == kNegInf ? 0.f : m * c; }
+  template <int N> __device__ void add(const float *z, float c) {
+    float top = z[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, z[i]);
+    if (top > m) {
+      s *= exp2_fast(fmaf(m, c, -base(top, c)));
+      m = top;
+    }
+    const float b = base(m, c);
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += exp2_fast(fmaf(z[i], c, -b));
+  }
+  __device__ void join(float m2, float s2, float c) {
+    const float top = fmaxf(m, m2), b = base(top, c);
+    s = s * exp2_fast(fmaf(m, c, -b)) + s2 * exp2_fast(fmaf(m2, c, -b));
+    m = top;
+  }
+};
+
+// Joins every thread's pair; thread order is fixed, so the result is too.
+__device__ MaxSum block_join(MaxSum v, float c, float2 *warp_part) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    const float m2 = __shfl_xor_sync(~0u, v.m, d), s2 = __shfl_xor_sync(~0u, v.s, d);
+    v.join(m2, s2, c);
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = blockDim.x >> 5;
+  __syncthreads();
+  if (lane == 0) warp_part[warp] = make_float2(v.m, v.s);
+  __syncthreads();
+  MaxSum r;
+  for (int w = 0; w < n; ++w) r.join(warp_part[w].x, warp_part[w].y, c);
+  return r;
+}
+
+__device__ float block_sum(float v, float *warp_part) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float r = 0.f;
+  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) r += warp_part[w];
+  return r;
+}
+
+// The row's entries, clamped into the arrays.
+template <typename I> __device__ void row_range(const DistillArgs &a, int64_t row, int64_t &lo, int64_t &hi) {
+  const I *ptr = static_cast<const I *>(a.t_ptr);
+  lo = max((int64_t)0, min((int64_t)ptr[row], a.nnz));
+  hi = max(lo, min((int64_t)ptr[row + 1], a.nnz));
+}
+
+template <typename T> __device__ MaxSum teacher_stats(const DistillArgs &a, int64_t lo, int64_t hi, float2 *part) {
+  const T *t = static_cast<const T *>(a.t_data);
+  MaxSum v;
+  for (int64_t e = lo + threadIdx.x; e < hi; e += blockDim.x) {
+    const float x = VT<T>::load(t[e]);
+    v.add<1>(&x, a.c);
+  }
+  return block_join(v, a.c, part);
+}
+
+// T^2 sum_e p_e (log p_e - log q_{c_e}); entries with p = 0 add nothing (0 log
+// 0 = 0), an entry outside the vocabulary makes the loss NaN.
+template <typename T, typename I>
+__device__ float row_loss(const DistillArgs &a, const T *z, int64_t lo, int64_t hi, const RowStats &st, float z_sum,
+                          float t_sum, float *part) {
+  const T *t = static_cast<const T *>(a.t_data);
+  const I *idx = static_cast<const I *>(a.t_idx);
+  const float lg_z = log2f(z_sum), lg_t = log2f(t_sum);
+  float v = 0.f;
+  for (int64_t e = lo + threadIdx.x; e < hi; e += blockDim.x) {
+    const int64_t col = (int64_t)idx[e];
+    const float lp = fmaf(VT<T>::load(t[e]), a.c, -st.t_max) - lg_t;
+    const float p = exp2_fast(lp);
+    if (col < 0 || col >= a.vocab) {
+      v = NAN;
+    } else if (!(p == 0.f)) {
+      const float lq = fmaf(VT<T>::load(z[col]), a.c, -st.z_max) - lg_z;
+      v = fmaf(p, lp - lq, v);
+    }
+  }
+  return block_sum(v, part) * (a.temperature * a.temperature * 0.69314718055994531f);
+}
+
+// The columns [c0, c1) of a row as 16-byte vectors of the row's own alignment:
+// `head` loose elements, `nvec` vectors, `tail` loose elements.
+template <typename T> struct SliceShape {
+  int head, tail, nvec;
+  __device__ SliceShape(const T *p, int64_t n) {
+    const int mis = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+    head = (int)min((int64_t)(mis ? Vec<T>::n - mis : 0), n);
+    nvec = (int)((n - head) / Vec<T>::n);
+    tail = (int)(n - head - (int64_t)nvec * Vec<T>::n);
+  }
+};
+
+// Subtracts the teacher's probabilities from the gradient of columns [c0, c1):
+// the gradient of every entry's column is recomputed and rounded once. `bits`
+// (a bit for each column) finds columns that occur twice; only then the
+// probabilities are added up in `table`, as integers of 2^-62 so that their
+// order does not matter, `table_n` columns at a time.
+template <typename T, typename I>
+__device__ void subtract_teacher(const DistillArgs &a, const T *z, T *g, int64_t lo, int64_t hi, int64_t c0,
+                                 int64_t c1, const RowStats &st, float scale, uint32_t *bits,
+                                 unsigned long long *table, int64_t table_n) {
+  const T *t = static_cast<const T *>(a.t_data);
+  const I *idx = static_cast<const I *>(a.t_idx);
+  const int words = (int)((c1 - c0 + 31) / 32);
+  for (int w = threadIdx.x; w < words; w += blockDim.x) bits[w] = 0;
+  __syncthreads();  // also: the gradient of this slice is written
+  int twice = 0;
+  for (int64_t e = lo + threadIdx.x; e < hi; e += blockDim.x) {
+    const int64_t col = (int64_t)idx[e];
+    if (col < c0 || col >= c1) continue;
+    const uint32_t bit = 1u << ((col - c0) & 31);
+    twice |= (atomicOr(&bits[(col - c0) >> 5], bit) & bit) != 0;
+    const float p = exp2_fast(fmaf(VT<T>::load(t[e]), a.c, -st.t_max)) * st.t_inv;
+    const float q = exp2_fast(fmaf(VT<T>::load(z[col]), a.c, -st.z_max)) * st.z_inv;
+    g[col] = VT<T>::store((q - p) * scale);
+  }
+  if (!__syncthreads_or(twice)) return;
+  for (int64_t b0 = c0; b0 < c1; b0 += table_n) {
+    const int64_t b1 = min(c1, b0 + table_n);
+    for (int64_t j = threadIdx.x; j < b1 - b0; j += blockDim.x) table[j] = 0;
+    __syncthreads();
+    for (int64_t e = lo + threadIdx.x; e < hi; e += blockDim.x) {
+      const int64_t col = (int64_t)idx[e];
+      if (col < b0 || col >= b1) continue;
+      const float p = exp2_fast(fmaf(VT<T>::load(t[e]), a.c, -st.t_max)) * st.t_inv;
+      atomicAdd(&table[col - b0], __float2ull_rn(p * 4611686018427387904.f));
+    }
+    __syncthreads();
+    for (int64_t e = lo + threadIdx.x; e < hi; e += blockDim.x) {
+      const int64_t col = (int64_t)idx[e];
+      if (col < b0 || col >= b1) continue;
+      // a NaN teacher row keeps the NaN that the first pass wrote
+      const float p1 = exp2_fast(fmaf(VT<T>::load(t[e]), a.c, -st.t_max)) * st.t_inv;
+      const float p = isnan(p1) ? p1 : __ull2float_rn(table[col - b0]) * 2.1684043449710089e-19f;
+      const float q = exp2_fast(fmaf(VT<T>::load(z[col]), a.c, -st.z_max)) * st.z_inv;
+      g[col] = VT<T>::store((q - p) * scale);
+    }
+    __syncthreads();
+  }
+}
+
+// Writes zeros to g[c0, c1).
+template <typename T> __device__ void zero_slice(T *g, int64_t n) {
+  const SliceShape<T> sh(g, n);
+  for (int i = threadIdx.x; i < sh.head + sh.tail; i += blockDim.x) {
+    const int64_t j = i < sh.head ? i : n - 1 - (i - sh.head);
+    g[j] = VT<T>::store(0.f);
+  }
+  uint4 *v = reinterpret_cast<uint4 *>(g + sh.head);
+  for (int i = threadIdx.x; i < sh.nvec; i += blockDim.x) __stcs(v + i, make_uint4(0, 0, 0, 0));
+}
+
+// Stores a vector of gradients at g (aligned like the logits or not).
+template <typename T> __device__ __forceinline__ void store_vec(T *g, const float *f, bool aligned) {
+  const uint4 v = Vec<T>::pack(f);
+  if (aligned) {
+    __stcs(reinterpret_cast<uint4 *>(g), v);
+  } else {
+    T e[Vec<T>::n];
+    *reinterpret_cast<uint4 *>(e) = v;
+#pragma unroll
+    for (int i = 0; i < Vec<T>::n; ++i) g[i] = e[i];
+  }
+}
+
+__device__ __forceinline__ void cp_async16(void *smem, const void *gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(gmem)
+               : "memory");
+}
+template <int N> __device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+constexpr int kThreads = 256;
+constexpr int kGroups = 4;  // commit groups of a slice: the sums start when the first quarter is there
+
+// One cluster for each row, one slice of the row for each CTA. KEEP: the slice
+// stays in shared memory and the gradient is written from it; else the forward
+// pass alone, straight from registers.
+template <typename T, typename I, bool KEEP>
+__global__ void __launch_bounds__(kThreads) distill_row_kernel(const DistillArgs a) {
+  extern __shared__ __align__(16) unsigned char dyn[];
+  __shared__ float2 part[kThreads / 32];
+  __shared__ float2 ranks[16];
+  constexpr int N = Vec<T>::n;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int n_ranks = a.n_slices;
+  const int rank = (int)(blockIdx.x % n_ranks);
+  const int64_t row = blockIdx.x / n_ranks;
+  int64_t lo, hi;
+  row_range<I>(a, row, lo, hi);
+  const int64_t c0 = min(a.vocab, (int64_t)rank * a.slice), c1 = min(a.vocab, c0 + a.slice);
+  T *g = KEEP ? static_cast<T *>(a.grad) + row * a.vocab : nullptr;
+  if (lo == hi) {  // every CTA of the cluster leaves
+    if (rank == 0 && threadIdx.x == 0) {
+      a.loss[row] = 0.f;
+      if (a.stats) a.stats[row] = RowStats{0.f, 0.f, 0.f, 0.f};
+    }
+    if (KEEP) zero_slice(g + c0, c1 - c0);
+    return;
+  }
+  const T *z = static_cast<const T *>(a.logits) + row * a.ld;
+  const SliceShape<T> sh(z + c0, c1 - c0);
+  if (n_ranks > 1) cluster.barrier_arrive();  // waited for before the first access to another CTA's memory
+  const uint4 *src = reinterpret_cast<const uint4 *>(z + c0 + sh.head);
+  uint4 *kept = reinterpret_cast<uint4 *>(dyn);
+  const int tid = threadIdx.x;
+
+  MaxSum ms;
+  float loose = 0.f;  // this thread's head or tail element
+  const int64_t loose_col = tid < sh.head ? c0 + tid : c1 - 1 - (tid - sh.head);
+  const bool has_loose = tid < sh.head + sh.tail;
+  if (has_loose) loose = VT<T>::load(z[loose_col]);
+  if (KEEP) {
+    const int per = (sh.nvec + kThreads * kGroups - 1) / (kThreads * kGroups);
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q) {
+      for (int it = q * per; it < (q + 1) * per; ++it) {
+        const int i = tid + it * kThreads;
+        if (i < sh.nvec) cp_async16(kept + i, src + i);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    // each thread reads back only what it copied itself, so its own wait is enough
+    auto take = [&](int q) {
+      for (int it = q * per; it < (q + 1) * per; ++it) {
+        const int i = tid + it * kThreads;
+        if (i < sh.nvec) {
+          float f[N];
+          Vec<T>::unpack(kept[i], f);
+          ms.add<N>(f, a.c);
+        }
+      }
+    };
+    cp_async_wait<3>(), take(0);
+    cp_async_wait<2>(), take(1);
+    cp_async_wait<1>(), take(2);
+    cp_async_wait<0>(), take(3);
+  } else {
+    constexpr int U = 4;  // 16-byte loads in flight for each thread
+    int i = tid;
+    for (; i + (U - 1) * kThreads < sh.nvec; i += U * kThreads) {
+      uint4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = __ldcs(src + i + u * kThreads);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float f[N];
+        Vec<T>::unpack(v[u], f);
+        ms.add<N>(f, a.c);
+      }
+    }
+    for (; i < sh.nvec; i += kThreads) {
+      float f[N];
+      Vec<T>::unpack(__ldcs(src + i), f);
+      ms.add<N>(f, a.c);
+    }
+  }
+  if (has_loose) ms.add<1>(&loose, a.c);
+  MaxSum all = block_join(ms, a.c, part);
+  const MaxSum ts = teacher_stats<T>(a, lo, hi, part);
+  if (n_ranks > 1) {
+    cluster.barrier_wait();
+    if (tid < n_ranks) *cluster.map_shared_rank(&ranks[rank], tid) = make_float2(all.m, all.s);
+    cluster.sync();
+    all = MaxSum();
+    for (int r = 0; r < n_ranks; ++r) all.join(ranks[r].x, ranks[r].y, a.c);
+  }
+  const RowStats st{all.m * a.c, 1.f / all.s, ts.m * a.c, 1.f / ts.s};
+  if (rank == 0) {
+    const float loss = row_loss<T, I>(a, z, lo, hi, st, all.s, ts.s, reinterpret_cast<float *>(part));
+    if (tid == 0) {
+      a.loss[row] = loss;
+      if (a.stats) a.stats[row] = st;
+    }
+  }
+  if (!KEEP) return;
+  const float w = a.cot ? a.cot[row] : 1.f;
+  if (w == 0.f) {
+    zero_slice(g + c0, c1 - c0);
+    return;
+  }
+  const float scale = w * a.temperature;
+  const float qs = st.z_inv * scale;
+  T *dst = g + c0 + sh.head;
+  const bool aligned = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+  for (int i = tid; i < sh.nvec; i += kThreads) {
+    float f[N];
+    Vec<T>::unpack(kept[i], f);
+#pragma unroll
+    for (int u = 0; u < N; ++u) f[u] = exp2_fast(fmaf(f[u], a.c, -st.z_max)) * qs;
+    store_vec(dst + (int64_t)i * N, f, aligned);
+  }
+  if (has_loose) g[loose_col] = VT<T>::store(exp2_fast(fmaf(loose, a.c, -st.z_max)) * qs);
+  __syncthreads();  // the slice in shared memory is done with: its space serves the teacher's entries
+  const int64_t words = (c1 - c0 + 31) / 32 * 4;
+  const int64_t bits_bytes = (words + 15) / 16 * 16;
+  subtract_teacher<T, I>(a, z, g, lo, hi, c0, c1, st, scale, reinterpret_cast<uint32_t *>(dyn),
+                         reinterpret_cast<unsigned long long *>(dyn + bits_bytes),
+                         (a.slice * (int64_t)sizeof(T) - bits_bytes) / 8);
+}
+
+// The backward pass from the forward's statistics: one CTA for each slice.
+constexpr int kBackwardTable = 1024;
+
+template <typename T, typename I>
+__global__ void __launch_bounds__(kThreads) distill_backward_kernel(const DistillArgs a) {
+  extern __shared__ __align__(16) unsigned char dyn[];
+  constexpr int N = Vec<T>::n, U = 4;
+  const int64_t row = blockIdx.x / a.n_slices;
+  const int64_t c0 = (int64_t)(blockIdx.x % a.n_slices) * a.slice, c1 = min(a.vocab, c0 + a.slice);
+  int64_t lo, hi;
+  row_range<I>(a, row, lo, hi);
+  T *g = static_cast<T *>(a.grad) + row * a.vocab;
+  const float w = a.cot ? a.cot[row] : 1.f;
+  if (lo == hi || w == 0.f) {
+    zero_slice(g + c0, c1 - c0);
+    return;
+  }
+  const RowStats st = a.stats[row];
+  const T *z = static_cast<const T *>(a.logits) + row * a.ld;
+  const SliceShape<T> sh(z + c0, c1 - c0);
+  const uint4 *src = reinterpret_cast<const uint4 *>(z + c0 + sh.head);
+  const int tid = threadIdx.x;
+  const float scale = w * a.temperature, qs = st.z_inv * scale;
+  T *dst = g + c0 + sh.head;
+  const bool aligned = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+  auto put = [&](int i, const uint4 &v) {
+    float f[N];
+    Vec<T>::unpack(v, f);
+#pragma unroll
+    for (int u = 0; u < N; ++u) f[u] = exp2_fast(fmaf(f[u], a.c, -st.z_max)) * qs;
+    store_vec(dst + (int64_t)i * N, f, aligned);
+  };
+  int i = tid;
+  for (; i + (U - 1) * kThreads < sh.nvec; i += U * kThreads) {
+    uint4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = __ldcs(src + i + u * kThreads);
+#pragma unroll
+    for (int u = 0; u < U; ++u) put(i + u * kThreads, v[u]);
+  }
+  for (; i < sh.nvec; i += kThreads) put(i, __ldcs(src + i));
+  if (tid < sh.head + sh.tail) {
+    const int64_t col = tid < sh.head ? c0 + tid : c1 - 1 - (tid - sh.head);
+    g[col] = VT<T>::store(exp2_fast(fmaf(VT<T>::load(z[col]), a.c, -st.z_max)) * qs);
+  }
+  unsigned long long *table = reinterpret_cast<unsigned long long *>(dyn);
+  subtract_teacher<T, I>(a, z, g, lo, hi, c0, c1, st, scale, reinterpret_cast<uint32_t *>(table + kBackwardTable),
+                         table, kBackwardTable);
+}
+
+template <typename K>
+void launch_rows(K kernel, const DistillArgs &a, size_t smem, cudaStream_t s) {
+  const int64_t grid = a.rows * a.n_slices;
+  if (grid > INT32_MAX) fail(MSX_ERR_OVERFLOW, "csr_distillation has too many rows for one call.");
+  MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKept));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)a.n_slices;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MSX_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+}
+
+int64_t slice_columns(int64_t vocab, int64_t n) { return ceil_div(ceil_div(vocab, n), 32) * 32; }
+
+// Slices of a row: enough of them that one is at most `most` bytes, and more
+// while the rows alone leave SMs idle and a slice stays above 8 KB.
+int64_t pick_slices(int64_t rows, int64_t row_bytes, int64_t most, int64_t max_slices) {
+  int64_t n = 1;
+  while (n < max_slices && ceil_div(row_bytes, n) > most) n *= 2;
+  while (n < max_slices && rows * n < 2 * num_sms() && row_bytes / n > 16384) n *= 2;
+  return n;
+}
+
+template <typename T, typename I> void run_typed(const DistillCall &call, cudaStream_t s) {
+  DistillArgs a{};
+  a.logits = call.logits, a.ld = call.ld;
+  a.t_data = call.t_data, a.t_idx = call.t_indices, a.t_ptr = call.t_indptr;
+  a.nnz = call.nnz, a.rows = call.rows, a.vocab = call.vocab;
+  a.c = 1.4426950408889634f / call.temperature, a.temperature = call.temperature;
+  a.cot = call.cotangent, a.loss = call.loss, a.stats = static_cast<RowStats *>(call.stats), a.grad = call.grad;
+  if (a.rows == 0) return;
+  const int64_t row_bytes = a.vocab * (int64_t)sizeof(T);
+  auto split = [&](int64_t n) { a.n_slices = (int)n, a.slice = slice_columns(a.vocab, n); };
+  auto backward = [&] {
+    split(pick_slices(a.rows, row_bytes, 65536, 1 << 20));
+    if (a.rows * a.n_slices > INT32_MAX) fail(MSX_ERR_OVERFLOW, "csr_distillation has too many rows for one call.");
+    const size_t smem = kBackwardTable * 8 + (size_t)(a.slice + 31) / 32 * 4;
+    distill_backward_kernel<T, I><<<(unsigned)(a.rows * a.n_slices), kThreads, smem, s>>>(a);
+    MSX_CHECK_LAUNCH();
+  };
+  if (call.loss == nullptr) return backward();
+  if (call.grad == nullptr) {
+    split(pick_slices(a.rows, row_bytes, INT64_MAX, 8));
+    return launch_rows(distill_row_kernel<T, I, false>, a, 0, s);
+  }
+  split(pick_slices(a.rows, row_bytes, 65536, 8));
+  const int64_t kept = a.slice * (int64_t)sizeof(T);
+  if (kept <= kMaxKept) return launch_rows(distill_row_kernel<T, I, true>, a, (size_t)kept, s);
+  // a row that a cluster's shared memory cannot hold: two passes
+  Scratch stats(sizeof(RowStats) * (size_t)a.rows, s);
+  a.stats = stats.as<RowStats>();
+  split(8);
+  void *grad = a.grad;
+  a.grad = nullptr;
+  launch_rows(distill_row_kernel<T, I, false>, a, 0, s);
+  a.grad = grad;
+  backward();
+}
+
+}  // namespace
+
+void distill_run(int value_dtype, int index_dtype, const DistillCall &call, cudaStream_t s) {
+  dispatch_value(value_dtype, [&](auto v) {
+    dispatch_index(index_dtype, [&](auto i) { run_typed<decltype(v), decltype(i)>(call, s); });
+  });
+}
+
+}  // namespace msx

@@ -38,4 +38,45 @@ void csr_transpose_run(int value_dtype, int index_dtype, const void *data, const
 void csr_data_vjp_run(int value_dtype, int index_dtype, const void *indices, const void *indptr, int64_t nnz,
                       int64_t n_rows, const void *rhs, const void *cot, int64_t k, void *out, cudaStream_t s);
 
+// Distillation against a CSR matrix of teacher logits (rows x vocab). With
+// `loss`: the forward pass (`stats`, 16 bytes a row, may be null); with `grad`
+// too: both in one pass; without `loss`: the backward pass from `stats`.
+struct DistillCall {
+  const void *logits;
+  int64_t ld;  // elements between rows of the logits
+  const void *t_data, *t_indices, *t_indptr;
+  int64_t nnz, rows, vocab;
+  float temperature;
+  const float *cotangent;  // per row; null: ones
+  float *loss;
+  void *stats, *grad;
+};
+void distill_run(int value_dtype, int index_dtype, const DistillCall &call, cudaStream_t s);
+
+// Windowed attention. q, k, v: (batch, tokens, heads, dim) with any batch,
+// token and head strides (in elements) and stride 1 along dim; out, grad_out and
+// the gradients are contiguous in that order. lse and delta: float (batch,
+// q_heads, q_len). A null dq (dk and dv) is not computed.
+struct WindowTensor {
+  const void *ptr;
+  int64_t batch, token, head;
+};
+struct WindowCall {
+  WindowTensor q, k, v;
+  const void *grad_out;
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta;
+  int64_t batch, q_len, k_len;
+  int q_heads, k_heads, dim;
+  int64_t window, sinks;
+  float scale;
+  const void *indptr;  // packed sequences (batch 1, q_len = k_len), or null
+  int indptr_dtype;    // of indptr or lengths
+  int64_t n_seq;
+  const void *lengths;  // keys of each batch entry (type indptr_dtype), or null: k_len
+};
+void window_forward_run(int value_dtype, const WindowCall &c, cudaStream_t s);
+void window_decode_run(int value_dtype, const WindowCall &c, cudaStream_t s);
+void window_backward_run(int value_dtype, const WindowCall &c, cudaStream_t s);
+
 }  // namespace msx

@@ -8,6 +8,7 @@ place of MLX arrays. Every product runs in the hand-written CUDA library
 """
 
 from mlx_sparse import linalg
+from mlx_sparse._attention import window_attention, window_attention_decode
 from mlx_sparse._coo import COOArray, coo_array
 from mlx_sparse._csr import CSRArray, csr_array
 from mlx_sparse._native import check_device_errors, extension, library_path
@@ -17,6 +18,8 @@ from mlx_sparse._ops import (
     coo_matvec,
     csr_batched_matmul,
     csr_batched_matvec,
+    csr_distillation_loss,
+    csr_distillation_loss_and_grad,
     csr_matmat,
     csr_matmul,
     csr_matmul_data_vjp,
@@ -41,6 +44,8 @@ __all__ = [
     "csr_matmat",
     "csr_batched_matmul",
     "csr_batched_matvec",
+    "csr_distillation_loss",
+    "csr_distillation_loss_and_grad",
     "csr_matmul",
     "csr_matmul_data_vjp",
     "csr_matmul_streamed",
@@ -51,4 +56,6 @@ __all__ = [
     "extension",
     "library_path",
     "linalg",
+    "window_attention",
+    "window_attention_decode",
 ]

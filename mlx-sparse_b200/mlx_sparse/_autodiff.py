@@ -49,3 +49,46 @@ class CsrProduct(torch.autograd.Function):
             else:
                 g_rhs = _native.csr_matmul(t_data, indices, indptr, grad, t_shape)
         return g_data, g_rhs, None
+
+
+class CsrDistillation(torch.autograd.Function):
+    """Per-row distillation losses, differentiable once in the logits; the
+    teacher is a constant. The forward pass keeps four numbers a row, the
+    backward pass reads the logits again."""
+
+    @staticmethod
+    def forward(ctx, logits, a, temperature):
+        loss, stats = _native.csr_distill_forward(a.data, a.indices, a.indptr, logits, temperature, with_stats=True)
+        ctx.a, ctx.temperature = a, temperature
+        ctx.save_for_backward(logits, stats)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        logits, stats = ctx.saved_tensors
+        a = ctx.a
+        return (_native.csr_distill_backward(a.data, a.indices, a.indptr, logits, ctx.temperature, stats, grad), None,
+                None)
+
+
+class WindowAttention(torch.autograd.Function):
+    """Windowed attention on rank-4 operands, differentiable once in ``q``,
+    ``k`` and ``v``. Keeps the output and each row's log-sum-exp."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, scale, indptr):
+        out, lse = _native.window_attention_forward(q, k, v, window, sinks, scale, indptr, with_lse=True)
+        ctx.args = (window, sinks, scale, indptr)
+        ctx.save_for_backward(q, k, v, out, lse)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        q, k, v, out, lse = ctx.saved_tensors
+        need_q, need_kv = ctx.needs_input_grad[0], any(ctx.needs_input_grad[1:3])
+        dq, dk, dv = _native.window_attention_backward(q, k, v, out, lse, grad, *ctx.args, want_q=need_q,
+                                                       want_kv=need_kv)
+        return (dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None,
+                None)

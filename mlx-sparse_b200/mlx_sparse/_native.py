@@ -85,6 +85,15 @@ def extension():
                                               p]
         L.msx_diagonal_preconditioner_apply.argtypes = [p, p, i64, i64, p, p]
         L.msx_csr_gershgorin_bounds.argtypes = [c_int, p, p, p, i64, i64, i64, p, p]
+        distill = [c_int, c_int, p, p, p, i64, p, i64, i64, i64, c_float]
+        L.msx_csr_distill_forward.argtypes = distill + [p, p, p]
+        L.msx_csr_distill_backward.argtypes = distill + [p, p, p, p]
+        L.msx_csr_distill_forward_backward.argtypes = distill + [p, p, p, p]
+        window = [c_int, p, p, p, p, p, p, i64, i64, i64, i64, i64, i64, i64, i64, c_float, c_int, p, i64]
+        L.msx_window_attention_forward.argtypes = window + [p, p, p]
+        L.msx_window_attention_backward.argtypes = window + [p, p, p, p, p, p, p, p]
+        L.msx_window_attention_decode.argtypes = [c_int, p, p, p, p, p, p, i64, i64, i64, i64, i64, i64, i64, c_float,
+                                                  c_int, p, p, p]
         L.msx_cg_context_create.argtypes = [c_int, p, p, p, i64, i64, i64, c_int, c_int, c_int, c_int, p, c_int, p,
                                             p, p, p, p, p, ctypes.POINTER(p)]
         L.msx_cg_context_ipc_handles.argtypes = [p, p, i64]
@@ -529,3 +538,129 @@ def csr_gershgorin_bounds(data, indices, indptr, shape):
         check(L.msx_csr_gershgorin_bounds(INDEX_CODES[indices.dtype], _p(data), _p(indices), _p(indptr),
                                           data.numel(), shape[0], shape[1], out, stream_ptr(dev)))
     return tuple(float(v) for v in out)
+
+
+def _distill_args(data, indices, indptr, logits, temperature):
+    return [VALUE_CODES[data.dtype], INDEX_CODES[indices.dtype], _p(data), _p(indices), _p(indptr), data.numel(),
+            _p(logits), logits.stride(0) if logits.shape[0] > 1 else logits.shape[1], logits.shape[0], logits.shape[1],
+            float(temperature)]
+
+
+def rows_of(t):
+    """``t`` (rank 2) with stride 1 along its rows and rows that do not
+    overlap; copied only where it has not."""
+    return t if t.stride(1) == 1 and (t.shape[0] < 2 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def csr_distill_forward(data, indices, indptr, logits, temperature, *, with_stats: bool):
+    """Per-row losses and, with ``with_stats``, what the backward call needs."""
+    L = extension()
+    dev = require_cuda(data, indices, indptr, logits)
+    data, indices, indptr, logits = data.contiguous(), indices.contiguous(), indptr.contiguous(), rows_of(logits)
+    loss = torch.empty(logits.shape[0], dtype=torch.float32, device=dev)
+    stats = torch.empty((logits.shape[0], 4), dtype=torch.float32, device=dev) if with_stats else None
+    with torch.cuda.device(dev):
+        check(L.msx_csr_distill_forward(*_distill_args(data, indices, indptr, logits, temperature), _p(loss),
+                                        _p(stats), stream_ptr(dev)))
+    return loss, stats
+
+
+def csr_distill_backward(data, indices, indptr, logits, temperature, stats, cotangent):
+    L = extension()
+    dev = require_cuda(data, indices, indptr, logits, stats, cotangent)
+    data, indices, indptr, logits = data.contiguous(), indices.contiguous(), indptr.contiguous(), rows_of(logits)
+    cotangent = cotangent.contiguous()
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    with torch.cuda.device(dev):
+        check(L.msx_csr_distill_backward(*_distill_args(data, indices, indptr, logits, temperature), _p(stats),
+                                         _p(cotangent), _p(grad), stream_ptr(dev)))
+    return grad
+
+
+def csr_distill_forward_backward(data, indices, indptr, logits, temperature, cotangent=None):
+    L = extension()
+    dev = require_cuda(data, indices, indptr, logits, *(() if cotangent is None else (cotangent,)))
+    data, indices, indptr, logits = data.contiguous(), indices.contiguous(), indptr.contiguous(), rows_of(logits)
+    cotangent = None if cotangent is None else cotangent.contiguous()
+    loss = torch.empty(logits.shape[0], dtype=torch.float32, device=dev)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    with torch.cuda.device(dev):
+        check(L.msx_csr_distill_forward_backward(*_distill_args(data, indices, indptr, logits, temperature),
+                                                 _p(cotangent), _p(loss), _p(grad), stream_ptr(dev)))
+    return loss, grad
+
+
+def _strides(t, dims):
+    """Element strides of ``t`` along ``dims`` as a C array; a dimension of
+    one element (or none) has the stride a contiguous tensor would have."""
+    out, span = {}, 1
+    for d in range(t.ndim - 1, -1, -1):
+        out[d] = t.stride(d) if t.shape[d] > 1 else span
+        span *= max(1, t.shape[d])
+    return (ctypes.c_int64 * len(dims))(*(out[d] for d in dims))
+
+
+def heads_of(t):
+    """``t`` (..., heads, dim) as the attention kernels read it: stride 1 along
+    dim. 16-bit tensors whose rows start on 16-byte boundaries go to the
+    tensor cores as they are; others (and broadcast ones) are copied."""
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        return t.contiguous()
+    if t.element_size() == 2 and t.shape[-1] % 8 == 0 and t.numel():
+        loose = any(t.shape[d] > 1 and (t.stride(d) % 8 or t.stride(d) == 0) for d in range(t.ndim - 1))
+        if loose or t.data_ptr() % 16:
+            return t.contiguous() if loose or not t.is_contiguous() else t.clone()
+    return t
+
+
+def _window_args(q, k, v, window, sinks, scale, indptr):
+    b, q_len, q_heads, dim = q.shape
+    qs, ks, vs = (_strides(t, (0, 1, 2)) for t in (q, k, v))
+    return [VALUE_CODES[q.dtype], _p(q), qs, _p(k), ks, _p(v), vs, b, q_len, k.shape[1], q_heads, k.shape[2], dim,
+            int(window), int(sinks), float(scale), INDEX_CODES[indptr.dtype] if indptr is not None else MSX_I32,
+            _p(indptr), indptr.numel() - 1 if indptr is not None else 0]
+
+
+def window_attention_forward(q, k, v, window, sinks, scale, indptr=None, *, with_lse: bool):
+    """Rank-4 ``q``, ``k``, ``v``; returns ``(out, lse)`` (lse None unless wanted)."""
+    L = extension()
+    dev = require_cuda(q, k, v, *(() if indptr is None else (indptr,)))
+    q, k, v = heads_of(q), heads_of(k), heads_of(v)
+    indptr = None if indptr is None else indptr.contiguous()
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=dev) if with_lse else None
+    with torch.cuda.device(dev):
+        check(L.msx_window_attention_forward(*_window_args(q, k, v, window, sinks, scale, indptr), _p(out), _p(lse),
+                                             stream_ptr(dev)))
+    return out, lse
+
+
+def window_attention_backward(q, k, v, out, lse, grad, window, sinks, scale, indptr=None, *, want_q=True,
+                              want_kv=True):
+    L = extension()
+    dev = require_cuda(q, k, v, out, lse, grad, *(() if indptr is None else (indptr,)))
+    q, k, v = heads_of(q), heads_of(k), heads_of(v)
+    indptr = None if indptr is None else indptr.contiguous()
+    grad = heads_of(grad.contiguous())
+    delta = torch.empty_like(lse)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if want_q else None
+    dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=dev) if want_kv else None for _ in range(2))
+    with torch.cuda.device(dev):
+        check(L.msx_window_attention_backward(*_window_args(q, k, v, window, sinks, scale, indptr), _p(out), _p(lse),
+                                              _p(grad), _p(delta), _p(dq), _p(dk), _p(dv), stream_ptr(dev)))
+    return dq, dk, dv
+
+
+def window_attention_decode(q, k_cache, v_cache, lengths, window, sinks, scale):
+    L = extension()
+    dev = require_cuda(q, k_cache, v_cache, lengths)
+    q, k_cache, v_cache, lengths = heads_of(q), heads_of(k_cache), heads_of(v_cache), lengths.contiguous()
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    b, q_heads, dim = q.shape
+    with torch.cuda.device(dev):
+        check(L.msx_window_attention_decode(VALUE_CODES[q.dtype], _p(q), _strides(q, (0, 1)), _p(k_cache),
+                                            _strides(k_cache, (0, 1, 2)), _p(v_cache), _strides(v_cache, (0, 1, 2)), b,
+                                            k_cache.shape[1], q_heads, k_cache.shape[2], dim, int(window), int(sinks),
+                                            float(scale), INDEX_CODES[lengths.dtype], _p(lengths), _p(out),
+                                            stream_ptr(dev)))
+    return out

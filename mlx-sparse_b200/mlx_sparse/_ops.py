@@ -18,6 +18,7 @@ from mlx_sparse._validation import (
     ensure_array,
     validate_csr_matmul_inputs,
     validate_csr_matvec_inputs,
+    validate_distillation_inputs,
 )
 
 
@@ -193,6 +194,62 @@ def csr_matmul_data_vjp(a: CSRArray, rhs, cotangent):
     if cotangent.shape != (a.shape[0], rhs.shape[1]):
         raise ValueError("csr_matmul_data_vjp cotangent must have shape (n_rows, rhs_cols).")
     return _native.csr_data_vjp(a.indices, a.indptr, rhs, cotangent, a.shape)
+
+
+# ---------------------------------------------------------------------------
+# Distillation against a teacher's stored top logits
+# ---------------------------------------------------------------------------
+def csr_distillation_loss(teacher: CSRArray, logits, *, temperature: float = 1.0):
+    """Per-row loss of dense student ``logits`` (tokens x vocabulary) against
+    a CSR matrix of a teacher's top logits, a float32 vector.
+
+    With ``p`` the softmax of a row's stored entries over ``temperature`` and
+    ``q`` the softmax of the student's whole row over it::
+
+        loss = temperature**2 * sum_e p_e * (log p_e - log q[col_e])
+        dloss/dlogits = temperature * (q - p)
+
+    A row without entries (a prompt, padding) has loss 0 and gradient 0
+    whatever its logits hold. Entries need no order; several of one column are
+    terms of their own. Entries with ``-inf`` teacher logits add nothing. A
+    column outside the vocabulary makes its row's loss NaN.
+
+    Differentiable (once) in ``logits``; the teacher is a constant. ``logits``
+    may have any row stride; a stride other than 1 along the vocabulary is
+    copied. Use ``csr_distillation_loss_and_grad`` where the losses' weights
+    are known beforehand: it reads the logits once instead of twice.
+    """
+    if not isinstance(teacher, CSRArray):
+        raise TypeError(f"csr_distillation_loss expects CSRArray, got {type(teacher).__name__}.")
+    logits = ensure_array(logits, device=teacher.device)
+    validate_distillation_inputs(teacher.data, teacher.indices, teacher.indptr, logits, teacher.shape, temperature)
+    if _wants_grad(logits):
+        from mlx_sparse._autodiff import CsrDistillation
+
+        return CsrDistillation.apply(logits, teacher, float(temperature))
+    return _native.csr_distill_forward(teacher.data, teacher.indices, teacher.indptr, logits, temperature,
+                                       with_stats=False)[0]
+
+
+def csr_distillation_loss_and_grad(teacher: CSRArray, logits, *, cotangent=None, temperature: float = 1.0):
+    """``(loss, grad)`` of ``csr_distillation_loss`` in one pass over the
+    logits: the per-row losses (unweighted, float32) and the gradient of
+    ``sum(cotangent * loss)`` in the logits' dtype. ``cotangent`` is a float32
+    vector, one weight for each row (None: ones); a row of weight 0 gets
+    gradient 0 whatever its logits hold. No autograd graph is recorded."""
+    if not isinstance(teacher, CSRArray):
+        raise TypeError(f"csr_distillation_loss_and_grad expects CSRArray, got {type(teacher).__name__}.")
+    logits = ensure_array(logits, device=teacher.device).detach()
+    validate_distillation_inputs(teacher.data, teacher.indices, teacher.indptr, logits, teacher.shape, temperature)
+    if cotangent is not None:
+        cotangent = ensure_array(cotangent, device=teacher.device).detach()
+        if cotangent.shape != (teacher.shape[0],):
+            raise ValueError(f"csr_distillation cotangent must have shape ({teacher.shape[0]},), "
+                             f"got {tuple(cotangent.shape)}.")
+        if cotangent.dtype != torch.float32:
+            raise TypeError(f"csr_distillation cotangent must be float32, got {cotangent.dtype}.")
+    return _native.csr_distill_forward_backward(teacher.data, teacher.indices, teacher.indptr, logits, temperature,
+                                                cotangent)
 
 
 # ---------------------------------------------------------------------------

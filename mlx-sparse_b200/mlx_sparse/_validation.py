@@ -151,3 +151,52 @@ def validate_csr_matmul_inputs(data, indices, indptr, rhs, shape) -> None:
             "csr_matmul requires sparse data and RHS to have the same dtype, "
             f"got {_dtype_name(data.dtype)} and {_dtype_name(rhs.dtype)}."
         )
+
+
+def validate_distillation_inputs(data, indices, indptr, logits, shape, temperature) -> None:
+    validate_csr_metadata(data, indices, indptr, shape)
+    if logits.ndim != 2 or tuple(logits.shape) != tuple(shape):
+        raise ValueError(
+            f"csr_distillation logits must have the teacher's shape {tuple(shape)}, got {tuple(logits.shape)}."
+        )
+    check_value_dtype("csr_distillation logits", logits)
+    if data.dtype != logits.dtype:
+        raise TypeError(
+            "csr_distillation requires teacher data and logits to have the same dtype, "
+            f"got {_dtype_name(data.dtype)} and {_dtype_name(logits.dtype)}."
+        )
+    if data.requires_grad:
+        raise ValueError("csr_distillation takes the teacher as a constant; detach its data first.")
+    if not (0.0 < float(temperature) < float("inf")):
+        raise ValueError(f"csr_distillation temperature must be positive and finite, got {temperature}.")
+
+
+def validate_window_inputs(q, k, v, window, sinks, scale, *, rank, name) -> float:
+    """Shapes and types of windowed attention; returns the scale to use."""
+    if q.ndim != rank or k.ndim != rank or v.ndim != rank:
+        raise ValueError(f"{name} got q of shape {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)}.")
+    for label, t in (("q", q), ("k", k), ("v", v)):
+        check_value_dtype(f"{name} {label}", t)
+    if not q.dtype == k.dtype == v.dtype:
+        raise TypeError(
+            f"{name} requires q, k and v to have the same dtype, "
+            f"got {_dtype_name(q.dtype)}, {_dtype_name(k.dtype)} and {_dtype_name(v.dtype)}."
+        )
+    if k.shape != v.shape:
+        raise ValueError(f"{name} k and v must have the same shape, got {tuple(k.shape)} and {tuple(v.shape)}.")
+    dim = int(q.shape[-1])
+    if k.shape[-1] != dim:
+        raise ValueError(f"{name} q and k must have the same head size, got {dim} and {k.shape[-1]}.")
+    if not 1 <= dim <= 256:
+        raise ValueError(f"{name} head size must be between 1 and 256, got {dim}.")
+    if q.shape[-2] == 0 or k.shape[-2] == 0 or q.shape[-2] % k.shape[-2]:
+        raise ValueError(f"{name} query heads must be a multiple of key heads, got {q.shape[-2]} and {k.shape[-2]}.")
+    for label, n in (("window", window), ("sinks", sinks)):
+        if isinstance(n, bool) or not isinstance(n, (int, np.integer)):
+            raise TypeError(f"{name} {label} must be an integer, got {n!r}.")
+        if n < 0:
+            raise ValueError(f"{name} {label} must be non-negative, got {n}.")
+    scale = float(dim) ** -0.5 if scale is None else float(scale)
+    if not np.isfinite(scale):
+        raise ValueError(f"{name} scale must be finite, got {scale}.")
+    return scale
