@@ -91,6 +91,10 @@ int msx_check_device_errors(void *stream) {
       fail(MSX_ERR_RUNTIME,
            "an SpMV bulk-copy wait on this device gave up (poll limit reached); the results of SpMV calls "
            "made since the last check are incomplete.");
+    if (window_take_error())
+      fail(MSX_ERR_RUNTIME,
+           "a windowed-attention kernel's wait on this device gave up; the results of window_attention calls made "
+           "since the last check are incomplete.");
   });
 }
 

@@ -77,6 +77,7 @@ struct WindowCall {
 };
 void window_forward_run(int value_dtype, const WindowCall &c, cudaStream_t s);
 void window_decode_run(int value_dtype, const WindowCall &c, cudaStream_t s);
+bool window_take_error();  // reads and clears the device's wait error flag
 void window_backward_run(int value_dtype, const WindowCall &c, cudaStream_t s);
 
 }  // namespace msx

@@ -38,39 +38,6 @@ __device__ __forceinline__ float dot(const float *a, const float *b, int dim) {
   return s;
 }
 
-// The tiles of keys that any row of a block of queries sees: those of its band
-// [low, last], preceded by the sink keys of its first sequence that lie before
-// the band (a sequence that starts inside the block has its own in the band).
-struct KeyTiles {
-  int sink0, n_sink, band0, n;
-  __device__ KeyTiles(const WindowProblem &w, int b, int i0, int rows, int tile) {
-    sink0 = n_sink = band0 = n = 0;
-    int low = INT_MAX, last = -1;
-    bool any = false;
-    for (int i = i0; i < i0 + rows && i < w.c.q_len; ++i) {
-      const QuerySpan s = query_span(w, b, i);
-      if (s.p < 0) continue;
-      if (!any) {
-        any = true;
-        sink0 = s.start;
-        n_sink = s.sink_end - s.start;
-      }
-      low = min(low, s.low), last = max(last, s.p);
-    }
-    if (!any) return;
-    n_sink = max(0, min(n_sink, low - sink0));
-    n_sink = (n_sink + tile - 1) / tile;
-    band0 = low;
-    n = n_sink + (last - low + tile) / tile;
-  }
-  __device__ int first(int t, int tile) const { return t < n_sink ? sink0 + t * tile : band0 + (t - n_sink) * tile; }
-  // the end of the tile's own keys: a sink tile stops where the band begins
-  __device__ int end(int t, int tile) const {
-    const int e = first(t, tile) + tile;
-    return t < n_sink ? min(e, band0) : e;
-  }
-};
-
 template <typename T> __global__ void __launch_bounds__(kWarps * 32) forward_kernel(const WindowProblem w) {
   extern __shared__ float sm[];
   const int dim = w.c.dim, ks = dim + 1;
@@ -81,7 +48,7 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) forward_ker
   const T *k = static_cast<const T *>(w.c.k.ptr) + b * w.c.k.batch + hk * w.c.k.head;
   const T *v = static_cast<const T *>(w.c.v.ptr) + b * w.c.v.batch + hk * w.c.v.head;
   load_rows(sq, dim, q, w.c.q.token, i0, (int)w.c.q_len, kRows, dim);
-  const KeyTiles tiles(w, b, i0, kRows, kTile);
+  const KeyTiles<kTile> tiles(key_range(w, b, i0, i0 + kRows - 1));
   QuerySpan span[kRowsPerWarp];
   float m[kRowsPerWarp], l[kRowsPerWarp], acc[kRowsPerWarp][kRegs];
 #pragma unroll
@@ -92,7 +59,7 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) forward_ker
     for (int x = 0; x < kRegs; ++x) acc[r][x] = 0.f;
   }
   for (int t = 0; t < tiles.n; ++t) {
-    const int j0 = tiles.first(t, kTile), j = j0 + lane, end = tiles.end(t, kTile);
+    const int j0 = tiles.first(t), j = j0 + lane, end = tiles.end(t);
     __syncthreads();
     load_rows(sk, ks, k, w.c.k.token, j0, (int)w.c.k_len, kTile, dim);
     load_rows(sv, ks, v, w.c.v.token, j0, (int)w.c.k_len, kTile, dim);
@@ -174,7 +141,7 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) dq_kernel(c
   load_rows(sq, dim, q, w.c.q.token, i0, (int)w.c.q_len, kRows, dim);
   load_rows(sg, dim, static_cast<const T *>(w.c.grad_out) + head0, (int64_t)w.c.q_heads * dim, i0, (int)w.c.q_len,
             kRows, dim);
-  const KeyTiles tiles(w, b, i0, kRows, kTile);
+  const KeyTiles<kTile> tiles(key_range(w, b, i0, i0 + kRows - 1));
   QuerySpan span[kRowsPerWarp];
   float lse[kRowsPerWarp], delta[kRowsPerWarp], acc[kRowsPerWarp][kRegs];
 #pragma unroll
@@ -188,7 +155,7 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) dq_kernel(c
     for (int x = 0; x < kRegs; ++x) acc[r][x] = 0.f;
   }
   for (int t = 0; t < tiles.n; ++t) {
-    const int j0 = tiles.first(t, kTile), j = j0 + lane, end = tiles.end(t, kTile);
+    const int j0 = tiles.first(t), j = j0 + lane, end = tiles.end(t);
     __syncthreads();
     load_rows(sk, ks, k, w.c.k.token, j0, (int)w.c.k_len, kTile, dim);
     load_rows(sv, ks, v, w.c.v.token, j0, (int)w.c.k_len, kTile, dim);
@@ -344,7 +311,11 @@ static WindowProblem problem(const WindowCall &c) {
 }
 
 void window_forward_run(int value_dtype, const WindowCall &c, cudaStream_t s) {
-  window_forward_general(problem(c), value_dtype, s);
+  const WindowProblem w = problem(c);
+  if (window_tc_ok(w, value_dtype))
+    window_forward_tc(w, value_dtype, s);
+  else
+    window_forward_general(w, value_dtype, s);
 }
 
 void window_decode_run(int value_dtype, const WindowCall &c, cudaStream_t s) {

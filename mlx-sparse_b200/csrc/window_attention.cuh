@@ -69,6 +69,52 @@ __device__ __forceinline__ QuerySpan query_span(const WindowProblem &w, int b, i
   return s;
 }
 
+// The keys that the queries [first, last] see: [low, end) and, before it, the
+// sink keys [sink0, sink_end) of the first query's sequence. (A sequence that
+// starts further on has its sinks in [low, end).) Positions rise with the
+// queries and so do the lower ends of their bands, so the ends decide.
+struct KeyRange {
+  int sink0, sink_end, low, end;
+  __device__ __forceinline__ bool empty() const { return end <= low && sink_end <= sink0; }
+  __device__ __forceinline__ bool touches(int j0, int j1) const {
+    return (j0 < end && j1 > low && end > low) || (j0 < sink_end && j1 > sink0);
+  }
+};
+
+__device__ __forceinline__ KeyRange key_range(const WindowProblem &w, int b, int first, int last) {
+  const int shift = key_count(w, b) - (int)w.c.q_len;
+  int64_t lo = max(first, max(0, -shift)), hi = min(last, (int)w.c.q_len - 1);
+  if (w.c.indptr != nullptr) {
+    const int64_t n = w.c.n_seq;
+    auto at = [&](int64_t r) -> int64_t {
+      return w.wide_ptr ? static_cast<const int64_t *>(w.c.indptr)[r]
+                        : (int64_t) static_cast<const int32_t *>(w.c.indptr)[r];
+    };
+    lo = max(lo, at(0)), hi = min(hi, at(n) - 1);
+  }
+  KeyRange r{0, 0, 0, 0};
+  if (lo > hi) return r;
+  const QuerySpan s = query_span(w, b, (int)lo);
+  if (s.p < 0) return r;
+  r.low = s.low, r.end = (int)hi + shift + 1;
+  r.sink0 = s.start, r.sink_end = max(s.start, min(s.start + w.sinks, s.low));
+  return r;
+}
+
+// A range as tiles of N keys: the sink keys' tiles, then the band's.
+template <int N> struct KeyTiles {
+  int sink0, low, n_sink, n;
+  __device__ __forceinline__ explicit KeyTiles(const KeyRange &r)
+      : sink0(r.sink0), low(r.low), n_sink((r.sink_end - r.sink0 + N - 1) / N),
+        n(n_sink + (max(r.end - r.low, 0) + N - 1) / N) {}
+  __device__ __forceinline__ int first(int t) const { return t < n_sink ? sink0 + t * N : low + (t - n_sink) * N; }
+  // end of the tile's own keys: a sink tile stops where the band begins
+  __device__ __forceinline__ int end(int t) const {
+    const int e = first(t) + N;
+    return t < n_sink ? min(e, low) : e;
+  }
+};
+
 // The query positions that see one key: [j, last]; nothing if last < j.
 __device__ __forceinline__ int last_query(const WindowProblem &w, int j) {
   if (j >= w.c.k_len) return -1;
@@ -81,5 +127,9 @@ __device__ __forceinline__ int last_query(const WindowProblem &w, int j) {
 // Kernels for every type and head size (window_attention.cu) ...
 void window_forward_general(const WindowProblem &w, int value_dtype, cudaStream_t s);
 void window_backward_general(const WindowProblem &w, int value_dtype, cudaStream_t s);
+// ... and for the tensor cores (window_forward_tc.cu).
+bool window_tc_ok(const WindowProblem &w, int value_dtype);
+void window_forward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s);
+int *window_error_flag();
 
 }  // namespace msx

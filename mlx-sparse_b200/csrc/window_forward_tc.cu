@@ -1,0 +1,571 @@
+// Windowed attention, forward, on the tensor cores (float16 / bfloat16, head
+// sizes that are multiples of 8 up to 128).
+//
+// A persistent CTA takes work items of two "slots" of 128 queries each: two
+// heads that share a key head, or two neighbouring query tiles of one head where
+// the group is odd. It walks the tiles of 128 keys that they see, the sink
+// tiles and then the band's, and no others. One warp loads Q, K and V tiles by
+// TMA into a ring of shared memory; one thread issues tcgen05.mma; a warpgroup
+// for each slot does its softmax, a query row for each thread, straight from
+// tensor memory. Scores and output of a slot stay in tensor memory (S 128
+// columns, O 128 columns, two slots: all 512); the probabilities, rounded to the
+// inputs' type for the second product (half a step each, against sums held in
+// fp32), take the place of the scores and are read from there as its left
+// operand. While one slot's softmax runs, the other slot's two products do.
+//
+// The running maximum is only raised when a row's new maximum is 2^8 above the
+// one in use, so the output is rescaled in tensor memory a few times at most;
+// the probabilities stay below 2^8 and the sum is of the same unrounded values.
+//
+// A masked score is -inf before the softmax, whatever it was. Its probability
+// is 0, but 0 times an infinite or NaN value row would still reach the second
+// product: rows that end not finite are computed again pair by pair.
+//
+// Bound: the exponentials (16 a clock and SM: 1024 clocks for 128 x 128 scores)
+// and the products (2 x 512 clocks at head size 128) take the same time, side
+// by side.
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+
+#include "tc.cuh"
+#include "window_attention.cuh"
+
+namespace msx {
+
+using namespace tc;
+
+namespace {
+
+__device__ int g_window_error;
+
+constexpr int kM = 128;  // queries of a slot: the lanes of tensor memory
+constexpr int kN = 128;  // keys of a tile
+constexpr int kThreads = 384;
+constexpr int kBox = 128 * 128;  // bytes of a TMA box: 128 rows of 64 elements
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int DB> struct Shape {  // DB boxes of 64 elements cover the head size
+  static constexpr int tile = DB * kBox;
+  static constexpr int stages = DB == 2 ? 5 : 8;
+  static constexpr int smem = 1024 + (2 + stages) * tile;
+};
+
+struct Bars {
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
+  uint64_t kv_full[8], kv_empty[8];
+  uint32_t tmem;
+  int stop;
+};
+
+struct Params {
+  WindowProblem w;
+  CUtensorMap q, k, v;
+  int64_t items;
+  int q_tiles, paired;
+  int *error;
+};
+
+// One work item: the two slots' heads and first queries, and the keys of each
+// and of both.
+struct Item {
+  int b, hk, head[2], i0[2];
+  KeyRange range[2], both;
+  int last[2];  // the last tile of keys that a slot takes part in, -1: none
+};
+
+__device__ __forceinline__ Item item_of(const Params &p, int64_t n) {
+  const WindowProblem &w = p.w;
+  Item it;
+  if (p.paired) {
+    const int pairs = w.group / 2;
+    const int pair = (int)(n % pairs);
+    n /= pairs;
+    it.i0[0] = it.i0[1] = (int)(n % p.q_tiles) * kM;
+    n /= p.q_tiles;
+    it.hk = (int)(n % w.c.k_heads);
+    it.b = (int)(n / w.c.k_heads);
+    it.head[0] = it.hk * w.group + 2 * pair;
+    it.head[1] = it.head[0] + 1;
+    it.both = it.range[0] = it.range[1] = key_range(w, it.b, it.i0[0], it.i0[0] + kM - 1);
+    it.last[0] = it.last[1] = KeyTiles<kN>(it.both).n - 1;
+  } else {
+    const int blocks = (p.q_tiles + 1) / 2;
+    const int h = (int)(n / blocks % w.c.q_heads);
+    it.b = (int)(n / blocks / w.c.q_heads);
+    it.hk = h / w.group;
+    it.head[0] = it.head[1] = h;
+    it.i0[0] = (int)(n % blocks) * 2 * kM;
+    it.i0[1] = it.i0[0] + kM;
+    it.both = key_range(w, it.b, it.i0[0], it.i0[1] + kM - 1);
+    const KeyTiles<kN> tiles(it.both);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      it.range[s] = key_range(w, it.b, it.i0[s], it.i0[s] + kM - 1);
+      it.last[s] = it.range[s].empty() ? -1 : tiles.n - 1;
+      while (it.last[s] >= 0 && !it.range[s].touches(tiles.first(it.last[s]), tiles.end(it.last[s]))) --it.last[s];
+    }
+  }
+  return it;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two fp32 operations for one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n"
+      " mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Bits [lo, hi) of the 32 that start at bit `from`.
+__device__ __forceinline__ uint32_t bits(int lo, int hi, int from) {
+  lo = max(lo - from, 0), hi = min(hi - from, 32);
+  return hi <= lo ? 0u : (~0u >> (32 - hi)) & (~0u << lo);
+}
+
+// One row again, by a warp, pair by pair: only what the query sees is touched.
+template <typename T>
+__device__ __noinline__ void repair_row(const WindowProblem &w, int b, int h, int i) {
+  const int lane = threadIdx.x & 31, dim = w.c.dim, hk = h / w.group;
+  const T *q = static_cast<const T *>(w.c.q.ptr) + b * w.c.q.batch + h * w.c.q.head + i * w.c.q.token;
+  const T *k = static_cast<const T *>(w.c.k.ptr) + b * w.c.k.batch + hk * w.c.k.head;
+  const T *v = static_cast<const T *>(w.c.v.ptr) + b * w.c.v.batch + hk * w.c.v.head;
+  const QuerySpan span = query_span(w, b, i);
+  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int part = 0; part < 2; ++part) {
+    const int from = part ? span.low : span.start, end = part ? span.p + 1 : span.sink_end;
+    for (int j0 = from; j0 < end; j0 += 32) {
+      const int j = j0 + lane;
+      float s = -INFINITY;
+      if (j < end) {
+        s = 0.f;
+        for (int d = 0; d < dim; ++d) s = fmaf(VT<T>::load(q[d]), VT<T>::load(k[j * w.c.k.token + d]), s);
+        s *= w.c.scale * kLog2e;
+      }
+      float top = s;
+#pragma unroll
+      for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+      top = fmaxf(top, m);
+      const float base = top == -INFINITY ? 0.f : top, keep = exp2f(m - base);
+      const float p = j < end ? exp2f(s - base) : 0.f;
+      float sum = p;
+#pragma unroll
+      for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
+      l = l * keep + sum, m = top;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) acc[x] *= keep;
+      for (int kk = 0; kk < min(32, end - j0); ++kk) {
+        const float pk = __shfl_sync(~0u, p, kk);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (x * 32 + lane < dim) acc[x] = fmaf(pk, VT<T>::load(v[(j0 + kk) * w.c.v.token + x * 32 + lane]), acc[x]);
+      }
+    }
+  }
+  T *out = static_cast<T *>(w.c.out) + ((b * w.c.q_len + i) * w.c.q_heads + h) * dim;
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    if (x * 32 + lane < dim) out[x * 32 + lane] = VT<T>::store(acc[x] / l);
+  if (w.c.lse && lane == 0) w.c.lse[((int64_t)b * w.c.q_heads + h) * w.c.q_len + i] = m + log2f(l);
+}
+
+template <typename T, int DB>
+__global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_constant__ Params p) {
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  using Sh = Shape<DB>;
+  extern __shared__ unsigned char raw[];
+  unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  __shared__ Bars bars;
+  unsigned char *q_tile = sm, *kv_tile = sm + 2 * Sh::tile;
+  const WindowProblem &w = p.w;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int *stop = &bars.stop;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      bar_init(&bars.q_full[s], 1), bar_init(&bars.q_empty[s], 1);
+      bar_init(&bars.s_full[s], 1), bar_init(&bars.p_full[s], 4), bar_init(&bars.o_full[s], 1);
+    }
+    for (int s = 0; s < Sh::stages; ++s) bar_init(&bars.kv_full[s], 1), bar_init(&bars.kv_empty[s], 1);
+    bars.stop = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) tmem_alloc(&bars.tmem, 512);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = bars.tmem;
+  if (warp == 0) {
+    // ---- loads -------------------------------------------------------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 1, q_phase[2] = {1, 1};  // an empty barrier's first wait passes
+      bool ok = true;
+      for (int64_t n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
+        const Item it = item_of(p, n);
+        const KeyTiles<kN> tiles(it.both);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (it.last[s] < 0) continue;
+          ok = ok && bar_wait(&bars.q_empty[s], q_phase[s], stop, p.error);
+          if (!ok) break;
+          q_phase[s] ^= 1;
+          bar_expect(&bars.q_full[s], Sh::tile);
+          for (int x = 0; x < DB; ++x)
+            tma_load_4d(q_tile + s * Sh::tile + x * kBox, &p.q, &bars.q_full[s], x * 64, it.i0[s], it.head[s], it.b);
+        }
+        for (int t = 0; ok && t < tiles.n; ++t) {
+          for (int kv = 0; kv < 2; ++kv) {
+            if (!(ok = bar_wait(&bars.kv_empty[stage], phase, stop, p.error))) break;
+            bar_expect(&bars.kv_full[stage], Sh::tile);
+            for (int x = 0; x < DB; ++x)
+              tma_load_4d(kv_tile + stage * Sh::tile + x * kBox, kv ? &p.v : &p.k, &bars.kv_full[stage], x * 64,
+                          tiles.first(t), it.hk, it.b);
+            if (++stage == Sh::stages) stage = 0, phase ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---- products ------------------------------------------------------------
+    if (lane == 0) {
+      const int k_steps = (w.c.dim + 15) / 16, n_out = k_steps * 16;
+      const uint32_t qk = mma_desc(BF16, kM, kN, false, false), pv = mma_desc(BF16, kM, n_out, false, true);
+      const uint32_t q_addr = smem_addr(q_tile), kv_addr = smem_addr(kv_tile);
+      int stage = 0;
+      uint32_t phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+      auto scores = [&](int s, int st, bool last_one) {
+        const uint32_t a = q_addr + s * Sh::tile, b = kv_addr + st * Sh::tile;
+        for (int x = 0; x < k_steps; ++x) {
+          const uint32_t off = (x >> 2) * kBox + (x & 3) * 32;
+          mma_ss(tmem + s * kN, desc_k_major(a + off), desc_k_major(b + off), qk, x > 0);
+        }
+        mma_commit(&bars.s_full[s]);
+        if (last_one) mma_commit(&bars.q_empty[s]);
+      };
+      auto values = [&](int s, int st, bool add) {
+        const uint32_t b = kv_addr + st * Sh::tile;
+#pragma unroll
+        for (int x = 0; x < kN / 16; ++x)
+          mma_ts(tmem + 256 + s * 128, tmem + s * kN + x * 8, desc_mn_major(b + x * 2048, kBox), pv, add || x > 0);
+      };
+      bool ok = true;
+      auto need = [&](bool waited) { return ok = ok && waited; };
+      for (int64_t n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
+        const Item it = item_of(p, n);
+        const KeyTiles<kN> tiles(it.both);
+        if (tiles.n == 0) continue;
+        bool started[2] = {false, false};
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (it.last[s] >= 0) {
+            if (!need(bar_wait(&bars.q_full[s], q_phase[s], stop, p.error))) break;
+            q_phase[s] ^= 1;
+          }
+        }
+        auto next = [&] {
+          if (++stage == Sh::stages) stage = 0, phase ^= 1;
+        };
+        // the stage of K_0 is now, V_t and K_{t+1} follow in turn
+        if (!need(bar_wait(&bars.kv_full[stage], phase, stop, p.error))) break;
+        fence_after();
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          if (it.range[s].touches(tiles.first(0), tiles.end(0))) scores(s, stage, it.last[s] == 0);
+        mma_commit(&bars.kv_empty[stage]);
+        next();
+        for (int t = 0; t < tiles.n; ++t) {
+          const int v_stage = stage;
+          if (!need(bar_wait(&bars.kv_full[stage], phase, stop, p.error))) break;
+          next();
+          const int k_stage = stage;
+          const bool more = t + 1 < tiles.n;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if (it.range[s].touches(tiles.first(t), tiles.end(t))) {
+              if (!need(bar_wait(&bars.p_full[s], p_phase[s], stop, p.error))) break;
+              p_phase[s] ^= 1;
+              fence_after();
+              values(s, v_stage, started[s]);
+              started[s] = true;
+              if (t == it.last[s]) mma_commit(&bars.o_full[s]);
+            }
+            if (s == 1) mma_commit(&bars.kv_empty[v_stage]);
+            if (more) {
+              if (s == 0) {
+                if (!need(bar_wait(&bars.kv_full[k_stage], phase, stop, p.error))) break;
+                fence_after();
+              }
+              if (it.range[s].touches(tiles.first(t + 1), tiles.end(t + 1))) scores(s, k_stage, it.last[s] == t + 1);
+              if (s == 1) mma_commit(&bars.kv_empty[k_stage]);
+            }
+          }
+          if (!ok) break;
+          if (more) next();
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    // ---- softmax, a query row for each thread ----------------------------------
+    const int s = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    const uint32_t t_s = tmem + s * kN + lanes, t_o = tmem + 256 + s * 128 + lanes;
+    const float c = w.c.scale * kLog2e;
+    uint32_t s_phase = 0, o_phase = 0;
+    bool ok = true;
+    for (int64_t n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
+      const Item it = item_of(p, n);
+      const KeyTiles<kN> tiles(it.both);
+      const KeyRange range = s ? it.range[1] : it.range[0];
+      const int i = (s ? it.i0[1] : it.i0[0]) + row, h = s ? it.head[1] : it.head[0];
+      const QuerySpan span = query_span(w, it.b, i);
+      // the keys that all 32 rows of this warp see: tiles inside need no mask
+      const int all_low = __reduce_max_sync(~0u, span.p < 0 ? INT_MAX : span.low);
+      const int all_end = __reduce_min_sync(~0u, span.p < 0 ? -1 : span.p) + 1;
+      float m = -INFINITY, l = 0.f;
+      bool started = false;
+      for (int t = 0; t < tiles.n; ++t) {
+        const int j0 = tiles.first(t), j1 = tiles.end(t);
+        if (!range.touches(j0, j1)) continue;
+        if (!(ok = bar_wait(&bars.s_full[s], s_phase, stop, p.error))) break;
+        s_phase ^= 1;
+        fence_after();
+        const bool masked = !(j0 >= all_low && j0 + kN <= all_end && j1 - j0 == kN);
+        uint32_t seen[4];
+        if (masked) {
+          const int b0 = span.low - j0, b1 = min(span.p + 1, j1) - j0, s0 = span.start - j0,
+                    s1 = min(span.sink_end, j1) - j0;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) seen[x] = bits(b0, b1, x * 32) | bits(s0, s1, x * 32);
+        }
+        uint32_t pk[kN / 2];
+        float2 sum[2];
+        float tops[4];
+        // Scores of 16 keys, loaded into `z` beforehand: their maximum and, with
+        // EXP, their exponentials over the maximum in use, packed.
+        auto part = [&](auto exp, uint32_t *z, int x, float2 base2) {
+          tie16(z);
+          if (masked) {
+#pragma unroll
+            for (int y = 0; y < 16; ++y)
+              if (!(seen[x >> 1] >> ((x & 1) * 16 + y) & 1)) z[y] = 0xff800000u;  // -inf
+          }
+#pragma unroll
+          for (int y = 0; y < 16; ++y) tops[y & 3] = fmaxf(tops[y & 3], __uint_as_float(z[y]));
+          if (decltype(exp)::value) {
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              float2 e = fma2(make_float2(__uint_as_float(z[2 * y]), __uint_as_float(z[2 * y + 1])), make_float2(c, c),
+                              base2);
+              e.x = exp2_fast(e.x), e.y = exp2_fast(e.y);
+              sum[y & 1] = add2(sum[y & 1], e);
+              pk[x * 8 + y] = pack2<BF16>(e.x, e.y);
+            }
+          }
+        };
+        auto tile = [&](auto exp) {
+          uint32_t z[2][16];
+          const float base = m == -INFINITY ? 0.f : m * c;
+          const float2 base2 = make_float2(-base, -base);
+          sum[0] = sum[1] = make_float2(0.f, 0.f);
+          tops[0] = tops[1] = tops[2] = tops[3] = -INFINITY;
+          tmem_ld16(t_s, z[0]);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            wait_ld();
+            if (x < 7) tmem_ld16(t_s + (x + 1) * 16, z[(x + 1) & 1]);
+            part(exp, z[x & 1], x, base2);
+          }
+          return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        };
+        // Later tiles rarely raise the maximum in use: their exponentials are
+        // taken at once and only taken again where it had to rise.
+        float top = started ? tile(std::true_type{}) : tile(std::false_type{});
+        bool raise = (top - m) * c > 8.f;
+        if (!started || __any_sync(~0u, raise)) {
+          const float keep = raise ? (m == -INFINITY ? 0.f : exp2_fast((m - top) * c)) : 1.f;
+          l *= keep;
+          if (raise) m = top;
+          if (started) {
+#pragma unroll 1
+            for (int x = 0; x < DB * 64; x += 32) {
+              uint32_t o[32];
+              tmem_ld32(t_o + x, o);
+              wait_ld();
+              tie32(o);
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * keep);
+              tmem_st32(t_o + x, o);
+            }
+          }
+          tile(std::true_type{});
+        }
+        tmem_st32(t_s, pk), tmem_st32(t_s + 32, pk + 32);
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&bars.p_full[s]);
+        started = true;
+      }
+      if (!ok) break;
+      if (started) {
+        if (!(ok = bar_wait(&bars.o_full[s], o_phase, stop, p.error))) break;
+        o_phase ^= 1;
+        fence_after();
+      }
+      const bool inside = i < w.c.q_len, empty = span.empty();
+      const float inv = empty ? 0.f : 1.f / l;
+      T *out = static_cast<T *>(w.c.out) + ((it.b * w.c.q_len + i) * w.c.q_heads + h) * w.c.dim;
+      bool bad = false;
+#pragma unroll 1
+      for (int x = 0; x < DB * 64; x += 32) {
+        uint32_t o[32];
+        if (started) {
+          tmem_ld32(t_o + x, o);
+          wait_ld();
+          tie32(o);
+        }
+#pragma unroll
+        for (int y = 0; y < 32; y += 8) {
+          uint32_t v[4];
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            const float e0 = empty ? 0.f : __uint_as_float(o[y + 2 * z]) * inv;
+            const float e1 = empty ? 0.f : __uint_as_float(o[y + 2 * z + 1]) * inv;
+            bad = bad || (x + y < w.c.dim && !(fabsf(e0) < INFINITY && fabsf(e1) < INFINITY));
+            v[z] = pack2<BF16>(e0, e1);
+          }
+          if (inside && x + y < w.c.dim) *reinterpret_cast<uint4 *>(out + x + y) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+      }
+      if (inside && w.c.lse)
+        w.c.lse[((int64_t)it.b * w.c.q_heads + h) * w.c.q_len + i] = empty ? INFINITY : m * c + log2f(l);
+      for (unsigned left = __ballot_sync(~0u, bad && inside); left; left &= left - 1)
+        repair_row<T>(w, it.b, h, i - lane + __ffs(left) - 1);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (threadIdx.x == 0 && *stop)  // a wait gave up: let copies in flight land before the memory goes away
+    for (int s = 0; s < Sh::stages; ++s)
+      for (int x = 0; x < (1 << 16) && !bar_try(&bars.kv_full[s], 0) && !bar_try(&bars.kv_full[s], 1); ++x) {
+      }
+  __syncthreads();
+  if (warp == 2) tmem_free(tmem, 512);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void *f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return fn;
+}
+
+// Boxes of 64 elements by `rows` tokens of one head; what lies outside the
+// tensor (elements past the head size, tokens past the end) reads as 0.
+CUtensorMap make_map(const WindowTensor &t, int64_t batch, int64_t tokens, int64_t heads, int64_t dim, bool bf16,
+                     int rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
+  if (fn == nullptr) fail(MSX_ERR_RUNTIME, "the driver does not offer cuTensorMapEncodeTiled.");
+  CUtensorMap map;
+  const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)tokens, (cuuint64_t)heads, (cuuint64_t)batch};
+  const cuuint64_t strides[3] = {(cuuint64_t)t.token * 2, (cuuint64_t)t.head * 2, (cuuint64_t)t.batch * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  const CUresult r = fn(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                        const_cast<void *>(t.ptr), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) fail(MSX_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r) + ".");
+  return map;
+}
+
+template <typename T, int DB> void launch(Params &p, cudaStream_t s) {
+  auto kernel = forward_tc_kernel<T, DB>;
+  MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DB>::smem));
+  kernel<<<(unsigned)std::min<int64_t>(p.items, num_sms()), kThreads, Shape<DB>::smem, s>>>(p);
+  MSX_CHECK_LAUNCH();
+}
+
+bool tma_ready(const WindowTensor &t) {
+  const int64_t most = (int64_t)1 << 39;  // elements; strides stay below 2^40 bytes
+  auto good = [&](int64_t x) { return x > 0 && x % 8 == 0 && x < most; };
+  return reinterpret_cast<uintptr_t>(t.ptr) % 16 == 0 && good(t.batch) && good(t.token) && good(t.head);
+}
+
+}  // namespace
+
+int *window_error_flag() {
+  int *ptr = nullptr;
+  MSX_CUDA(cudaGetSymbolAddress(reinterpret_cast<void **>(&ptr), g_window_error));
+  return ptr;
+}
+
+bool window_take_error() {
+  int v = 0;
+  MSX_CUDA(cudaMemcpyFromSymbol(&v, g_window_error, sizeof(int)));
+  if (v) {
+    const int zero = 0;
+    MSX_CUDA(cudaMemcpyToSymbol(g_window_error, &zero, sizeof(int)));
+  }
+  return v != 0;
+}
+
+// 16-bit types, head sizes and layouts that TMA can read; the running maximum
+// of raw scores needs a positive scale.
+bool window_tc_ok(const WindowProblem &w, int value_dtype) {
+  return value_dtype != MSX_F32 && w.c.dim % 8 == 0 && w.c.dim <= 128 && w.c.scale > 0.f && w.c.k_len > 0 &&
+         tma_ready(w.c.q) && tma_ready(w.c.k) && tma_ready(w.c.v);
+}
+
+void window_forward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s) {
+  if (w.c.batch == 0 || w.c.q_len == 0) return;
+  Params p{};
+  p.w = w;
+  const bool bf16 = value_dtype == MSX_BF16;
+  p.q = make_map(w.c.q, w.c.batch, w.c.q_len, w.c.q_heads, w.c.dim, bf16, kM);
+  p.k = make_map(w.c.k, w.c.batch, w.c.k_len, w.c.k_heads, w.c.dim, bf16, kN);
+  p.v = make_map(w.c.v, w.c.batch, w.c.k_len, w.c.k_heads, w.c.dim, bf16, kN);
+  p.q_tiles = (int)ceil_div(w.c.q_len, kM);
+  p.paired = w.group % 2 == 0;
+  p.items = p.paired ? w.c.batch * w.c.k_heads * p.q_tiles * (w.group / 2)
+                     : w.c.batch * w.c.q_heads * ((p.q_tiles + 1) / 2);
+  p.error = window_error_flag();
+  if (bf16) {
+    if (w.c.dim <= 64) launch<__nv_bfloat16, 1>(p, s); else launch<__nv_bfloat16, 2>(p, s);
+  } else {
+    if (w.c.dim <= 64) launch<__half, 1>(p, s); else launch<__half, 2>(p, s);
+  }
+}
+
+}  // namespace msx
