@@ -498,7 +498,8 @@ MSX_API int msx_csr_distill_forward_backward(
  * q_len = k_len) sequences lie one after another along the tokens; tokens
  * outside all of them see nothing and get zeros.
  * out, grad_out, dq are contiguous like q; dk, dv like k. lse: float (batch,
- * q_heads, q_len), written by forward (null: not wanted), read by backward;
+ * q_heads, q_len rounded up to a multiple of 128), 16-byte aligned, written by
+ * forward (null: not wanted), read by backward;
  * delta: float workspace of the same size. backward reads forward's out. */
 MSX_API int msx_window_attention_forward(
     int value_dtype, const void *q, const int64_t *q_strides, const void *k,

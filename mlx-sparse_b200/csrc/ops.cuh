@@ -56,7 +56,7 @@ void distill_run(int value_dtype, int index_dtype, const DistillCall &call, cuda
 // Windowed attention. q, k, v: (batch, tokens, heads, dim) with any batch,
 // token and head strides (in elements) and stride 1 along dim; out, grad_out and
 // the gradients are contiguous in that order. lse and delta: float (batch,
-// q_heads, q_len). A null dq (dk and dv) is not computed.
+// q_heads, q_len rounded up to a multiple of 128). A null dq (dk and dv) is not computed.
 struct WindowTensor {
   const void *ptr;
   int64_t batch, token, head;

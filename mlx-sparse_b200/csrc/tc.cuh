@@ -39,7 +39,7 @@ __device__ __forceinline__ unsigned long long now_ns() {
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
   return t;
 }
-__device__ __noinline__ bool bar_wait_slow(uint64_t *bar, uint32_t parity, volatile int *stop, int *error) {
+static __device__ __noinline__ bool bar_wait_slow(uint64_t *bar, uint32_t parity, volatile int *stop, int *error) {
   const unsigned long long begin = now_ns();
   while (!bar_try(bar, parity)) {
     if (*stop) return false;
@@ -65,6 +65,14 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, u
           smem_addr(dst)),
       "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
+}
+
+// Untiled: both addresses 16-byte aligned, a multiple of 16 bytes.
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_addr(dst)),
+               "l"(src), "r"(bytes), "r"(smem_addr(bar))
+               : "memory");
 }
 
 // ---- tensor memory -------------------------------------------------------------

@@ -108,7 +108,7 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) forward_ker
     }
     // an empty row's +inf makes its probabilities 0 in the backward pass
     if (w.c.lse && lane == 0)
-      w.c.lse[((int64_t)b * w.c.q_heads + h) * w.c.q_len + i] = empty ? INFINITY : m[r] + log2f(l[r]);
+      w.c.lse[((int64_t)b * w.c.q_heads + h) * w.lse_row + i] = empty ? INFINITY : m[r] + log2f(l[r]);
   }
 }
 
@@ -125,7 +125,7 @@ template <typename T> __global__ void delta_kernel(const WindowProblem w) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
   const int64_t h = x % w.c.q_heads, bi = x / w.c.q_heads, b = bi / w.c.q_len, i = bi % w.c.q_len;
-  if (lane == 0) w.c.delta[(b * w.c.q_heads + h) * w.c.q_len + i] = s;
+  if (lane == 0) w.c.delta[(b * w.c.q_heads + h) * w.lse_row + i] = s;
 }
 
 template <typename T> __global__ void __launch_bounds__(kWarps * 32) dq_kernel(const WindowProblem w) {
@@ -148,7 +148,7 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) dq_kernel(c
   for (int r = 0; r < kRowsPerWarp; ++r) {
     const int i = i0 + warp * kRowsPerWarp + r;
     span[r] = query_span(w, b, i);
-    const int64_t at = ((int64_t)b * w.c.q_heads + h) * w.c.q_len + i;
+    const int64_t at = ((int64_t)b * w.c.q_heads + h) * w.lse_row + i;
     lse[r] = i < w.c.q_len ? w.c.lse[at] : INFINITY;
     delta[r] = i < w.c.q_len ? w.c.delta[at] : 0.f;
 #pragma unroll
@@ -216,7 +216,7 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) dkv_kernel(
   for (int h = hk * w.group; h < (hk + 1) * w.group; ++h) {
     const T *q = static_cast<const T *>(w.c.q.ptr) + b * w.c.q.batch + h * w.c.q.head;
     const T *g = static_cast<const T *>(w.c.grad_out) + (b * w.c.q_len * w.c.q_heads + h) * dim;
-    const int64_t at = ((int64_t)b * w.c.q_heads + h) * w.c.q_len;
+    const int64_t at = ((int64_t)b * w.c.q_heads + h) * w.lse_row;
     for (int i0 = first; i0 < stop; i0 += kTile) {
       __syncthreads();
       load_rows(sq, ks, q, w.c.q.token, i0, (int)w.c.q_len, kTile, dim);
@@ -305,6 +305,7 @@ static WindowProblem problem(const WindowCall &c) {
   w.group = (int)(c.q_heads / c.k_heads);
   w.offset = (int)(c.k_len - c.q_len);
   w.wide_ptr = c.indptr_dtype == MSX_I64;
+  w.lse_row = ceil_div(c.q_len, 128) * 128;
   w.window = (int)std::min(c.window, c.k_len);
   w.sinks = (int)std::min(c.sinks, c.k_len);
   return w;
@@ -323,7 +324,11 @@ void window_decode_run(int value_dtype, const WindowCall &c, cudaStream_t s) {
 }
 
 void window_backward_run(int value_dtype, const WindowCall &c, cudaStream_t s) {
-  window_backward_general(problem(c), value_dtype, s);
+  const WindowProblem w = problem(c);
+  if (window_tc_ok(w, value_dtype) && reinterpret_cast<uintptr_t>(c.grad_out) % 16 == 0)
+    window_backward_tc(w, value_dtype, s);
+  else
+    window_backward_general(w, value_dtype, s);
 }
 
 }  // namespace msx

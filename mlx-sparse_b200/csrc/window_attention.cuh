@@ -19,6 +19,7 @@ struct WindowProblem {
   int offset;   // position of query 0
   int wide_ptr; // indptr or lengths are int64
   int window, sinks;  // clamped to k_len
+  int64_t lse_row;    // floats of lse (delta) for each head: q_len rounded up to whole tiles
 };
 
 // Sequence of a position: [start, end), empty (start = end) outside all.
@@ -127,9 +128,11 @@ __device__ __forceinline__ int last_query(const WindowProblem &w, int j) {
 // Kernels for every type and head size (window_attention.cu) ...
 void window_forward_general(const WindowProblem &w, int value_dtype, cudaStream_t s);
 void window_backward_general(const WindowProblem &w, int value_dtype, cudaStream_t s);
-// ... and for the tensor cores (window_forward_tc.cu).
+// ... and for the tensor cores (window_forward_tc.cu, window_backward_tc.cu).
 bool window_tc_ok(const WindowProblem &w, int value_dtype);
 void window_forward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s);
+void window_backward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s);
+void window_delta(const WindowProblem &w, int value_dtype, cudaStream_t s);
 int *window_error_flag();
 
 }  // namespace msx

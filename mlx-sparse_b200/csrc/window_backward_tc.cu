@@ -1,0 +1,731 @@
+// Windowed attention, backward, on the tensor cores (float16 / bfloat16, head
+// sizes that are multiples of 8 up to 128). Two kernels, so that every gradient
+// is summed in one place and in one order:
+//
+//  dQ:    a query tile of 128 rows walks the tiles of 128 keys that it sees:
+//         S = Q K^T, dP = dO V^T, dS = P (dP - delta), dQ += dS K.
+//  dK/dV: a key tile of 128 rows walks the tiles of 128 queries that see it, of
+//         every head that shares it: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO,
+//         dK += dS^T Q.
+//
+// P = 2^(c S - lse) is recomputed from the forward pass's log-sum-exp. That is 7
+// products of 128 x 128 x dim for each tile pair where one kernel with atomic
+// sums of dQ would make 5; atomics would change results from run to run.
+//
+// As in the forward pass one warp loads tiles by TMA, one thread issues
+// tcgen05.mma, and two warpgroups do the arithmetic in between, straight from
+// tensor memory, 64 columns of every row each. P and dS, rounded to the inputs'
+// type for the second products (half a step each; the sums are fp32), take the
+// place of the scores they came from. The products of one tile pair are issued
+// between those of its neighbours, so that the tensor cores work while the
+// exponentials of the next tile and the differences of this one are taken.
+//
+// Bound: the tensor cores, 4 x 512 (3 x 512) clocks for each tile pair at head
+// size 128, against 128 x 128 / 16 = 1024 clocks of exponentials.
+//
+// A masked P or dS is 0, but 0 times an infinity or NaN in a hidden row of dO, Q
+// or K would reach the sums: rows that end not finite while something not finite
+// hides in their tiles are computed again pair by pair.
+#include <algorithm>
+
+#include "window_tc.cuh"
+
+namespace msx {
+
+using namespace tc;
+
+namespace {
+
+constexpr int kT = 128;        // rows and columns of a tile pair
+constexpr int kThreads = 384;  // loads, products, one warp for tensor memory, one idle; 8 warps of arithmetic
+constexpr int kStages = 4;
+
+struct Params {
+  WindowProblem w;
+  CUtensorMap q, k, v, g;
+  int64_t items;
+  int q_tiles;
+  int *error;
+};
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n"
+      " mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// The score of one pair times log2(e) and dO_i . V_j, from global memory.
+template <typename T> struct PairDots {
+  const T *q, *k, *g, *v;
+  __device__ PairDots(const WindowProblem &w, int b, int h, int64_t i, int64_t j) {
+    const int hk = h / w.group;
+    q = static_cast<const T *>(w.c.q.ptr) + b * w.c.q.batch + h * w.c.q.head + i * w.c.q.token;
+    g = static_cast<const T *>(w.c.grad_out) + ((b * w.c.q_len + i) * w.c.q_heads + h) * w.c.dim;
+    k = static_cast<const T *>(w.c.k.ptr) + b * w.c.k.batch + hk * w.c.k.head + j * w.c.k.token;
+    v = static_cast<const T *>(w.c.v.ptr) + b * w.c.v.batch + hk * w.c.v.head + j * w.c.v.token;
+  }
+  __device__ void weights(const WindowProblem &w, float lse, float delta, float &p, float &ds) const {
+    float s = 0.f, dp = 0.f;
+    for (int d = 0; d < w.c.dim; ++d) {
+      s = fmaf(VT<T>::load(q[d]), VT<T>::load(k[d]), s);
+      dp = fmaf(VT<T>::load(g[d]), VT<T>::load(v[d]), dp);
+    }
+    p = exp2f(s * (w.c.scale * kLog2e) - lse);
+    ds = p * (dp - delta);
+  }
+};
+
+// One row of dQ again, by a warp, pair by pair; columns [d0, d1) are written.
+template <typename T>
+__device__ __noinline__ void repair_dq(const WindowProblem &w, int b, int h, int i, int d0, int d1) {
+  const int lane = threadIdx.x & 31;
+  const QuerySpan span = query_span(w, b, i);
+  const int64_t at = ((int64_t)b * w.c.q_heads + h) * w.lse_row + i;
+  const float lse = w.c.lse[at], delta = w.c.delta[at];
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int part = 0; part < 2; ++part) {
+    const int from = part ? span.low : span.start, end = part ? span.p + 1 : span.sink_end;
+    for (int j0 = from; j0 < end; j0 += 32) {
+      float p = 0.f, ds = 0.f;
+      if (j0 + lane < end) PairDots<T>(w, b, h, i, j0 + lane).weights(w, lse, delta, p, ds);
+      for (int x = 0; x < min(32, end - j0); ++x) {
+        const float e = __shfl_sync(~0u, ds, x);
+        const T *k = PairDots<T>(w, b, h, i, j0 + x).k;
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if (y * 32 + lane < w.c.dim) acc[y] = fmaf(e, VT<T>::load(k[y * 32 + lane]), acc[y]);
+      }
+    }
+  }
+  T *dq = static_cast<T *>(w.c.dq) + ((b * w.c.q_len + i) * w.c.q_heads + h) * w.c.dim;
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    const int d = y * 32 + lane;
+    if (d >= d0 && d < d1 && d < w.c.dim) dq[d] = VT<T>::store(acc[y] * w.c.scale);
+  }
+}
+
+// One row of dK (keys) or dV again.
+template <typename T>
+__device__ __noinline__ void repair_dkv(const WindowProblem &w, int b, int hk, int j, bool keys) {
+  const int lane = threadIdx.x & 31, shift = key_count(w, b) - (int)w.c.q_len;
+  const int i0 = max(0, j - shift), i1 = min((int)w.c.q_len, last_query(w, j) - shift + 1);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int h = hk * w.group; h < (hk + 1) * w.group; ++h) {
+    const int64_t at = ((int64_t)b * w.c.q_heads + h) * w.lse_row;
+    for (int i = i0; i < i1; i += 32) {
+      float p = 0.f, ds = 0.f;
+      if (i + lane < i1)
+        PairDots<T>(w, b, h, i + lane, j).weights(w, w.c.lse[at + i + lane], w.c.delta[at + i + lane], p, ds);
+      for (int x = 0; x < min(32, i1 - i); ++x) {
+        const float e = __shfl_sync(~0u, keys ? ds : p, x);
+        const PairDots<T> pair(w, b, h, i + x, j);
+        const T *row = keys ? pair.q : pair.g;
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if (y * 32 + lane < w.c.dim) acc[y] = fmaf(e, VT<T>::load(row[y * 32 + lane]), acc[y]);
+      }
+    }
+  }
+  T *out = static_cast<T *>(keys ? w.c.dk : w.c.dv) + ((b * w.c.k_len + j) * w.c.k_heads + hk) * w.c.dim;
+#pragma unroll
+  for (int y = 0; y < 4; ++y)
+    if (y * 32 + lane < w.c.dim) out[y * 32 + lane] = VT<T>::store(acc[y] * (keys ? w.c.scale : 1.f));
+}
+
+// Products issued by one thread. Scores: both operands K-major in shared
+// memory. Sums: left operand in tensor memory, its columns 64.. at `left_hi`,
+// right operand MN-major in shared memory.
+struct Products {
+  int k_steps;
+  uint32_t scores_desc, sums_desc;
+  template <bool BF16> __device__ static Products make(int dim) {
+    Products r;
+    r.k_steps = (dim + 15) / 16;
+    r.scores_desc = mma_desc(BF16, kT, kT, false, false);
+    r.sums_desc = mma_desc(BF16, kT, r.k_steps * 16, false, true);
+    return r;
+  }
+  __device__ void scores(uint32_t d, uint32_t a, uint32_t b) const {
+    for (int x = 0; x < k_steps; ++x) {
+      const uint32_t off = (x >> 2) * kBox + (x & 3) * 32;
+      mma_ss(d, desc_k_major(a + off), desc_k_major(b + off), scores_desc, x > 0);
+    }
+  }
+  __device__ void sums(uint32_t d, uint32_t left, uint32_t b, bool add) const {
+#pragma unroll
+    for (int x = 0; x < kT / 16; ++x)
+      mma_ts(d, left + (x >> 2) * 64 + (x & 3) * 8, desc_mn_major(b + x * 2048, kBox), sums_desc, add || x > 0);
+  }
+};
+
+// Writes 32 accumulator columns of a row, scaled; true if one is not finite.
+template <typename T> __device__ __forceinline__ bool store32(T *row, uint32_t *o, float scale, int d0, int dim, bool inside) {
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  bool bad = false;
+#pragma unroll
+  for (int y = 0; y < 32; y += 8) {
+    uint32_t v[4];
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+      const float a = __uint_as_float(o[y + 2 * z]) * scale, c = __uint_as_float(o[y + 2 * z + 1]) * scale;
+      bad = bad || (d0 + y < dim && !(fabsf(a) < INFINITY && fabsf(c) < INFINITY));
+      v[z] = pack2<BF16>(a, c);
+    }
+    if (inside && d0 + y < dim) *reinterpret_cast<uint4 *>(row + d0 + y) = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+  return bad;
+}
+
+__device__ __forceinline__ void drain(uint64_t *bars, int n) {
+  for (int s = 0; s < n; ++s)
+    for (int x = 0; x < (1 << 16) && !bar_try(&bars[s], 0) && !bar_try(&bars[s], 1); ++x) {
+    }
+}
+
+// ---- dK and dV -------------------------------------------------------------------
+struct KvBars {
+  uint64_t kv_full, full[kStages], empty[kStages], s_full, dp_full, p_full, ds_full, done;
+  uint32_t tmem;
+  int stop, last;
+};
+
+template <int DB> constexpr int kKvSmem = 1024 + (2 + kStages) * DB * kBox + 2 * 2 * kT * 4;
+
+template <typename T, int DB>
+__global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_constant__ Params p) {
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kTile = DB * kBox;
+  extern __shared__ unsigned char raw[];
+  unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  __shared__ KvBars bars;
+  unsigned char *k_tile = sm, *v_tile = sm + kTile, *ring = sm + 2 * kTile;
+  float *row_stats = reinterpret_cast<float *>(ring + kStages * kTile);  // two of {lse[128], delta[128]}
+  const WindowProblem &w = p.w;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hk = (int)(blockIdx.x % w.c.k_heads);
+  const int b = (int)(blockIdx.x / w.c.k_heads % w.c.batch);
+  const int j0 = (int)(blockIdx.x / w.c.k_heads / w.c.batch) * kT;
+  const int shift = w.offset;
+  volatile int *stop = &bars.stop;
+  if (threadIdx.x == 0) {
+    bar_init(&bars.kv_full, 1);
+    for (int s = 0; s < kStages; ++s) bar_init(&bars.full[s], 1), bar_init(&bars.empty[s], 1);
+    bar_init(&bars.s_full, 1), bar_init(&bars.dp_full, 1), bar_init(&bars.done, 1);
+    bar_init(&bars.p_full, 8), bar_init(&bars.ds_full, 8);
+    bars.stop = 0, bars.last = -1;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) tmem_alloc(&bars.tmem, 512);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = bars.tmem, t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
+  // the tiles of queries that see any of these keys
+  const int key = j0 + (warp & 3) * 32 + lane, own_last = last_query(w, key);
+  if (warp >= 4 && warp < 8) {
+    const int top = __reduce_max_sync(~0u, own_last);
+    if (lane == 0) atomicMax(&bars.last, top);
+  }
+  __syncthreads();
+  const int i_first = max(0, j0 - shift), i_stop = min((int)w.c.q_len, bars.last - shift + 1);
+  const int t0 = i_first / kT, n_tiles = i_stop > i_first ? (i_stop - t0 * kT + kT - 1) / kT : 0;
+  const int n = n_tiles * w.group;
+  auto head_of = [&](int it) { return hk * w.group + it / n_tiles; };
+  auto query_of = [&](int it) { return (t0 + it % n_tiles) * kT; };
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      bar_expect(&bars.kv_full, 2 * kTile);
+      for (int x = 0; x < DB; ++x) {
+        tma_load_4d(k_tile + x * kBox, &p.k, &bars.kv_full, x * 64, j0, hk, b);
+        tma_load_4d(v_tile + x * kBox, &p.v, &bars.kv_full, x * 64, j0, hk, b);
+      }
+      bool ok = true;
+      for (int e = 0; ok && e < 2 * n; ++e) {  // Q and dO of each pair in turn
+        const int s = e % kStages, it = e >> 1;
+        const int h = head_of(it), i0 = query_of(it);
+        if (!(ok = bar_wait(&bars.empty[s], (e / kStages & 1) ^ 1, stop, p.error))) break;
+        if (e & 1) {
+          bar_expect(&bars.full[s], kTile);
+        } else {
+          bar_expect(&bars.full[s], kTile + 2 * kT * 4);
+          const int64_t at = ((int64_t)b * w.c.q_heads + h) * w.lse_row + i0;
+          float *dst = row_stats + (it & 1) * 2 * kT;
+          bulk_load(dst, w.c.lse + at, kT * 4, &bars.full[s]);
+          bulk_load(dst + kT, w.c.delta + at, kT * 4, &bars.full[s]);
+        }
+        for (int x = 0; x < DB; ++x)
+          tma_load_4d(ring + s * kTile + x * kBox, e & 1 ? &p.g : &p.q, &bars.full[s], x * 64, i0, h, b);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      const Products mm = Products::make<BF16>(w.c.dim);
+      const uint32_t ka = smem_addr(k_tile), va = smem_addr(v_tile), ra = smem_addr(ring);
+      bool ok = bar_wait(&bars.kv_full, 0, stop, p.error);
+      auto ready = [&](int e) { return ok = ok && bar_wait(&bars.full[e % kStages], e / kStages & 1, stop, p.error); };
+      auto tile = [&](int e) { return ra + (e % kStages) * kTile; };
+      if (ready(0)) {
+        fence_after();
+        mm.scores(t_s, ka, tile(0));
+        mma_commit(&bars.s_full);
+      }
+      if (ready(1)) {
+        mm.scores(t_dp, va, tile(1));
+        mma_commit(&bars.dp_full);
+      }
+      for (int it = 0; ok && it < n; ++it) {
+        const int q = 2 * it, g = q + 1;
+        if (!(ok = bar_wait(&bars.p_full, it & 1, stop, p.error))) break;
+        fence_after();
+        mm.sums(t_dv, t_s, tile(g), it > 0);
+        mma_commit(&bars.empty[g % kStages]);
+        if (it + 1 < n) {
+          if (!ready(q + 2)) break;
+          mm.scores(t_s, ka, tile(q + 2));
+          mma_commit(&bars.s_full);
+        }
+        if (!(ok = bar_wait(&bars.ds_full, it & 1, stop, p.error))) break;
+        fence_after();
+        mm.sums(t_dk, t_dp, tile(q), it > 0);
+        mma_commit(&bars.empty[q % kStages]);
+        if (it + 1 < n) {
+          if (!ready(g + 2)) break;
+          mm.scores(t_dp, va, tile(g + 2));
+          mma_commit(&bars.dp_full);
+        }
+      }
+      mma_commit(&bars.done);
+    }
+  } else if (warp >= 4) {
+    const int half = (warp - 4) >> 2;
+    const uint32_t at = ((uint32_t)(warp & 3) << 21) + half * 64;
+    const float c = w.c.scale * kLog2e;
+    const float2 minus_c = make_float2(-c, -c), minus_1 = make_float2(-1.f, -1.f);
+    // the queries that all 32 keys of this warp are seen by
+    const int all_first = __reduce_max_sync(~0u, key) - shift, all_last = __reduce_min_sync(~0u, own_last) - shift;
+    bool ok = true;
+    for (int it = 0; ok && it < n; ++it) {
+      const int i0 = query_of(it) + half * 64;
+      const float *lse = row_stats + (it & 1) * 2 * kT + half * 64, *delta = lse + kT;
+      const bool masked = !(i0 >= all_first && i0 + 63 <= all_last);
+      const int c0 = key - shift - i0, c1 = min(own_last - shift, (int)w.c.q_len - 1) - i0 + 1;
+      const uint32_t seen[2] = {bits(c0, c1, 0), bits(c0, c1, 32)};
+      // lse and delta came with Q's tile, which the products of s_full have read
+      if (!(ok = bar_wait(&bars.full[2 * it % kStages], 2 * it / kStages & 1, stop, p.error))) break;
+      if (!(ok = bar_wait(&bars.s_full, it & 1, stop, p.error))) break;
+      fence_after();
+      float2 pr[32];
+      {
+        uint32_t z[2][16], pk[16];
+        tmem_ld16(t_s + at, z[0]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          wait_ld();
+          if (x < 3) tmem_ld16(t_s + at + (x + 1) * 16, z[(x + 1) & 1]);
+          uint32_t *zz = z[x & 1];
+          tie16(zz);
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            const int col = x * 16 + 2 * y;
+            float2 e = fma2(make_float2(__uint_as_float(zz[2 * y]), __uint_as_float(zz[2 * y + 1])), minus_c,
+                            *reinterpret_cast<const float2 *>(lse + col));
+            e.x = exp2_fast(-e.x), e.y = exp2_fast(-e.y);
+            if (masked) {
+              if (!(seen[col >> 5] >> (col & 31) & 1)) e.x = 0.f;
+              if (!(seen[col >> 5] >> (col & 31) & 2)) e.y = 0.f;
+            }
+            pr[x * 8 + y] = e;
+            pk[(x & 1) * 8 + y] = pack2<BF16>(e.x, e.y);
+          }
+          if (x & 1) tmem_st16(t_s + at + (x >> 1) * 16, pk);
+        }
+      }
+      wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&bars.p_full);
+      if (!(ok = bar_wait(&bars.dp_full, it & 1, stop, p.error))) break;
+      fence_after();
+      {
+        uint32_t z[2][16], pk[16];
+        tmem_ld16(t_dp + at, z[0]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          wait_ld();
+          if (x < 3) tmem_ld16(t_dp + at + (x + 1) * 16, z[(x + 1) & 1]);
+          uint32_t *zz = z[x & 1];
+          tie16(zz);
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            const int col = x * 16 + 2 * y;
+            // delta - dP: minus dS comes out, and dK takes the sign back at the end
+            float2 e = fma2(make_float2(__uint_as_float(zz[2 * y]), __uint_as_float(zz[2 * y + 1])), minus_1,
+                            *reinterpret_cast<const float2 *>(delta + col));
+            e = mul2(e, pr[x * 8 + y]);
+            if (masked) {
+              if (!(seen[col >> 5] >> (col & 31) & 1)) e.x = 0.f;
+              if (!(seen[col >> 5] >> (col & 31) & 2)) e.y = 0.f;
+            }
+            pk[(x & 1) * 8 + y] = pack2<BF16>(e.x, e.y);
+          }
+          if (x & 1) tmem_st16(t_dp + at + (x >> 1) * 16, pk);
+        }
+      }
+      wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&bars.ds_full);
+    }
+    if (ok && n > 0) ok = bar_wait(&bars.done, 0, stop, p.error);
+    if (ok) {
+      fence_after();
+      // the first warpgroup writes dV, the second dK
+      const bool inside = key < w.c.k_len;
+      T *out = static_cast<T *>(half ? w.c.dk : w.c.dv) + ((b * w.c.k_len + key) * w.c.k_heads + hk) * w.c.dim;
+      const uint32_t from = (half ? t_dk : t_dv) + ((uint32_t)(warp & 3) << 21);
+      bool bad = false;
+#pragma unroll 1
+      for (int x = 0; x < DB * 64; x += 32) {
+        uint32_t o[32];
+        if (n > 0) {
+          tmem_ld32(from + x, o);
+          wait_ld();
+          tie32(o);
+        } else {
+#pragma unroll
+          for (int y = 0; y < 32; ++y) o[y] = 0;
+        }
+        bad = store32<T>(out, o, half ? -w.c.scale : 1.f, x, w.c.dim, inside) || bad;
+      }
+      if (__any_sync(~0u, bad && inside)) {
+        bool hidden = false;
+        for (int it = 0; it < n; ++it) {
+          const int i0 = query_of(it);
+          if (i0 >= all_first && i0 + kT - 1 <= all_last) continue;
+          const PairDots<T> row(w, b, head_of(it), 0, 0);
+          for (int x = 0; x < kT; x += 32) {
+            const bool odd = half ? row_not_finite(row.q, w.c.q.token, i0 + x + lane, w.c.q_len, w.c.dim)
+                                  : row_not_finite(row.g, (int64_t)w.c.q_heads * w.c.dim, i0 + x + lane, w.c.q_len, w.c.dim);
+            for (unsigned left = __ballot_sync(~0u, odd); left; left &= left - 1) {
+              const int i = i0 + x + __ffs(left) - 1;
+              hidden = hidden || i < key - shift || i > own_last - shift;
+            }
+          }
+        }
+        for (unsigned left = __ballot_sync(~0u, bad && inside && hidden); left; left &= left - 1)
+          repair_dkv<T>(w, b, hk, key - lane + __ffs(left) - 1, half != 0);
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (threadIdx.x == 0 && *stop) drain(bars.full, kStages);
+  __syncthreads();
+  if (warp == 2) tmem_free(tmem, 512);
+}
+
+// ---- dQ ---------------------------------------------------------------------------
+struct QBars {
+  uint64_t q_full, q_empty, full[kStages], empty[kStages], s_full[2], dp_full, ds_full, dq_full;
+  uint32_t tmem;
+  int stop;
+};
+
+template <int DB> constexpr int kQSmem = 1024 + (2 + kStages) * DB * kBox;
+
+template <typename T, int DB>
+__global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constant__ Params p) {
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kTile = DB * kBox;
+  extern __shared__ unsigned char raw[];
+  unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  __shared__ QBars bars;
+  unsigned char *q_tile = sm, *g_tile = sm + kTile, *ring = sm + 2 * kTile;
+  const WindowProblem &w = p.w;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int *stop = &bars.stop;
+  if (threadIdx.x == 0) {
+    bar_init(&bars.q_full, 1), bar_init(&bars.q_empty, 1);
+    for (int s = 0; s < kStages; ++s) bar_init(&bars.full[s], 1), bar_init(&bars.empty[s], 1);
+    bar_init(&bars.s_full[0], 1), bar_init(&bars.s_full[1], 1);
+    bar_init(&bars.dp_full, 1), bar_init(&bars.ds_full, 8), bar_init(&bars.dq_full, 1);
+    bars.stop = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) tmem_alloc(&bars.tmem, 512);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = bars.tmem, t_dp = tmem + 256, t_dq = tmem + 384;  // two score tiles before them
+  auto item = [&](int64_t x, int &b, int &h, int &i0) {  // heads of one key head side by side
+    const int g = (int)(x % w.group);
+    x /= w.group;
+    i0 = (int)(x % p.q_tiles) * kT;
+    x /= p.q_tiles;
+    h = (int)(x % w.c.k_heads) * w.group + g;
+    b = (int)(x / w.c.k_heads);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0, b, h, i0;
+      uint32_t phase = 1, q_phase = 1;
+      bool ok = true;
+      for (int64_t x = blockIdx.x; ok && x < p.items; x += gridDim.x) {
+        item(x, b, h, i0);
+        const KeyTiles<kT> tiles(key_range(w, b, i0, i0 + kT - 1));
+        if (tiles.n == 0) continue;
+        if (!(ok = bar_wait(&bars.q_empty, q_phase, stop, p.error))) break;
+        q_phase ^= 1;
+        bar_expect(&bars.q_full, 2 * kTile);
+        for (int d = 0; d < DB; ++d) {
+          tma_load_4d(q_tile + d * kBox, &p.q, &bars.q_full, d * 64, i0, h, b);
+          tma_load_4d(g_tile + d * kBox, &p.g, &bars.q_full, d * 64, i0, h, b);
+        }
+        for (int e = 0; ok && e < 2 * tiles.n; ++e) {
+          if (!(ok = bar_wait(&bars.empty[stage], phase, stop, p.error))) break;
+          bar_expect(&bars.full[stage], kTile);
+          for (int d = 0; d < DB; ++d)
+            tma_load_4d(ring + stage * kTile + d * kBox, e & 1 ? &p.v : &p.k, &bars.full[stage], d * 64,
+                        tiles.first(e >> 1), h / w.group, b);
+          if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const Products mm = Products::make<BF16>(w.c.dim);
+      const uint32_t qa = smem_addr(q_tile), ga = smem_addr(g_tile), ra = smem_addr(ring);
+      int64_t done = 0;  // tile pairs of earlier items: K of pair t is ring entry 2 (done + t), V the next
+      uint32_t q_phase = 0;
+      bool ok = true;
+      auto ready = [&](int64_t e) {
+        return ok = ok && bar_wait(&bars.full[e % kStages], (uint32_t)(e / kStages & 1), stop, p.error);
+      };
+      auto tile = [&](int64_t e) { return ra + (uint32_t)(e % kStages) * kTile; };
+      auto s_at = [&](int64_t t) { return tmem + (uint32_t)(t & 1) * 128; };
+      for (int64_t x = blockIdx.x; ok && x < p.items; x += gridDim.x) {
+        int b, h, i0;
+        item(x, b, h, i0);
+        const KeyTiles<kT> tiles(key_range(w, b, i0, i0 + kT - 1));
+        if (tiles.n == 0) continue;
+        if (!(ok = bar_wait(&bars.q_full, q_phase, stop, p.error))) break;
+        q_phase ^= 1;
+        auto scores = [&](int64_t t) {
+          if (!ready(2 * t)) return;
+          fence_after();
+          mm.scores(s_at(t), qa, tile(2 * t));
+          mma_commit(&bars.s_full[t & 1]);
+        };
+        auto grads = [&](int64_t t, bool last) {
+          if (!ready(2 * t + 1)) return;
+          fence_after();
+          mm.scores(t_dp, ga, tile(2 * t + 1));
+          mma_commit(&bars.dp_full);
+          mma_commit(&bars.empty[(2 * t + 1) % kStages]);
+          if (last) mma_commit(&bars.q_empty);
+        };
+        scores(done);
+        grads(done, tiles.n == 1);
+        for (int t = 0; ok && t < tiles.n; ++t) {
+          const int64_t e = done + t;
+          if (t + 1 < tiles.n) scores(e + 1);
+          if (!(ok = ok && bar_wait(&bars.ds_full, (uint32_t)(e & 1), stop, p.error))) break;
+          fence_after();
+          mm.sums(t_dq, t_dp, tile(2 * e), t > 0);
+          mma_commit(&bars.empty[2 * e % kStages]);
+          if (t + 1 < tiles.n) grads(e + 1, t + 2 == tiles.n);
+        }
+        mma_commit(&bars.dq_full);
+        done += tiles.n;
+      }
+    }
+  } else if (warp >= 4) {
+    const int half = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    const float c = w.c.scale * kLog2e;
+    const float2 minus_c = make_float2(-c, -c), minus_1 = make_float2(-1.f, -1.f);
+    int64_t done = 0;
+    uint32_t dq_phase = 0;
+    bool ok = true;
+    for (int64_t x = blockIdx.x; ok && x < p.items; x += gridDim.x) {
+      int b, h, i0;
+      item(x, b, h, i0);
+      const KeyTiles<kT> tiles(key_range(w, b, i0, i0 + kT - 1));
+      const int i = i0 + row;
+      const bool inside = i < w.c.q_len;
+      const QuerySpan span = query_span(w, b, i);
+      const int all_low = __reduce_max_sync(~0u, span.p < 0 ? INT_MAX : span.low);
+      const int all_end = __reduce_min_sync(~0u, span.p < 0 ? -1 : span.p) + 1;
+      const int64_t stat = ((int64_t)b * w.c.q_heads + h) * w.lse_row + i;
+      const float lse = inside ? w.c.lse[stat] : INFINITY, delta = inside ? w.c.delta[stat] : 0.f;
+      const float2 lse2 = make_float2(lse, lse), delta2 = make_float2(delta, delta);
+      for (int t = 0; t < tiles.n; ++t) {
+        const int64_t e = done + t;
+        const int j0 = tiles.first(t) + half * 64, j1 = tiles.end(t);
+        const bool masked = !(j0 >= all_low && j0 + 64 <= all_end && j1 - j0 >= 64);
+        uint32_t seen[2];
+        {
+          const int b0 = span.low - j0, b1 = min(span.p + 1, j1) - j0, s0 = span.start - j0,
+                    s1 = min(span.sink_end, j1) - j0;
+          seen[0] = bits(b0, b1, 0) | bits(s0, s1, 0), seen[1] = bits(b0, b1, 32) | bits(s0, s1, 32);
+        }
+        if (!(ok = bar_wait(&bars.s_full[e & 1], (uint32_t)(e >> 1 & 1), stop, p.error))) break;
+        fence_after();
+        const uint32_t t_s = tmem + (uint32_t)(e & 1) * 128 + lanes + half * 64, t_d = t_dp + lanes + half * 64;
+        float2 pr[32];
+        {
+          uint32_t z[2][16];
+          tmem_ld16(t_s, z[0]);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            wait_ld();
+            if (y < 3) tmem_ld16(t_s + (y + 1) * 16, z[(y + 1) & 1]);
+            uint32_t *zz = z[y & 1];
+            tie16(zz);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              const int col = y * 16 + 2 * u;
+              float2 f = fma2(make_float2(__uint_as_float(zz[2 * u]), __uint_as_float(zz[2 * u + 1])), minus_c, lse2);
+              f.x = exp2_fast(-f.x), f.y = exp2_fast(-f.y);
+              if (masked) {
+                if (!(seen[col >> 5] >> (col & 31) & 1)) f.x = 0.f;
+                if (!(seen[col >> 5] >> (col & 31) & 2)) f.y = 0.f;
+              }
+              pr[y * 8 + u] = f;
+            }
+          }
+        }
+        if (!(ok = bar_wait(&bars.dp_full, (uint32_t)(e & 1), stop, p.error))) break;
+        fence_after();
+        {
+          uint32_t z[2][16], pk[16];
+          tmem_ld16(t_d, z[0]);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            wait_ld();
+            if (y < 3) tmem_ld16(t_d + (y + 1) * 16, z[(y + 1) & 1]);
+            uint32_t *zz = z[y & 1];
+            tie16(zz);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              const int col = y * 16 + 2 * u;
+              // delta - dP: minus dS; the sign goes at the end
+              float2 f = fma2(make_float2(__uint_as_float(zz[2 * u]), __uint_as_float(zz[2 * u + 1])), minus_1, delta2);
+              f = mul2(f, pr[y * 8 + u]);
+              if (masked) {
+                if (!(seen[col >> 5] >> (col & 31) & 1)) f.x = 0.f;
+                if (!(seen[col >> 5] >> (col & 31) & 2)) f.y = 0.f;
+              }
+              pk[(y & 1) * 8 + u] = pack2<BF16>(f.x, f.y);
+            }
+            if (y & 1) tmem_st16(t_d + (y >> 1) * 16, pk);
+          }
+        }
+        wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&bars.ds_full);
+      }
+      if (!ok) break;
+      done += tiles.n;
+      if (tiles.n > 0) {
+        if (!(ok = bar_wait(&bars.dq_full, dq_phase, stop, p.error))) break;
+        dq_phase ^= 1;
+        fence_after();
+      }
+      T *dq = static_cast<T *>(w.c.dq) + ((b * w.c.q_len + i) * w.c.q_heads + h) * w.c.dim;
+      const int d0 = half * DB * 32;
+      bool bad = false;
+#pragma unroll 1
+      for (int d = d0; d < d0 + DB * 32; d += 32) {
+        uint32_t o[32];
+        if (tiles.n > 0) {
+          tmem_ld32(t_dq + lanes + d, o);
+          wait_ld();
+          tie32(o);
+        } else {
+#pragma unroll
+          for (int y = 0; y < 32; ++y) o[y] = 0;
+        }
+        bad = store32<T>(dq, o, -w.c.scale, d, w.c.dim, inside) || bad;
+      }
+      if (__any_sync(~0u, bad && inside)) {
+        bool hidden = false;
+        const PairDots<T> pair(w, b, h, 0, 0);
+        for (int t = 0; t < tiles.n; ++t) {
+          const int j0 = tiles.first(t);
+          if (j0 >= all_low && j0 + kT <= all_end && tiles.end(t) - j0 == kT) continue;
+          for (int y = 0; y < kT; y += 32) {
+            const bool odd = row_not_finite(pair.k, w.c.k.token, j0 + y + lane, w.c.k_len, w.c.dim);
+            for (unsigned left = __ballot_sync(~0u, odd); left; left &= left - 1) {
+              const int j = j0 + y + __ffs(left) - 1;
+              hidden = hidden || j >= tiles.end(t) || !span.sees(j);
+            }
+          }
+        }
+        for (unsigned left = __ballot_sync(~0u, bad && inside && hidden); left; left &= left - 1)
+          repair_dq<T>(w, b, h, i - lane + __ffs(left) - 1, d0, d0 + DB * 32);
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (threadIdx.x == 0 && *stop) drain(bars.full, kStages);
+  __syncthreads();
+  if (warp == 2) tmem_free(tmem, 512);
+}
+
+template <typename T, int DB> void launch(Params &p, cudaStream_t s) {
+  const WindowProblem &w = p.w;
+  if (w.c.dq && w.c.q_len > 0) {
+    auto kernel = dq_tc_kernel<T, DB>;
+    MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kQSmem<DB>));
+    kernel<<<(unsigned)std::min<int64_t>(p.items, num_sms()), kThreads, kQSmem<DB>, s>>>(p);
+    MSX_CHECK_LAUNCH();
+  }
+  if (w.c.dk) {
+    auto kernel = dkv_tc_kernel<T, DB>;
+    // The tiles of the first keys come first: sinks are seen by all that follow,
+    // so theirs are the longest.
+    const int64_t grid = ceil_div(w.c.k_len, kT) * w.c.batch * w.c.k_heads;
+    if (grid > INT32_MAX) fail(MSX_ERR_OVERFLOW, "window_attention has too many key tiles for one call.");
+    MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKvSmem<DB>));
+    kernel<<<(unsigned)grid, kThreads, kKvSmem<DB>, s>>>(p);
+    MSX_CHECK_LAUNCH();
+  }
+}
+
+}  // namespace
+
+void window_backward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s) {
+  if (w.c.batch == 0) return;
+  if (w.c.q_len == 0) return window_backward_general(w, value_dtype, s);  // zeros
+  window_delta(w, value_dtype, s);
+  Params p{};
+  p.w = w;
+  const bool bf16 = value_dtype == MSX_BF16;
+  const int64_t heads = w.c.q_heads, dim = w.c.dim;
+  const WindowTensor g{w.c.grad_out, w.c.q_len * heads * dim, heads * dim, dim};
+  p.q = make_map(w.c.q, w.c.batch, w.c.q_len, heads, dim, bf16, kT);
+  p.g = make_map(g, w.c.batch, w.c.q_len, heads, dim, bf16, kT);
+  p.k = make_map(w.c.k, w.c.batch, w.c.k_len, w.c.k_heads, dim, bf16, kT);
+  p.v = make_map(w.c.v, w.c.batch, w.c.k_len, w.c.k_heads, dim, bf16, kT);
+  p.q_tiles = (int)ceil_div(w.c.q_len, kT);
+  p.items = w.c.batch * heads * p.q_tiles;
+  p.error = window_error_flag();
+  if (bf16) {
+    if (dim <= 64) launch<__nv_bfloat16, 1>(p, s); else launch<__nv_bfloat16, 2>(p, s);
+  } else {
+    if (dim <= 64) launch<__half, 1>(p, s); else launch<__half, 2>(p, s);
+  }
+}
+
+}  // namespace msx

@@ -24,12 +24,9 @@
 // Bound: the exponentials (16 a clock and SM: 1024 clocks for 128 x 128 scores)
 // and the products (2 x 512 clocks at head size 128) take the same time, side
 // by side.
-#include <cudaTypedefs.h>
-
 #include <algorithm>
 
-#include "tc.cuh"
-#include "window_attention.cuh"
+#include "window_tc.cuh"
 
 namespace msx {
 
@@ -42,8 +39,6 @@ __device__ int g_window_error;
 constexpr int kM = 128;  // queries of a slot: the lanes of tensor memory
 constexpr int kN = 128;  // keys of a tile
 constexpr int kThreads = 384;
-constexpr int kBox = 128 * 128;  // bytes of a TMA box: 128 rows of 64 elements
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <int DB> struct Shape {  // DB boxes of 64 elements cover the head size
   static constexpr int tile = DB * kBox;
@@ -109,45 +104,6 @@ __device__ __forceinline__ Item item_of(const Params &p, int64_t n) {
   return it;
 }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Two fp32 operations for one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
-      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n"
-      " mov.b64 {%0, %1}, x;\n}\n"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-
-template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if (BF16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-  }
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-// Bits [lo, hi) of the 32 that start at bit `from`.
-__device__ __forceinline__ uint32_t bits(int lo, int hi, int from) {
-  lo = max(lo - from, 0), hi = min(hi - from, 32);
-  return hi <= lo ? 0u : (~0u >> (32 - hi)) & (~0u << lo);
-}
-
 // One row again, by a warp, pair by pair: only what the query sees is touched.
 template <typename T>
 __device__ __noinline__ void repair_row(const WindowProblem &w, int b, int h, int i) {
@@ -191,7 +147,7 @@ __device__ __noinline__ void repair_row(const WindowProblem &w, int b, int h, in
 #pragma unroll
   for (int x = 0; x < 4; ++x)
     if (x * 32 + lane < dim) out[x * 32 + lane] = VT<T>::store(acc[x] / l);
-  if (w.c.lse && lane == 0) w.c.lse[((int64_t)b * w.c.q_heads + h) * w.c.q_len + i] = m + log2f(l);
+  if (w.c.lse && lane == 0) w.c.lse[((int64_t)b * w.c.q_heads + h) * w.lse_row + i] = m + log2f(l);
 }
 
 template <typename T, int DB>
@@ -464,9 +420,26 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         }
       }
       if (inside && w.c.lse)
-        w.c.lse[((int64_t)it.b * w.c.q_heads + h) * w.c.q_len + i] = empty ? INFINITY : m * c + log2f(l);
-      for (unsigned left = __ballot_sync(~0u, bad && inside); left; left &= left - 1)
-        repair_row<T>(w, it.b, h, i - lane + __ffs(left) - 1);
+        w.c.lse[((int64_t)it.b * w.c.q_heads + h) * w.lse_row + i] = empty ? INFINITY : m * c + log2f(l);
+      if (__any_sync(~0u, bad && inside)) {
+        // What the row sees may be at fault; recompute it only if something not
+        // finite hides among the tiles' other keys.
+        bool hidden = false;
+        const T *v = static_cast<const T *>(w.c.v.ptr) + it.b * w.c.v.batch + it.hk * w.c.v.head;
+        for (int t = 0; t < tiles.n; ++t) {
+          const int j0 = tiles.first(t);
+          if (!range.touches(j0, tiles.end(t)) || (j0 >= all_low && j0 + kN <= all_end && tiles.end(t) - j0 == kN)) continue;
+          for (int x = 0; x < kN; x += 32) {
+            const unsigned flags = __ballot_sync(~0u, row_not_finite(v, w.c.v.token, j0 + x + lane, w.c.k_len, w.c.dim));
+            for (unsigned left = flags; left; left &= left - 1) {
+              const int j = j0 + x + __ffs(left) - 1;
+              hidden = hidden || j >= tiles.end(t) || !span.sees(j);
+            }
+          }
+        }
+        for (unsigned left = __ballot_sync(~0u, bad && inside && hidden); left; left &= left - 1)
+          repair_row<T>(w, it.b, h, i - lane + __ffs(left) - 1);
+      }
     }
   }
   fence_before();
@@ -480,47 +453,11 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
   if (warp == 2) tmem_free(tmem, 512);
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void *f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      f = nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-  }();
-  return fn;
-}
-
-// Boxes of 64 elements by `rows` tokens of one head; what lies outside the
-// tensor (elements past the head size, tokens past the end) reads as 0.
-CUtensorMap make_map(const WindowTensor &t, int64_t batch, int64_t tokens, int64_t heads, int64_t dim, bool bf16,
-                     int rows) {
-  PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
-  if (fn == nullptr) fail(MSX_ERR_RUNTIME, "the driver does not offer cuTensorMapEncodeTiled.");
-  CUtensorMap map;
-  const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)tokens, (cuuint64_t)heads, (cuuint64_t)batch};
-  const cuuint64_t strides[3] = {(cuuint64_t)t.token * 2, (cuuint64_t)t.head * 2, (cuuint64_t)t.batch * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, step[4] = {1, 1, 1, 1};
-  const CUresult r = fn(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                        const_cast<void *>(t.ptr), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) fail(MSX_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r) + ".");
-  return map;
-}
-
 template <typename T, int DB> void launch(Params &p, cudaStream_t s) {
   auto kernel = forward_tc_kernel<T, DB>;
   MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DB>::smem));
   kernel<<<(unsigned)std::min<int64_t>(p.items, num_sms()), kThreads, Shape<DB>::smem, s>>>(p);
   MSX_CHECK_LAUNCH();
-}
-
-bool tma_ready(const WindowTensor &t) {
-  const int64_t most = (int64_t)1 << 39;  // elements; strides stay below 2^40 bytes
-  auto good = [&](int64_t x) { return x > 0 && x % 8 == 0 && x < most; };
-  return reinterpret_cast<uintptr_t>(t.ptr) % 16 == 0 && good(t.batch) && good(t.token) && good(t.head);
 }
 
 }  // namespace

@@ -1,0 +1,109 @@
+// What the tensor-core kernels of windowed attention share.
+#pragma once
+#include <cudaTypedefs.h>
+
+#include <type_traits>
+
+#include "tc.cuh"
+#include "window_attention.cuh"
+
+namespace msx {
+
+constexpr int kBox = 128 * 128;  // bytes of a TMA box: 128 rows of 64 elements
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ex2.approx: within 2 ulp; results below 2^-126 are flushed to 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two fp32 operations for one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n"
+      " mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Bits [lo, hi) of the 32 that start at bit `from`.
+__device__ __forceinline__ uint32_t bits(int lo, int hi, int from) {
+  lo = max(lo - from, 0), hi = min(hi - from, 32);
+  return hi <= lo ? 0u : (~0u >> (32 - hi)) & (~0u << lo);
+}
+
+// Whether row t of a 16-bit matrix (dim elements from `p`, a multiple of 8,
+// 16-byte aligned) holds an infinity or a NaN; rows outside [0, limit) do not.
+template <typename T> __device__ inline bool row_not_finite(const T *p, int64_t token_stride, int64_t t, int64_t limit, int dim) {
+  if (t < 0 || t >= limit) return false;
+  const uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  const uint4 *v = reinterpret_cast<const uint4 *>(p + t * token_stride);
+  bool bad = false;
+  for (int x = 0; x < dim / 8; ++x) {
+    const uint4 u = v[x];
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int y = 0; y < 4; ++y) bad = bad || (w[y] & e & 0xffffu) == (e & 0xffffu) || (w[y] & e & 0xffff0000u) == (e & 0xffff0000u);
+  }
+  return bad;
+}
+
+// ---- host ---------------------------------------------------------------------
+inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void *f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return fn;
+}
+
+// Boxes of 64 elements by `rows` tokens of one head; what lies outside the
+// tensor (elements past the head size, tokens past the end) reads as 0.
+inline CUtensorMap make_map(const WindowTensor &t, int64_t batch, int64_t tokens, int64_t heads, int64_t dim, bool bf16,
+                     int rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
+  if (fn == nullptr) fail(MSX_ERR_RUNTIME, "the driver does not offer cuTensorMapEncodeTiled.");
+  CUtensorMap map;
+  const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)tokens, (cuuint64_t)heads, (cuuint64_t)batch};
+  const cuuint64_t strides[3] = {(cuuint64_t)t.token * 2, (cuuint64_t)t.head * 2, (cuuint64_t)t.batch * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  const CUresult r = fn(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                        const_cast<void *>(t.ptr), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) fail(MSX_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r) + ".");
+  return map;
+}
+
+// Strides and base that a tensor map takes.
+inline bool tma_ready(const WindowTensor &t) {
+  const int64_t most = (int64_t)1 << 39;  // elements; strides stay below 2^40 bytes
+  auto good = [&](int64_t x) { return x > 0 && x % 8 == 0 && x < most; };
+  return reinterpret_cast<uintptr_t>(t.ptr) % 16 == 0 && good(t.batch) && good(t.token) && good(t.head);
+}
+
+}  // namespace msx

@@ -628,7 +628,8 @@ def window_attention_forward(q, k, v, window, sinks, scale, indptr=None, *, with
     q, k, v = heads_of(q), heads_of(k), heads_of(v)
     indptr = None if indptr is None else indptr.contiguous()
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=dev) if with_lse else None
+    rows = (q.shape[1] + 127) // 128 * 128  # the kernels read whole tiles of it
+    lse = torch.empty((q.shape[0], q.shape[2], rows), dtype=torch.float32, device=dev) if with_lse else None
     with torch.cuda.device(dev):
         check(L.msx_window_attention_forward(*_window_args(q, k, v, window, sinks, scale, indptr), _p(out), _p(lse),
                                              stream_ptr(dev)))
