@@ -112,20 +112,32 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) forward_ker
   }
 }
 
-// delta_i = dO_i . O_i, a warp for each row and head. O is the rounded output:
-// the error that brings (half a step of O's type, times dO) is of the size of
-// the rounding of the gradients themselves.
-template <typename T> __global__ void delta_kernel(const WindowProblem w) {
-  const int64_t x = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (x >= w.c.batch * w.c.q_len * w.c.q_heads) return;
-  const T *o = static_cast<const T *>(w.c.out) + x * w.c.dim, *g = static_cast<const T *>(w.c.grad_out) + x * w.c.dim;
+// delta_i = dO_i . O_i, 16 lanes for each row and head, VEC elements at a time.
+// O is the rounded output: the error that brings (half a step of O's type, times
+// dO) is of the size of the rounding of the gradients themselves.
+template <typename T, int VEC> __global__ void delta_kernel(const WindowProblem w) {
+  const int64_t x = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
+  const int lane = threadIdx.x & 15;
+  const bool inside = x < w.c.batch * w.c.q_len * w.c.q_heads;
   float s = 0.f;
-  for (int d = lane; d < w.c.dim; d += 32) s = fmaf(VT<T>::load(o[d]), VT<T>::load(g[d]), s);
+  if (inside) {
+    const T *o = static_cast<const T *>(w.c.out) + x * w.c.dim, *g = static_cast<const T *>(w.c.grad_out) + x * w.c.dim;
+    for (int d = lane * VEC; d < w.c.dim; d += 16 * VEC) {
+      alignas(16) T a[VEC], b[VEC];
+      if (VEC > 1) {
+        *reinterpret_cast<uint4 *>(a) = __ldcs(reinterpret_cast<const uint4 *>(o + d));
+        *reinterpret_cast<uint4 *>(b) = __ldcs(reinterpret_cast<const uint4 *>(g + d));
+      } else {
+        a[0] = o[d], b[0] = g[d];
+      }
 #pragma unroll
-  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+      for (int y = 0; y < VEC; ++y) s = fmaf(VT<T>::load(a[y]), VT<T>::load(b[y]), s);
+    }
+  }
+#pragma unroll
+  for (int d = 8; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
   const int64_t h = x % w.c.q_heads, bi = x / w.c.q_heads, b = bi / w.c.q_len, i = bi % w.c.q_len;
-  if (lane == 0) w.c.delta[(b * w.c.q_heads + h) * w.lse_row + i] = s;
+  if (inside && lane == 0) w.c.delta[(b * w.c.q_heads + h) * w.lse_row + i] = s;
 }
 
 template <typename T> __global__ void __launch_bounds__(kWarps * 32) dq_kernel(const WindowProblem w) {
@@ -283,10 +295,17 @@ void window_forward_general(const WindowProblem &w, int value_dtype, cudaStream_
 }
 
 void window_delta(const WindowProblem &w, int value_dtype, cudaStream_t s) {
-  const int64_t warps = w.c.batch * w.c.q_len * w.c.q_heads;
-  if (warps == 0) return;
+  const int64_t rows = w.c.batch * w.c.q_len * w.c.q_heads;
+  if (rows == 0) return;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(w.c.out) | reinterpret_cast<uintptr_t>(w.c.grad_out);
   dispatch_value(value_dtype, [&](auto v) {
-    delta_kernel<decltype(v)><<<(unsigned)ceil_div(warps, 8), 256, 0, s>>>(w);
+    using T = decltype(v);
+    constexpr int kVec = 16 / sizeof(T);
+    const unsigned grid = (unsigned)ceil_div(rows, 16);
+    if (w.c.dim % kVec == 0 && at % 16 == 0)
+      delta_kernel<T, kVec><<<grid, 256, 0, s>>>(w);
+    else
+      delta_kernel<T, 1><<<grid, 256, 0, s>>>(w);
     MSX_CHECK_LAUNCH();
   });
 }
@@ -320,7 +339,7 @@ void window_forward_run(int value_dtype, const WindowCall &c, cudaStream_t s) {
 }
 
 void window_decode_run(int value_dtype, const WindowCall &c, cudaStream_t s) {
-  window_forward_general(problem(c), value_dtype, s);
+  window_decode(problem(c), value_dtype, s);
 }
 
 void window_backward_run(int value_dtype, const WindowCall &c, cudaStream_t s) {
