@@ -68,7 +68,7 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, scale=None, indptr
 
         out = WindowAttention.apply(q, k, v, int(window), int(sinks), scale, indptr)
     else:
-        out, _ = _native.window_attention_forward(q, k, v, window, sinks, scale, indptr, with_lse=False)
+        out, _ = _native.window_attention_forward(q, k, v, int(window), int(sinks), scale, indptr, with_lse=False)
     return out if indptr is None else out.squeeze(0)
 
 
@@ -99,4 +99,4 @@ def window_attention_decode(q, k_cache, v_cache, lengths, *, window: int, sinks:
                          f"{k_cache.shape[0]} and {lengths.shape[0]}.")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise ValueError(f"{name} has no gradient; use window_attention, or call it under torch.no_grad().")
-    return _native.window_attention_decode(q, k_cache, v_cache, lengths, window, sinks, scale)
+    return _native.window_attention_decode(q, k_cache, v_cache, lengths, int(window), int(sinks), scale)

@@ -12,6 +12,7 @@ library or a CUDA device is missing, every op raises ``RuntimeError``.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -559,9 +560,9 @@ def csr_distill_forward(data, indices, indptr, logits, temperature, *, with_stat
     data, indices, indptr, logits = data.contiguous(), indices.contiguous(), indptr.contiguous(), rows_of(logits)
     loss = torch.empty(logits.shape[0], dtype=torch.float32, device=dev)
     stats = torch.empty((logits.shape[0], 4), dtype=torch.float32, device=dev) if with_stats else None
-    with torch.cuda.device(dev):
+    with _on(dev):
         check(L.msx_csr_distill_forward(*_distill_args(data, indices, indptr, logits, temperature), _p(loss),
-                                        _p(stats), stream_ptr(dev)))
+                                        _p(stats), _stream(dev)))
     return loss, stats
 
 
@@ -571,9 +572,9 @@ def csr_distill_backward(data, indices, indptr, logits, temperature, stats, cota
     data, indices, indptr, logits = data.contiguous(), indices.contiguous(), indptr.contiguous(), rows_of(logits)
     cotangent = cotangent.contiguous()
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         check(L.msx_csr_distill_backward(*_distill_args(data, indices, indptr, logits, temperature), _p(stats),
-                                         _p(cotangent), _p(grad), stream_ptr(dev)))
+                                         _p(cotangent), _p(grad), _stream(dev)))
     return grad
 
 
@@ -584,71 +585,104 @@ def csr_distill_forward_backward(data, indices, indptr, logits, temperature, cot
     cotangent = None if cotangent is None else cotangent.contiguous()
     loss = torch.empty(logits.shape[0], dtype=torch.float32, device=dev)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         check(L.msx_csr_distill_forward_backward(*_distill_args(data, indices, indptr, logits, temperature),
-                                                 _p(cotangent), _p(loss), _p(grad), stream_ptr(dev)))
+                                                 _p(cotangent), _p(loss), _p(grad), _stream(dev)))
     return loss, grad
 
 
-def _strides(t, dims):
-    """Element strides of ``t`` along ``dims`` as a C array; a dimension of
-    one element (or none) has the stride a contiguous tensor would have."""
-    out, span = {}, 1
-    for d in range(t.ndim - 1, -1, -1):
-        out[d] = t.stride(d) if t.shape[d] > 1 else span
-        span *= max(1, t.shape[d])
-    return (ctypes.c_int64 * len(dims))(*(out[d] for d in dims))
+_NO_GUARD = contextlib.nullcontext()
+_Strides = ctypes.c_int64 * 9
+
+
+# The raw handle of the current stream, without a Stream object on the way.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
+def _stream(dev):
+    return _raw_stream(dev.index) if _raw_stream is not None else stream_ptr(dev)
+
+
+def _on(dev):
+    """Makes ``dev`` the current device where it is not already."""
+    return _NO_GUARD if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _strides(t):
+    """Element strides of ``t`` but for its last dimension; a dimension of one
+    element (or none) has the stride a contiguous tensor would have."""
+    if t.is_contiguous() and 0 not in t.shape:
+        span, out = t.shape[-1], []
+        for n in t.shape[-2::-1]:
+            out.append(span)
+            span *= n
+        return out[::-1]
+    span, out = max(1, t.shape[-1]), []
+    for n, step in zip(t.shape[-2::-1], t.stride()[-2::-1]):
+        out.append(step if n > 1 else span)
+        span *= max(1, n)
+    return out[::-1]
 
 
 def heads_of(t):
     """``t`` (..., heads, dim) as the attention kernels read it: stride 1 along
     dim. 16-bit tensors whose rows start on 16-byte boundaries go to the
     tensor cores as they are; others (and broadcast ones) are copied."""
+    if t.is_contiguous():
+        return t.clone() if t.data_ptr() % 16 and t.element_size() == 2 and t.shape[-1] % 8 == 0 else t
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         return t.contiguous()
     if t.element_size() == 2 and t.shape[-1] % 8 == 0 and t.numel():
-        loose = any(t.shape[d] > 1 and (t.stride(d) % 8 or t.stride(d) == 0) for d in range(t.ndim - 1))
-        if loose or t.data_ptr() % 16:
-            return t.contiguous() if loose or not t.is_contiguous() else t.clone()
+        if t.data_ptr() % 16 or any(n > 1 and (step % 8 or step == 0) for n, step in zip(t.shape[:-1], t.stride())):
+            return t.contiguous()
     return t
 
 
 def _window_args(q, k, v, window, sinks, scale, indptr):
     b, q_len, q_heads, dim = q.shape
-    qs, ks, vs = (_strides(t, (0, 1, 2)) for t in (q, k, v))
-    return [VALUE_CODES[q.dtype], _p(q), qs, _p(k), ks, _p(v), vs, b, q_len, k.shape[1], q_heads, k.shape[2], dim,
-            int(window), int(sinks), float(scale), INDEX_CODES[indptr.dtype] if indptr is not None else MSX_I32,
-            _p(indptr), indptr.numel() - 1 if indptr is not None else 0]
+    _, k_len, k_heads, _ = k.shape
+    st = _Strides(*_strides(q), *_strides(k), *_strides(v))
+    at = ctypes.addressof(st)
+    # st comes last, outside the call's arguments: it lives as long as they do
+    args = [VALUE_CODES[q.dtype], q.data_ptr(), at, k.data_ptr(), at + 24, v.data_ptr(), at + 48, b, q_len, k_len,
+            q_heads, k_heads, dim, window, sinks, scale]
+    if indptr is None:
+        args += [MSX_I32, None, 0]
+    else:
+        args += [INDEX_CODES[indptr.dtype], indptr.data_ptr(), indptr.shape[0] - 1]
+    return args, st
 
 
 def window_attention_forward(q, k, v, window, sinks, scale, indptr=None, *, with_lse: bool):
     """Rank-4 ``q``, ``k``, ``v``; returns ``(out, lse)`` (lse None unless wanted)."""
     L = extension()
-    dev = require_cuda(q, k, v, *(() if indptr is None else (indptr,)))
+    dev = require_cuda(q, k, v) if indptr is None else require_cuda(q, k, v, indptr)
     q, k, v = heads_of(q), heads_of(k), heads_of(v)
     indptr = None if indptr is None else indptr.contiguous()
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    rows = (q.shape[1] + 127) // 128 * 128  # the kernels read whole tiles of it
-    lse = torch.empty((q.shape[0], q.shape[2], rows), dtype=torch.float32, device=dev) if with_lse else None
-    with torch.cuda.device(dev):
-        check(L.msx_window_attention_forward(*_window_args(q, k, v, window, sinks, scale, indptr), _p(out), _p(lse),
-                                             stream_ptr(dev)))
+    out = q.new_empty(q.shape)
+    lse = None
+    if with_lse:  # the kernels read whole tiles of it
+        lse = torch.empty((q.shape[0], q.shape[2], (q.shape[1] + 127) // 128 * 128), dtype=torch.float32, device=dev)
+    args, _keep = _window_args(q, k, v, window, sinks, scale, indptr)
+    with _on(dev):
+        check(L.msx_window_attention_forward(*args, out.data_ptr(), _p(lse), _stream(dev)))
     return out, lse
 
 
 def window_attention_backward(q, k, v, out, lse, grad, window, sinks, scale, indptr=None, *, want_q=True,
                               want_kv=True):
     L = extension()
-    dev = require_cuda(q, k, v, out, lse, grad, *(() if indptr is None else (indptr,)))
+    dev = require_cuda(q, k, v, out, lse, grad)
     q, k, v = heads_of(q), heads_of(k), heads_of(v)
     indptr = None if indptr is None else indptr.contiguous()
     grad = heads_of(grad.contiguous())
     delta = torch.empty_like(lse)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if want_q else None
-    dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=dev) if want_kv else None for _ in range(2))
-    with torch.cuda.device(dev):
-        check(L.msx_window_attention_backward(*_window_args(q, k, v, window, sinks, scale, indptr), _p(out), _p(lse),
-                                              _p(grad), _p(delta), _p(dq), _p(dk), _p(dv), stream_ptr(dev)))
+    dq = q.new_empty(q.shape) if want_q else None
+    dk, dv = (k.new_empty(k.shape), k.new_empty(k.shape)) if want_kv else (None, None)
+    args, _keep = _window_args(q, k, v, window, sinks, scale, indptr)
+    with _on(dev):
+        check(L.msx_window_attention_backward(*args, out.data_ptr(), lse.data_ptr(), grad.data_ptr(), delta.data_ptr(),
+                                              _p(dq), _p(dk), _p(dv), _stream(dev)))
     return dq, dk, dv
 
 
@@ -656,12 +690,14 @@ def window_attention_decode(q, k_cache, v_cache, lengths, window, sinks, scale):
     L = extension()
     dev = require_cuda(q, k_cache, v_cache, lengths)
     q, k_cache, v_cache, lengths = heads_of(q), heads_of(k_cache), heads_of(v_cache), lengths.contiguous()
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    out = q.new_empty(q.shape)
     b, q_heads, dim = q.shape
-    with torch.cuda.device(dev):
-        check(L.msx_window_attention_decode(VALUE_CODES[q.dtype], _p(q), _strides(q, (0, 1)), _p(k_cache),
-                                            _strides(k_cache, (0, 1, 2)), _p(v_cache), _strides(v_cache, (0, 1, 2)), b,
-                                            k_cache.shape[1], q_heads, k_cache.shape[2], dim, int(window), int(sinks),
-                                            float(scale), INDEX_CODES[lengths.dtype], _p(lengths), _p(out),
-                                            stream_ptr(dev)))
+    _, top, k_heads, _ = k_cache.shape
+    st = _Strides(*_strides(q), 0, *_strides(k_cache), *_strides(v_cache))
+    at = ctypes.addressof(st)
+    with _on(dev):
+        check(L.msx_window_attention_decode(VALUE_CODES[q.dtype], q.data_ptr(), at, k_cache.data_ptr(), at + 24,
+                                            v_cache.data_ptr(), at + 48, b, top, q_heads, k_heads, dim, window, sinks,
+                                            scale, INDEX_CODES[lengths.dtype], lengths.data_ptr(), out.data_ptr(),
+                                            _stream(dev)))
     return out
