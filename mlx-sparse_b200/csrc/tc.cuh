@@ -143,13 +143,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
 //  MN-major (the box's 64 elements run along M/N): atoms along K every 1024
 //           bytes, the next 64 of M/N `box_bytes` further; 16 rows of K are
 //           2048 bytes further on.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead_bytes, uint32_t stride_bytes) {
-  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lead_bytes >> 4) & 0x3fff) << 16 |
-         (uint64_t)((stride_bytes >> 4) & 0x3fff) << 32 | 1ull << 46 | 2ull << 61;
-}
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) { return smem_desc(addr, 16, 1024); }
-__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t box_bytes) {
-  return smem_desc(addr, box_bytes, 1024);
+// A descriptor's upper word is the same for all (atoms 1024 bytes apart); the
+// lower holds the address and the distance of M/N boxes, and steps along K add
+// to it.
+constexpr uint32_t kDescHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_k_major(uint32_t addr) { return addr >> 4 | 1u << 16; }
+__device__ __forceinline__ uint32_t desc_mn_major(uint32_t addr, uint32_t box_bytes) {
+  return addr >> 4 | (box_bytes >> 4) << 16;
 }
 
 // Instruction descriptor of kind::f16 with fp32 accumulation; both operands are
@@ -158,20 +158,32 @@ __host__ __device__ constexpr uint32_t mma_desc(bool bf16, int m, int n, bool a_
   return 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (a_mn ? 1u : 0u) << 15 | (b_mn ? 1u : 0u) << 16 |
          (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool accumulate) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-               "l"(a), "l"(b), "r"(desc), "r"((uint32_t)accumulate)
-               : "memory");
+// a, b: lower descriptor words; mma_ts: a is an address in tensor memory. The
+// whole warp runs these with the same operands, which keeps them in uniform
+// registers; the one lane with `leader` issues.
+__device__ __forceinline__ void mma_ss(bool leader, uint32_t d, uint32_t a, uint32_t b, uint32_t desc, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .b64 x, y;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %6, 0;\n"
+      " mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(desc), "r"((uint32_t)accumulate), "r"(kDescHigh), "r"((uint32_t)leader)
+      : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool accumulate) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-               "r"(a), "l"(b), "r"(desc), "r"((uint32_t)accumulate)
-               : "memory");
+__device__ __forceinline__ void mma_ts(bool leader, uint32_t d, uint32_t a, uint32_t b, uint32_t desc, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .b64 y;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %6, 0;\n"
+      " mov.b64 y, {%2, %5};\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(desc), "r"((uint32_t)accumulate), "r"(kDescHigh), "r"((uint32_t)leader)
+      : "memory");
 }
 // Arrives at `bar` when every product issued so far by this thread is done.
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-               : "memory");
+__device__ __forceinline__ void mma_commit(bool leader, uint64_t *bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_addr(bar)),
+      "r"((uint32_t)leader)
+      : "memory");
 }
 
 }  // namespace tc

@@ -136,32 +136,6 @@ __device__ __noinline__ void repair_dkv(const WindowProblem &w, int b, int hk, i
     if (y * 32 + lane < w.c.dim) out[y * 32 + lane] = VT<T>::store(acc[y] * (keys ? w.c.scale : 1.f));
 }
 
-// Products issued by one thread. Scores: both operands K-major in shared
-// memory. Sums: left operand in tensor memory, its columns 64.. at `left_hi`,
-// right operand MN-major in shared memory.
-struct Products {
-  int k_steps;
-  uint32_t scores_desc, sums_desc;
-  template <bool BF16> __device__ static Products make(int dim) {
-    Products r;
-    r.k_steps = (dim + 15) / 16;
-    r.scores_desc = mma_desc(BF16, kT, kT, false, false);
-    r.sums_desc = mma_desc(BF16, kT, r.k_steps * 16, false, true);
-    return r;
-  }
-  __device__ void scores(uint32_t d, uint32_t a, uint32_t b) const {
-    for (int x = 0; x < k_steps; ++x) {
-      const uint32_t off = (x >> 2) * kBox + (x & 3) * 32;
-      mma_ss(d, desc_k_major(a + off), desc_k_major(b + off), scores_desc, x > 0);
-    }
-  }
-  __device__ void sums(uint32_t d, uint32_t left, uint32_t b, bool add) const {
-#pragma unroll
-    for (int x = 0; x < kT / 16; ++x)
-      mma_ts(d, left + (x >> 2) * 64 + (x & 3) * 8, desc_mn_major(b + x * 2048, kBox), sums_desc, add || x > 0);
-  }
-};
-
 // Writes 32 accumulator columns of a row, scaled; true if one is not finite.
 template <typename T> __device__ __forceinline__ bool store32(T *row, uint32_t *o, float scale, int d0, int dim, bool inside) {
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
@@ -205,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
   unsigned char *k_tile = sm, *v_tile = sm + kTile, *ring = sm + 2 * kTile;
   float *row_stats = reinterpret_cast<float *>(ring + kStages * kTile);  // two of {lse[128], delta[128]}
   const WindowProblem &w = p.w;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int hk = (int)(blockIdx.x % w.c.k_heads);
   const int b = (int)(blockIdx.x / w.c.k_heads % w.c.batch);
   const int j0 = (int)(blockIdx.x / w.c.k_heads / w.c.batch) * kT;
@@ -223,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = bars.tmem, t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
+  const uint32_t tmem = __shfl_sync(~0u, bars.tmem, 0), t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
   // the tiles of queries that see any of these keys
   const int key = j0 + (warp & 3) * 32 + lane, own_last = last_query(w, key);
   if (warp >= 4 && warp < 8) {
@@ -263,8 +237,8 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
-      const Products mm = Products::make<BF16>(w.c.dim);
+    if (n > 0) {
+      const Products<DB, 64> mm(BF16, w.c.dim);
       const uint32_t ka = smem_addr(k_tile), va = smem_addr(v_tile), ra = smem_addr(ring);
       bool ok = bar_wait(&bars.kv_full, 0, stop, p.error);
       auto ready = [&](int e) { return ok = ok && bar_wait(&bars.full[e % kStages], e / kStages & 1, stop, p.error); };
@@ -272,34 +246,34 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       if (ready(0)) {
         fence_after();
         mm.scores(t_s, ka, tile(0));
-        mma_commit(&bars.s_full);
+        mma_commit(mm.leader, &bars.s_full);
       }
       if (ready(1)) {
         mm.scores(t_dp, va, tile(1));
-        mma_commit(&bars.dp_full);
+        mma_commit(mm.leader, &bars.dp_full);
       }
       for (int it = 0; ok && it < n; ++it) {
         const int q = 2 * it, g = q + 1;
         if (!(ok = bar_wait(&bars.p_full, it & 1, stop, p.error))) break;
         fence_after();
         mm.sums(t_dv, t_s, tile(g), it > 0);
-        mma_commit(&bars.empty[g % kStages]);
+        mma_commit(mm.leader, &bars.empty[g % kStages]);
         if (it + 1 < n) {
           if (!ready(q + 2)) break;
           mm.scores(t_s, ka, tile(q + 2));
-          mma_commit(&bars.s_full);
+          mma_commit(mm.leader, &bars.s_full);
         }
         if (!(ok = bar_wait(&bars.ds_full, it & 1, stop, p.error))) break;
         fence_after();
         mm.sums(t_dk, t_dp, tile(q), it > 0);
-        mma_commit(&bars.empty[q % kStages]);
+        mma_commit(mm.leader, &bars.empty[q % kStages]);
         if (it + 1 < n) {
           if (!ready(g + 2)) break;
           mm.scores(t_dp, va, tile(g + 2));
-          mma_commit(&bars.dp_full);
+          mma_commit(mm.leader, &bars.dp_full);
         }
       }
-      mma_commit(&bars.done);
+      mma_commit(mm.leader, &bars.done);
     }
   } else if (warp >= 4) {
     const int half = (warp - 4) >> 2;
@@ -448,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
   __shared__ QBars bars;
   unsigned char *q_tile = sm, *g_tile = sm + kTile, *ring = sm + 2 * kTile;
   const WindowProblem &w = p.w;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int *stop = &bars.stop;
   if (threadIdx.x == 0) {
     bar_init(&bars.q_full, 1), bar_init(&bars.q_empty, 1);
@@ -462,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = bars.tmem, t_dp = tmem + 256, t_dq = tmem + 384;  // two score tiles before them
+  const uint32_t tmem = __shfl_sync(~0u, bars.tmem, 0), t_dp = tmem + 256, t_dq = tmem + 384;  // two score tiles before them
   auto item = [&](int64_t x, int &b, int &h, int &i0) {  // heads of one key head side by side
     const int g = (int)(x % w.group);
     x /= w.group;
@@ -499,8 +473,8 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const Products mm = Products::make<BF16>(w.c.dim);
+    {
+      const Products<DB, 64> mm(BF16, w.c.dim);
       const uint32_t qa = smem_addr(q_tile), ga = smem_addr(g_tile), ra = smem_addr(ring);
       int64_t done = 0;  // tile pairs of earlier items: K of pair t is ring entry 2 (done + t), V the next
       uint32_t q_phase = 0;
@@ -521,15 +495,15 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
           if (!ready(2 * t)) return;
           fence_after();
           mm.scores(s_at(t), qa, tile(2 * t));
-          mma_commit(&bars.s_full[t & 1]);
+          mma_commit(mm.leader, &bars.s_full[t & 1]);
         };
         auto grads = [&](int64_t t, bool last) {
           if (!ready(2 * t + 1)) return;
           fence_after();
           mm.scores(t_dp, ga, tile(2 * t + 1));
-          mma_commit(&bars.dp_full);
-          mma_commit(&bars.empty[(2 * t + 1) % kStages]);
-          if (last) mma_commit(&bars.q_empty);
+          mma_commit(mm.leader, &bars.dp_full);
+          mma_commit(mm.leader, &bars.empty[(2 * t + 1) % kStages]);
+          if (last) mma_commit(mm.leader, &bars.q_empty);
         };
         scores(done);
         grads(done, tiles.n == 1);
@@ -539,10 +513,10 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
           if (!(ok = ok && bar_wait(&bars.ds_full, (uint32_t)(e & 1), stop, p.error))) break;
           fence_after();
           mm.sums(t_dq, t_dp, tile(2 * e), t > 0);
-          mma_commit(&bars.empty[2 * e % kStages]);
+          mma_commit(mm.leader, &bars.empty[2 * e % kStages]);
           if (t + 1 < tiles.n) grads(e + 1, t + 2 == tiles.n);
         }
-        mma_commit(&bars.dq_full);
+        mma_commit(mm.leader, &bars.dq_full);
         done += tiles.n;
       }
     }

@@ -38,19 +38,21 @@ __device__ int g_window_error;
 
 constexpr int kM = 128;  // queries of a slot: the lanes of tensor memory
 constexpr int kN = 128;  // keys of a tile
-constexpr int kThreads = 384;
-
-template <int DB> struct Shape {  // DB boxes of 64 elements cover the head size
-  static constexpr int tile = DB * kBox;
-  static constexpr int stages = DB == 2 ? 5 : 8;
-  static constexpr int smem = 1024 + (2 + stages) * tile;
-};
+constexpr int kSoftmaxWarps = 16;
+constexpr int kThreads = 64 + kSoftmaxWarps * 32;  // loads, products, softmax
 
 struct Bars {
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
   uint64_t kv_full[8], kv_empty[8];
   uint32_t tmem;
   int stop;
+  float row[2][2][kM];  // what the two threads of a row tell each other
+};
+
+template <int DB> struct Shape {  // DB boxes of 64 elements cover the head size
+  static constexpr int tile = DB * kBox;
+  static constexpr int stages = DB == 2 ? 5 : 8;
+  static constexpr int smem = (2 + stages) * tile + (int)sizeof(Bars);
 };
 
 struct Params {
@@ -104,9 +106,21 @@ __device__ __forceinline__ Item item_of(const Params &p, int64_t n) {
   return it;
 }
 
+// Named barriers of two warps.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool pair_any(int id, bool x) {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %2, 0;\n bar.red.or.pred q, %1, 64, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+               : "=r"(r)
+               : "r"(id), "r"((uint32_t)x)
+               : "memory");
+  return r != 0;
+}
+
 // One row again, by a warp, pair by pair: only what the query sees is touched.
+// Columns [d0, d1) are written.
 template <typename T>
-__device__ __noinline__ void repair_row(const WindowProblem &w, int b, int h, int i) {
+__device__ __noinline__ void repair_row(const WindowProblem &w, int b, int h, int i, int d0, int d1) {
   const int lane = threadIdx.x & 31, dim = w.c.dim, hk = h / w.group;
   const T *q = static_cast<const T *>(w.c.q.ptr) + b * w.c.q.batch + h * w.c.q.head + i * w.c.q.token;
   const T *k = static_cast<const T *>(w.c.k.ptr) + b * w.c.k.batch + hk * w.c.k.head;
@@ -146,7 +160,7 @@ __device__ __noinline__ void repair_row(const WindowProblem &w, int b, int h, in
   T *out = static_cast<T *>(w.c.out) + ((b * w.c.q_len + i) * w.c.q_heads + h) * dim;
 #pragma unroll
   for (int x = 0; x < 4; ++x)
-    if (x * 32 + lane < dim) out[x * 32 + lane] = VT<T>::store(acc[x] / l);
+    if (x * 32 + lane >= d0 && x * 32 + lane < min(d1, dim)) out[x * 32 + lane] = VT<T>::store(acc[x] / l);
   if (w.c.lse && lane == 0) w.c.lse[((int64_t)b * w.c.q_heads + h) * w.lse_row + i] = m + log2f(l);
 }
 
@@ -154,27 +168,30 @@ template <typename T, int DB>
 __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_constant__ Params p) {
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   using Sh = Shape<DB>;
-  extern __shared__ unsigned char raw[];
-  unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  __shared__ Bars bars;
+  extern __shared__ __align__(1024) unsigned char sm[];  // no static shared memory: all 227 KB are needed
+  Bars &bars = *reinterpret_cast<Bars *>(sm + (2 + Sh::stages) * Sh::tile);
   unsigned char *q_tile = sm, *kv_tile = sm + 2 * Sh::tile;
   const WindowProblem &w = p.w;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int *stop = &bars.stop;
+  if (smem_addr(sm) % 1024 != 0) {  // the swizzle's atoms would not lie where they are read
+    *p.error = 1;
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       bar_init(&bars.q_full[s], 1), bar_init(&bars.q_empty[s], 1);
-      bar_init(&bars.s_full[s], 1), bar_init(&bars.p_full[s], 4), bar_init(&bars.o_full[s], 1);
+      bar_init(&bars.s_full[s], 1), bar_init(&bars.p_full[s], 8), bar_init(&bars.o_full[s], 1);
     }
     for (int s = 0; s < Sh::stages; ++s) bar_init(&bars.kv_full[s], 1), bar_init(&bars.kv_empty[s], 1);
     bars.stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 2) tmem_alloc(&bars.tmem, 512);
+  if (warp == 1) tmem_alloc(&bars.tmem, 512);
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = bars.tmem;
+  const uint32_t tmem = __shfl_sync(~0u, bars.tmem, 0);
   if (warp == 0) {
     // ---- loads -------------------------------------------------------------
     if (lane == 0) {
@@ -208,26 +225,15 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
     }
   } else if (warp == 1) {
     // ---- products ------------------------------------------------------------
-    if (lane == 0) {
-      const int k_steps = (w.c.dim + 15) / 16, n_out = k_steps * 16;
-      const uint32_t qk = mma_desc(BF16, kM, kN, false, false), pv = mma_desc(BF16, kM, n_out, false, true);
+    {
+      const Products<DB, 64> mm(BF16, w.c.dim);
       const uint32_t q_addr = smem_addr(q_tile), kv_addr = smem_addr(kv_tile);
       int stage = 0;
       uint32_t phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
       auto scores = [&](int s, int st, bool last_one) {
-        const uint32_t a = q_addr + s * Sh::tile, b = kv_addr + st * Sh::tile;
-        for (int x = 0; x < k_steps; ++x) {
-          const uint32_t off = (x >> 2) * kBox + (x & 3) * 32;
-          mma_ss(tmem + s * kN, desc_k_major(a + off), desc_k_major(b + off), qk, x > 0);
-        }
-        mma_commit(&bars.s_full[s]);
-        if (last_one) mma_commit(&bars.q_empty[s]);
-      };
-      auto values = [&](int s, int st, bool add) {
-        const uint32_t b = kv_addr + st * Sh::tile;
-#pragma unroll
-        for (int x = 0; x < kN / 16; ++x)
-          mma_ts(tmem + 256 + s * 128, tmem + s * kN + x * 8, desc_mn_major(b + x * 2048, kBox), pv, add || x > 0);
+        mm.scores(tmem + s * kN, q_addr + s * Sh::tile, kv_addr + st * Sh::tile);
+        mma_commit(mm.leader, &bars.s_full[s]);
+        if (last_one) mma_commit(mm.leader, &bars.q_empty[s]);
       };
       bool ok = true;
       auto need = [&](bool waited) { return ok = ok && waited; };
@@ -243,6 +249,9 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
             q_phase[s] ^= 1;
           }
         }
+        auto takes = [&](const Item &x, int s, const KeyTiles<kN> &k, int t) {
+          return p.paired || x.range[s].touches(k.first(t), k.end(t));
+        };
         auto next = [&] {
           if (++stage == Sh::stages) stage = 0, phase ^= 1;
         };
@@ -251,8 +260,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         fence_after();
 #pragma unroll
         for (int s = 0; s < 2; ++s)
-          if (it.range[s].touches(tiles.first(0), tiles.end(0))) scores(s, stage, it.last[s] == 0);
-        mma_commit(&bars.kv_empty[stage]);
+          if (takes(it, s, tiles, 0)) scores(s, stage, it.last[s] == 0);
+        mma_commit(mm.leader, &bars.kv_empty[stage]);
         next();
         for (int t = 0; t < tiles.n; ++t) {
           const int v_stage = stage;
@@ -262,22 +271,22 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
           const bool more = t + 1 < tiles.n;
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            if (it.range[s].touches(tiles.first(t), tiles.end(t))) {
+            if (takes(it, s, tiles, t)) {
               if (!need(bar_wait(&bars.p_full[s], p_phase[s], stop, p.error))) break;
               p_phase[s] ^= 1;
               fence_after();
-              values(s, v_stage, started[s]);
+              mm.sums(tmem + 256 + s * 128, tmem + s * kN, kv_addr + v_stage * Sh::tile, started[s]);
               started[s] = true;
-              if (t == it.last[s]) mma_commit(&bars.o_full[s]);
+              if (t == it.last[s]) mma_commit(mm.leader, &bars.o_full[s]);
             }
-            if (s == 1) mma_commit(&bars.kv_empty[v_stage]);
+            if (s == 1) mma_commit(mm.leader, &bars.kv_empty[v_stage]);
             if (more) {
               if (s == 0) {
                 if (!need(bar_wait(&bars.kv_full[k_stage], phase, stop, p.error))) break;
                 fence_after();
               }
-              if (it.range[s].touches(tiles.first(t + 1), tiles.end(t + 1))) scores(s, k_stage, it.last[s] == t + 1);
-              if (s == 1) mma_commit(&bars.kv_empty[k_stage]);
+              if (takes(it, s, tiles, t + 1)) scores(s, k_stage, it.last[s] == t + 1);
+              if (s == 1) mma_commit(mm.leader, &bars.kv_empty[k_stage]);
             }
           }
           if (!ok) break;
@@ -285,15 +294,24 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         }
       }
     }
-  } else if (warp >= 4) {
-    // ---- softmax, a query row for each thread ----------------------------------
-    const int s = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+  } else {
+    // ---- softmax: two threads for each query row, 64 of its columns each --------
+    const int s = (warp - 2) >> 3, half = (warp - 2) >> 2 & 1, row = (warp & 3) * 32 + lane;
+    const int pair_bar = 1 + s * 4 + (warp & 3);  // named barrier of the two warps of these rows
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-    const uint32_t t_s = tmem + s * kN + lanes, t_o = tmem + 256 + s * 128 + lanes;
+    const uint32_t t_s = tmem + s * kN + half * 64 + lanes, t_o = tmem + 256 + s * 128 + half * DB * 32 + lanes;
     const float c = w.c.scale * kLog2e;
     uint32_t s_phase = 0, o_phase = 0;
-    bool ok = true;
-    for (int64_t n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
+    // These warps meet at barriers of their own, so none leaves early: a wait that
+    // gave up makes the rest run through on whatever is there.
+    auto swap = [&](float x) {  // the other thread's x
+      bars.row[s][half][row] = x;
+      pair_sync(pair_bar);
+      const float y = bars.row[s][half ^ 1][row];
+      pair_sync(pair_bar);
+      return y;
+    };
+    for (int64_t n = blockIdx.x; n < p.items; n += gridDim.x) {
       const Item it = item_of(p, n);
       const KeyTiles<kN> tiles(it.both);
       const KeyRange range = s ? it.range[1] : it.range[0];
@@ -305,20 +323,19 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
       float m = -INFINITY, l = 0.f;
       bool started = false;
       for (int t = 0; t < tiles.n; ++t) {
-        const int j0 = tiles.first(t), j1 = tiles.end(t);
-        if (!range.touches(j0, j1)) continue;
-        if (!(ok = bar_wait(&bars.s_full[s], s_phase, stop, p.error))) break;
+        if (!p.paired && !range.touches(tiles.first(t), tiles.end(t))) continue;
+        const int j0 = tiles.first(t) + half * 64, j1 = tiles.end(t);
+        bar_wait(&bars.s_full[s], s_phase, stop, p.error);
         s_phase ^= 1;
         fence_after();
-        const bool masked = !(j0 >= all_low && j0 + kN <= all_end && j1 - j0 == kN);
-        uint32_t seen[4];
+        const bool masked = !(j0 >= all_low && j0 + 64 <= all_end && j1 - j0 >= 64);
+        uint32_t seen[2] = {~0u, ~0u};
         if (masked) {
           const int b0 = span.low - j0, b1 = min(span.p + 1, j1) - j0, s0 = span.start - j0,
                     s1 = min(span.sink_end, j1) - j0;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) seen[x] = bits(b0, b1, x * 32) | bits(s0, s1, x * 32);
+          seen[0] = bits(b0, b1, 0) | bits(s0, s1, 0), seen[1] = bits(b0, b1, 32) | bits(s0, s1, 32);
         }
-        uint32_t pk[kN / 2];
+        uint32_t pk[32];
         float2 sum[2];
         float tops[4];
         // Scores of 16 keys, loaded into `z` beforehand: their maximum and, with
@@ -351,9 +368,9 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
           tops[0] = tops[1] = tops[2] = tops[3] = -INFINITY;
           tmem_ld16(t_s, z[0]);
 #pragma unroll
-          for (int x = 0; x < 8; ++x) {
+          for (int x = 0; x < 4; ++x) {
             wait_ld();
-            if (x < 7) tmem_ld16(t_s + (x + 1) * 16, z[(x + 1) & 1]);
+            if (x < 3) tmem_ld16(t_s + (x + 1) * 16, z[(x + 1) & 1]);
             part(exp, z[x & 1], x, base2);
           }
           return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
@@ -361,26 +378,27 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         // Later tiles rarely raise the maximum in use: their exponentials are
         // taken at once and only taken again where it had to rise.
         float top = started ? tile(std::true_type{}) : tile(std::false_type{});
-        bool raise = (top - m) * c > 8.f;
-        if (!started || __any_sync(~0u, raise)) {
+        if (pair_any(pair_bar, !started || (top - m) * c > 8.f)) {
+          top = fmaxf(top, swap(top));
+          const bool raise = (top - m) * c > 8.f;
           const float keep = raise ? (m == -INFINITY ? 0.f : exp2_fast((m - top) * c)) : 1.f;
           l *= keep;
           if (raise) m = top;
           if (started) {
 #pragma unroll 1
-            for (int x = 0; x < DB * 64; x += 32) {
-              uint32_t o[32];
-              tmem_ld32(t_o + x, o);
+            for (int x = 0; x < DB * 32; x += 16) {
+              uint32_t o[16];
+              tmem_ld16(t_o + x, o);
               wait_ld();
-              tie32(o);
+              tie16(o);
 #pragma unroll
-              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * keep);
-              tmem_st32(t_o + x, o);
+              for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * keep);
+              tmem_st16(t_o + x, o);
             }
           }
           tile(std::true_type{});
         }
-        tmem_st32(t_s, pk), tmem_st32(t_s + 32, pk + 32);
+        tmem_st32(t_s, pk);
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         wait_st();
         fence_before();
@@ -388,38 +406,40 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         if (lane == 0) bar_arrive(&bars.p_full[s]);
         started = true;
       }
-      if (!ok) break;
       if (started) {
-        if (!(ok = bar_wait(&bars.o_full[s], o_phase, stop, p.error))) break;
+        bar_wait(&bars.o_full[s], o_phase, stop, p.error);
         o_phase ^= 1;
         fence_after();
       }
+      l += swap(l);
       const bool inside = i < w.c.q_len, empty = span.empty();
       const float inv = empty ? 0.f : 1.f / l;
+      const int d0 = half * DB * 32;  // this thread's share of the head
       T *out = static_cast<T *>(w.c.out) + ((it.b * w.c.q_len + i) * w.c.q_heads + h) * w.c.dim;
       bool bad = false;
 #pragma unroll 1
-      for (int x = 0; x < DB * 64; x += 32) {
-        uint32_t o[32];
+      for (int x = 0; x < DB * 32; x += 16) {
+        uint32_t o[16];
         if (started) {
-          tmem_ld32(t_o + x, o);
+          tmem_ld16(t_o + x, o);
           wait_ld();
-          tie32(o);
+          tie16(o);
         }
 #pragma unroll
-        for (int y = 0; y < 32; y += 8) {
+        for (int y = 0; y < 16; y += 8) {
           uint32_t v[4];
 #pragma unroll
           for (int z = 0; z < 4; ++z) {
             const float e0 = empty ? 0.f : __uint_as_float(o[y + 2 * z]) * inv;
             const float e1 = empty ? 0.f : __uint_as_float(o[y + 2 * z + 1]) * inv;
-            bad = bad || (x + y < w.c.dim && !(fabsf(e0) < INFINITY && fabsf(e1) < INFINITY));
+            bad = bad || (d0 + x + y < w.c.dim && !(fabsf(e0) < INFINITY && fabsf(e1) < INFINITY));
             v[z] = pack2<BF16>(e0, e1);
           }
-          if (inside && x + y < w.c.dim) *reinterpret_cast<uint4 *>(out + x + y) = make_uint4(v[0], v[1], v[2], v[3]);
+          if (inside && d0 + x + y < w.c.dim)
+            *reinterpret_cast<uint4 *>(out + d0 + x + y) = make_uint4(v[0], v[1], v[2], v[3]);
         }
       }
-      if (inside && w.c.lse)
+      if (inside && half == 0 && w.c.lse)
         w.c.lse[((int64_t)it.b * w.c.q_heads + h) * w.lse_row + i] = empty ? INFINITY : m * c + log2f(l);
       if (__any_sync(~0u, bad && inside)) {
         // What the row sees may be at fault; recompute it only if something not
@@ -428,7 +448,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         const T *v = static_cast<const T *>(w.c.v.ptr) + it.b * w.c.v.batch + it.hk * w.c.v.head;
         for (int t = 0; t < tiles.n; ++t) {
           const int j0 = tiles.first(t);
-          if (!range.touches(j0, tiles.end(t)) || (j0 >= all_low && j0 + kN <= all_end && tiles.end(t) - j0 == kN)) continue;
+          if (!range.touches(j0, tiles.end(t)) ||
+              (j0 >= all_low && j0 + kN <= all_end && tiles.end(t) - j0 == kN)) continue;
           for (int x = 0; x < kN; x += 32) {
             const unsigned flags = __ballot_sync(~0u, row_not_finite(v, w.c.v.token, j0 + x + lane, w.c.k_len, w.c.dim));
             for (unsigned left = flags; left; left &= left - 1) {
@@ -438,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
           }
         }
         for (unsigned left = __ballot_sync(~0u, bad && inside && hidden); left; left &= left - 1)
-          repair_row<T>(w, it.b, h, i - lane + __ffs(left) - 1);
+          repair_row<T>(w, it.b, h, i - lane + __ffs(left) - 1, d0, d0 + DB * 32);
       }
     }
   }
@@ -450,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
       for (int x = 0; x < (1 << 16) && !bar_try(&bars.kv_full[s], 0) && !bar_try(&bars.kv_full[s], 1); ++x) {
       }
   __syncthreads();
-  if (warp == 2) tmem_free(tmem, 512);
+  if (warp == 1) tmem_free(tmem, 512);
 }
 
 template <typename T, int DB> void launch(Params &p, cudaStream_t s) {

@@ -52,6 +52,36 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi, int from) {
   return hi <= lo ? 0u : (~0u >> (32 - hi)) & (~0u << lo);
 }
 
+// Products issued by a warp's leader, of tiles of 128 x 128 and head sizes covered by
+// DB boxes of 64 elements. Scores: both operands K-major in shared memory. Sums:
+// left operand in tensor memory, where each run of W columns of scores holds its
+// 16-bit values in its first W / 2 columns; right operand MN-major in shared
+// memory. Unrolled: the issuing warp is on the critical path of every tile.
+template <int DB, int W> struct Products {
+  bool leader;
+  int k_steps;
+  uint32_t scores_desc, sums_desc;
+  __device__ Products(bool bf16, int dim) : leader((threadIdx.x & 31) == 0), k_steps((dim + 15) / 16) {
+    scores_desc = tc::mma_desc(bf16, 128, 128, false, false);
+    sums_desc = tc::mma_desc(bf16, 128, k_steps * 16, false, true);
+  }
+  __device__ __forceinline__ void scores(uint32_t d, uint32_t a, uint32_t b) const {
+    const uint32_t x = tc::desc_k_major(a), y = tc::desc_k_major(b);
+#pragma unroll
+    for (int k = 0; k < DB * 4; ++k)
+      if (k < k_steps) {
+        const uint32_t off = ((k >> 2) * kBox + (k & 3) * 32) >> 4;
+        tc::mma_ss(leader, d, x + off, y + off, scores_desc, k > 0);
+      }
+  }
+  __device__ __forceinline__ void sums(uint32_t d, uint32_t left, uint32_t b, bool add) const {
+    const uint32_t y = tc::desc_mn_major(b, kBox);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      tc::mma_ts(leader, d, left + k * 16 / W * W + k * 16 % W / 2, y + (k * 2048 >> 4), sums_desc, add || k > 0);
+  }
+};
+
 // Whether row t of a 16-bit matrix (dim elements from `p`, a multiple of 8,
 // 16-byte aligned) holds an infinity or a NaN; rows outside [0, limit) do not.
 template <typename T> __device__ inline bool row_not_finite(const T *p, int64_t token_stride, int64_t t, int64_t limit, int dim) {
