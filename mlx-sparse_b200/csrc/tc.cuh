@@ -33,7 +33,7 @@ __device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
 // A wait that gives up after `kWaitNs`, far beyond any run of these kernels: it
 // then sets the device's error flag and the CTA's `stop`, which makes every
 // other wait of the CTA give up too, so that all warps reach the kernel's end.
-constexpr unsigned long long kWaitNs = 20ull * 1000 * 1000 * 1000;
+constexpr unsigned long long kWaitNs = 4ull * 1000 * 1000 * 1000;
 __device__ __forceinline__ unsigned long long now_ns() {
   unsigned long long t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
@@ -56,6 +56,11 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatil
   for (int i = 0; i < 64; ++i)
     if (bar_try(bar, parity)) return true;
   return bar_wait_slow(bar, parity, stop, error);
+}
+
+// The same by a whole warp, which goes on or gives up as one.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *stop, int *error) {
+  return __all_sync(~0u, bar_wait(bar, parity, stop, error));
 }
 
 // ---- TMA -----------------------------------------------------------------------
@@ -124,6 +129,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t *r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
   asm volatile(

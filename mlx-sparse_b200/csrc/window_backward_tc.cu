@@ -48,15 +48,6 @@ struct Params {
   int *error;
 };
 
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n"
-      " mov.b64 {%0, %1}, x;\n}\n"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-
 // The score of one pair times log2(e) and dO_i . V_j, from global memory.
 template <typename T> struct PairDots {
   const T *q, *k, *g, *v;
@@ -134,24 +125,6 @@ __device__ __noinline__ void repair_dkv(const WindowProblem &w, int b, int hk, i
 #pragma unroll
   for (int y = 0; y < 4; ++y)
     if (y * 32 + lane < w.c.dim) out[y * 32 + lane] = VT<T>::store(acc[y] * (keys ? w.c.scale : 1.f));
-}
-
-// Writes 32 accumulator columns of a row, scaled; true if one is not finite.
-template <typename T> __device__ __forceinline__ bool store32(T *row, uint32_t *o, float scale, int d0, int dim, bool inside) {
-  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  bool bad = false;
-#pragma unroll
-  for (int y = 0; y < 32; y += 8) {
-    uint32_t v[4];
-#pragma unroll
-    for (int z = 0; z < 4; ++z) {
-      const float a = __uint_as_float(o[y + 2 * z]) * scale, c = __uint_as_float(o[y + 2 * z + 1]) * scale;
-      bad = bad || (d0 + y < dim && !(fabsf(a) < INFINITY && fabsf(c) < INFINITY));
-      v[z] = pack2<BF16>(a, c);
-    }
-    if (inside && d0 + y < dim) *reinterpret_cast<uint4 *>(row + d0 + y) = make_uint4(v[0], v[1], v[2], v[3]);
-  }
-  return bad;
 }
 
 __device__ __forceinline__ void drain(uint64_t *bars, int n) {
@@ -238,10 +211,10 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
     }
   } else if (warp == 1) {
     if (n > 0) {
-      const Products<DB, 64> mm(BF16, w.c.dim);
+      const Products<DB> mm(BF16, w.c.dim);
       const uint32_t ka = smem_addr(k_tile), va = smem_addr(v_tile), ra = smem_addr(ring);
-      bool ok = bar_wait(&bars.kv_full, 0, stop, p.error);
-      auto ready = [&](int e) { return ok = ok && bar_wait(&bars.full[e % kStages], e / kStages & 1, stop, p.error); };
+      bool ok = warp_wait(&bars.kv_full, 0, stop, p.error);
+      auto ready = [&](int e) { return ok = ok && warp_wait(&bars.full[e % kStages], e / kStages & 1, stop, p.error); };
       auto tile = [&](int e) { return ra + (e % kStages) * kTile; };
       if (ready(0)) {
         fence_after();
@@ -254,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       }
       for (int it = 0; ok && it < n; ++it) {
         const int q = 2 * it, g = q + 1;
-        if (!(ok = bar_wait(&bars.p_full, it & 1, stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.p_full, it & 1, stop, p.error))) break;
         fence_after();
         mm.sums(t_dv, t_s, tile(g), it > 0);
         mma_commit(mm.leader, &bars.empty[g % kStages]);
@@ -263,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
           mm.scores(t_s, ka, tile(q + 2));
           mma_commit(mm.leader, &bars.s_full);
         }
-        if (!(ok = bar_wait(&bars.ds_full, it & 1, stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.ds_full, it & 1, stop, p.error))) break;
         fence_after();
         mm.sums(t_dk, t_dp, tile(q), it > 0);
         mma_commit(mm.leader, &bars.empty[q % kStages]);
@@ -290,8 +263,8 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       const int c0 = key - shift - i0, c1 = min(own_last - shift, (int)w.c.q_len - 1) - i0 + 1;
       const uint32_t seen[2] = {bits(c0, c1, 0), bits(c0, c1, 32)};
       // lse and delta came with Q's tile, which the products of s_full have read
-      if (!(ok = bar_wait(&bars.full[2 * it % kStages], 2 * it / kStages & 1, stop, p.error))) break;
-      if (!(ok = bar_wait(&bars.s_full, it & 1, stop, p.error))) break;
+      if (!(ok = warp_wait(&bars.full[2 * it % kStages], 2 * it / kStages & 1, stop, p.error))) break;
+      if (!(ok = warp_wait(&bars.s_full, it & 1, stop, p.error))) break;
       fence_after();
       float2 pr[32];
       {
@@ -323,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive(&bars.p_full);
-      if (!(ok = bar_wait(&bars.dp_full, it & 1, stop, p.error))) break;
+      if (!(ok = warp_wait(&bars.dp_full, it & 1, stop, p.error))) break;
       fence_after();
       {
         uint32_t z[2][16], pk[16];
@@ -355,12 +328,12 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       __syncwarp();
       if (lane == 0) bar_arrive(&bars.ds_full);
     }
-    if (ok && n > 0) ok = bar_wait(&bars.done, 0, stop, p.error);
+    if (ok && n > 0) ok = warp_wait(&bars.done, 0, stop, p.error);
     if (ok) {
       fence_after();
       // the first warpgroup writes dV, the second dK
       const bool inside = key < w.c.k_len;
-      T *out = static_cast<T *>(half ? w.c.dk : w.c.dv) + ((b * w.c.k_len + key) * w.c.k_heads + hk) * w.c.dim;
+      T *out = static_cast<T *>(half ? w.c.dk : w.c.dv) + ((b * w.c.k_len + key - lane) * w.c.k_heads + hk) * w.c.dim;
       const uint32_t from = (half ? t_dk : t_dv) + ((uint32_t)(warp & 3) << 21);
       bool bad = false;
 #pragma unroll 1
@@ -374,7 +347,8 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
 #pragma unroll
           for (int y = 0; y < 32; ++y) o[y] = 0;
         }
-        bad = store32<T>(out, o, half ? -w.c.scale : 1.f, x, w.c.dim, inside) || bad;
+        bad = store32<T>(out, (int64_t)w.c.k_heads * w.c.dim, o, half ? -w.c.scale : 1.f, x, w.c.dim,
+                         (int)w.c.k_len - (key - lane)) || bad;
       }
       if (__any_sync(~0u, bad && inside)) {
         bool hidden = false;
@@ -474,13 +448,13 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
     }
   } else if (warp == 1) {
     {
-      const Products<DB, 64> mm(BF16, w.c.dim);
+      const Products<DB> mm(BF16, w.c.dim);
       const uint32_t qa = smem_addr(q_tile), ga = smem_addr(g_tile), ra = smem_addr(ring);
       int64_t done = 0;  // tile pairs of earlier items: K of pair t is ring entry 2 (done + t), V the next
       uint32_t q_phase = 0;
       bool ok = true;
       auto ready = [&](int64_t e) {
-        return ok = ok && bar_wait(&bars.full[e % kStages], (uint32_t)(e / kStages & 1), stop, p.error);
+        return ok = ok && warp_wait(&bars.full[e % kStages], (uint32_t)(e / kStages & 1), stop, p.error);
       };
       auto tile = [&](int64_t e) { return ra + (uint32_t)(e % kStages) * kTile; };
       auto s_at = [&](int64_t t) { return tmem + (uint32_t)(t & 1) * 128; };
@@ -489,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
         item(x, b, h, i0);
         const KeyTiles<kT> tiles(key_range(w, b, i0, i0 + kT - 1));
         if (tiles.n == 0) continue;
-        if (!(ok = bar_wait(&bars.q_full, q_phase, stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.q_full, q_phase, stop, p.error))) break;
         q_phase ^= 1;
         auto scores = [&](int64_t t) {
           if (!ready(2 * t)) return;
@@ -510,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
         for (int t = 0; ok && t < tiles.n; ++t) {
           const int64_t e = done + t;
           if (t + 1 < tiles.n) scores(e + 1);
-          if (!(ok = ok && bar_wait(&bars.ds_full, (uint32_t)(e & 1), stop, p.error))) break;
+          if (!(ok = ok && warp_wait(&bars.ds_full, (uint32_t)(e & 1), stop, p.error))) break;
           fence_after();
           mm.sums(t_dq, t_dp, tile(2 * e), t > 0);
           mma_commit(mm.leader, &bars.empty[2 * e % kStages]);
@@ -550,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
                     s1 = min(span.sink_end, j1) - j0;
           seen[0] = bits(b0, b1, 0) | bits(s0, s1, 0), seen[1] = bits(b0, b1, 32) | bits(s0, s1, 32);
         }
-        if (!(ok = bar_wait(&bars.s_full[e & 1], (uint32_t)(e >> 1 & 1), stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.s_full[e & 1], (uint32_t)(e >> 1 & 1), stop, p.error))) break;
         fence_after();
         const uint32_t t_s = tmem + (uint32_t)(e & 1) * 128 + lanes + half * 64, t_d = t_dp + lanes + half * 64;
         float2 pr[32];
@@ -576,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
             }
           }
         }
-        if (!(ok = bar_wait(&bars.dp_full, (uint32_t)(e & 1), stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.dp_full, (uint32_t)(e & 1), stop, p.error))) break;
         fence_after();
         {
           uint32_t z[2][16], pk[16];
@@ -610,11 +584,11 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
       if (!ok) break;
       done += tiles.n;
       if (tiles.n > 0) {
-        if (!(ok = bar_wait(&bars.dq_full, dq_phase, stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.dq_full, dq_phase, stop, p.error))) break;
         dq_phase ^= 1;
         fence_after();
       }
-      T *dq = static_cast<T *>(w.c.dq) + ((b * w.c.q_len + i) * w.c.q_heads + h) * w.c.dim;
+      T *dq = static_cast<T *>(w.c.dq) + ((b * w.c.q_len + i - lane) * w.c.q_heads + h) * w.c.dim;
       const int d0 = half * DB * 32;
       bool bad = false;
 #pragma unroll 1
@@ -628,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
 #pragma unroll
           for (int y = 0; y < 32; ++y) o[y] = 0;
         }
-        bad = store32<T>(dq, o, -w.c.scale, d, w.c.dim, inside) || bad;
+        bad = store32<T>(dq, (int64_t)w.c.q_heads * w.c.dim, o, -w.c.scale, d, w.c.dim, (int)w.c.q_len - (i - lane)) || bad;
       }
       if (__any_sync(~0u, bad && inside)) {
         bool hidden = false;

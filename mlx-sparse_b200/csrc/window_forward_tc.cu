@@ -5,13 +5,14 @@
 // heads that share a key head, or two neighbouring query tiles of one head where
 // the group is odd. It walks the tiles of 128 keys that they see, the sink
 // tiles and then the band's, and no others. One warp loads Q, K and V tiles by
-// TMA into a ring of shared memory; one thread issues tcgen05.mma; a warpgroup
+// TMA into a ring of shared memory; one warp issues tcgen05.mma; a warpgroup
 // for each slot does its softmax, a query row for each thread, straight from
-// tensor memory. Scores and output of a slot stay in tensor memory (S 128
-// columns, O 128 columns, two slots: all 512); the probabilities, rounded to the
-// inputs' type for the second product (half a step each, against sums held in
-// fp32), take the place of the scores and are read from there as its left
-// operand. While one slot's softmax runs, the other slot's two products do.
+// tensor memory. Scores and output of a slot stay there (S 128 columns, O 128, two
+// slots: all 512). The probabilities, rounded to the inputs' type for the second
+// product (half a step each, against sums held in fp32), take the place of the
+// scores and are read from there as its left operand, the first 64 of a tile
+// while the softmax of the last 64 goes on. While one slot's softmax runs, the
+// other slot's products do.
 //
 // The running maximum is only raised when a row's new maximum is 2^8 above the
 // one in use, so the output is rescaled in tensor memory a few times at most;
@@ -19,11 +20,12 @@
 //
 // A masked score is -inf before the softmax, whatever it was. Its probability
 // is 0, but 0 times an infinite or NaN value row would still reach the second
-// product: rows that end not finite are computed again pair by pair.
+// product: rows that end not finite are computed again pair by pair where
+// something not finite hides among their tiles' other keys.
 //
-// Bound: the exponentials (16 a clock and SM: 1024 clocks for 128 x 128 scores)
-// and the products (2 x 512 clocks at head size 128) take the same time, side
-// by side.
+// Bound: the products (2 x 520 clocks for 128 x 128 scores at head size 128) and
+// the exponentials (16 a clock and SM: 1024 clocks, less a share that is computed
+// as polynomials on the FMA units) take about the same time, side by side.
 #include <algorithm>
 
 #include "window_tc.cuh"
@@ -38,15 +40,13 @@ __device__ int g_window_error;
 
 constexpr int kM = 128;  // queries of a slot: the lanes of tensor memory
 constexpr int kN = 128;  // keys of a tile
-constexpr int kSoftmaxWarps = 16;
-constexpr int kThreads = 64 + kSoftmaxWarps * 32;  // loads, products, softmax
+constexpr int kThreads = 64 + 2 * 128;  // loads, products, two softmax warpgroups
 
 struct Bars {
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
-  uint64_t kv_full[8], kv_empty[8];
+  uint64_t kv_full[8], step[8];
   uint32_t tmem;
   int stop;
-  float row[2][2][kM];  // what the two threads of a row tell each other
 };
 
 template <int DB> struct Shape {  // DB boxes of 64 elements cover the head size
@@ -106,21 +106,9 @@ __device__ __forceinline__ Item item_of(const Params &p, int64_t n) {
   return it;
 }
 
-// Named barriers of two warps.
-__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ bool pair_any(int id, bool x) {
-  uint32_t r;
-  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %2, 0;\n bar.red.or.pred q, %1, 64, p;\n selp.u32 %0, 1, 0, q;\n}\n"
-               : "=r"(r)
-               : "r"(id), "r"((uint32_t)x)
-               : "memory");
-  return r != 0;
-}
-
 // One row again, by a warp, pair by pair: only what the query sees is touched.
-// Columns [d0, d1) are written.
 template <typename T>
-__device__ __noinline__ void repair_row(const WindowProblem &w, int b, int h, int i, int d0, int d1) {
+__device__ __noinline__ void repair_row(const WindowProblem &w, int b, int h, int i) {
   const int lane = threadIdx.x & 31, dim = w.c.dim, hk = h / w.group;
   const T *q = static_cast<const T *>(w.c.q.ptr) + b * w.c.q.batch + h * w.c.q.head + i * w.c.q.token;
   const T *k = static_cast<const T *>(w.c.k.ptr) + b * w.c.k.batch + hk * w.c.k.head;
@@ -160,7 +148,7 @@ __device__ __noinline__ void repair_row(const WindowProblem &w, int b, int h, in
   T *out = static_cast<T *>(w.c.out) + ((b * w.c.q_len + i) * w.c.q_heads + h) * dim;
 #pragma unroll
   for (int x = 0; x < 4; ++x)
-    if (x * 32 + lane >= d0 && x * 32 + lane < min(d1, dim)) out[x * 32 + lane] = VT<T>::store(acc[x] / l);
+    if (x * 32 + lane < dim) out[x * 32 + lane] = VT<T>::store(acc[x] / l);
   if (w.c.lse && lane == 0) w.c.lse[((int64_t)b * w.c.q_heads + h) * w.lse_row + i] = m + log2f(l);
 }
 
@@ -181,9 +169,10 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       bar_init(&bars.q_full[s], 1), bar_init(&bars.q_empty[s], 1);
-      bar_init(&bars.s_full[s], 1), bar_init(&bars.p_full[s], 8), bar_init(&bars.o_full[s], 1);
+      bar_init(&bars.s_full[s], 1), bar_init(&bars.p_full[s], 4), bar_init(&bars.o_full[s], 1);
     }
-    for (int s = 0; s < Sh::stages; ++s) bar_init(&bars.kv_full[s], 1), bar_init(&bars.kv_empty[s], 1);
+    for (int s = 0; s < Sh::stages; ++s) bar_init(&bars.kv_full[s], 1);
+    for (int s = 0; s < 8; ++s) bar_init(&bars.step[s], 1);
     bars.stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -195,8 +184,16 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
   if (warp == 0) {
     // ---- loads -------------------------------------------------------------
     if (lane == 0) {
+      uint32_t q_phase[2] = {1, 1};  // an empty barrier's first wait passes
+      // Step g of all tiles so far frees V of tile g, K of tile g + 1 and, where that
+      // is an item's first, K of tile g: an item's entries of the ring, K and V in
+      // turn, are free after the steps t - 1 (0 for the first) and t. `freed`: the
+      // step that frees each stage's entry. It has barrier freed % 8, more than the
+      // steps that the ring lets the products run ahead.
+      int64_t base = 0, freed[Sh::stages];
+#pragma unroll
+      for (int x = 0; x < Sh::stages; ++x) freed[x] = -1;
       int stage = 0;
-      uint32_t phase = 1, q_phase[2] = {1, 1};  // an empty barrier's first wait passes
       bool ok = true;
       for (int64_t n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
         const Item it = item_of(p, n);
@@ -213,180 +210,157 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         }
         for (int t = 0; ok && t < tiles.n; ++t) {
           for (int kv = 0; kv < 2; ++kv) {
-            if (!(ok = bar_wait(&bars.kv_empty[stage], phase, stop, p.error))) break;
+            const int64_t g = freed[stage];
+            if (g >= 0 && !(ok = bar_wait(&bars.step[g & 7], (uint32_t)(g >> 3 & 1), stop, p.error))) break;
+            freed[stage] = base + (kv || t == 0 ? t : t - 1);
             bar_expect(&bars.kv_full[stage], Sh::tile);
             for (int x = 0; x < DB; ++x)
               tma_load_4d(kv_tile + stage * Sh::tile + x * kBox, kv ? &p.v : &p.k, &bars.kv_full[stage], x * 64,
                           tiles.first(t), it.hk, it.b);
-            if (++stage == Sh::stages) stage = 0, phase ^= 1;
+            if (++stage == Sh::stages) stage = 0;
           }
         }
+        base += tiles.n;
       }
     }
   } else if (warp == 1) {
     // ---- products ------------------------------------------------------------
-    {
-      const Products<DB, 64> mm(BF16, w.c.dim);
-      const uint32_t q_addr = smem_addr(q_tile), kv_addr = smem_addr(kv_tile);
-      int stage = 0;
-      uint32_t phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+    const Products<DB> mm(BF16, w.c.dim);
+    const uint32_t q_addr = smem_addr(q_tile), kv_addr = smem_addr(kv_tile);
+    int stage = 0;
+    uint32_t phase = 0, steps = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+    bool ok = true;
+    auto need = [&](bool waited) { return ok = ok && waited; };
+    auto next = [&] {
+      if (++stage == Sh::stages) stage = 0, phase ^= 1;
+    };
+    for (int64_t n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
+      const Item it = item_of(p, n);
+      const KeyTiles<kN> tiles(it.both);
+      if (tiles.n == 0) continue;
+      auto takes = [&](int s, int t) { return p.paired || it.range[s].touches(tiles.first(t), tiles.end(t)); };
       auto scores = [&](int s, int st, bool last_one) {
         mm.scores(tmem + s * kN, q_addr + s * Sh::tile, kv_addr + st * Sh::tile);
         mma_commit(mm.leader, &bars.s_full[s]);
         if (last_one) mma_commit(mm.leader, &bars.q_empty[s]);
       };
-      bool ok = true;
-      auto need = [&](bool waited) { return ok = ok && waited; };
-      for (int64_t n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
-        const Item it = item_of(p, n);
-        const KeyTiles<kN> tiles(it.both);
-        if (tiles.n == 0) continue;
-        bool started[2] = {false, false};
+      bool started[2] = {false, false};
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (it.last[s] >= 0) {
+          need(warp_wait(&bars.q_full[s], q_phase[s], stop, p.error));
+          q_phase[s] ^= 1;
+        }
+      // the stage of K_0 is now, V_t and K_{t+1} follow in turn
+      if (!need(warp_wait(&bars.kv_full[stage], phase, stop, p.error))) break;
+      fence_after();
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (takes(s, 0)) scores(s, stage, it.last[s] == 0);
+      next();
+      for (int t = 0; ok && t < tiles.n; ++t) {
+        const int v_stage = stage;
+        if (!need(warp_wait(&bars.kv_full[stage], phase, stop, p.error))) break;
+        next();
+        const int k_stage = stage;
+        const bool more = t + 1 < tiles.n;
+        const bool now[2] = {takes(0, t), takes(1, t)}, then[2] = {more && takes(0, t + 1), more && takes(1, t + 1)};
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          if (it.last[s] >= 0) {
-            if (!need(bar_wait(&bars.q_full[s], q_phase[s], stop, p.error))) break;
-            q_phase[s] ^= 1;
+          if (now[s]) {
+            need(warp_wait(&bars.p_full[s], p_phase[s], stop, p.error));
+            fence_after();
+            mm.sums(tmem + 256 + s * 128, tmem + s * kN, kv_addr + v_stage * Sh::tile, started[s]);
+            if (t == it.last[s]) mma_commit(mm.leader, &bars.o_full[s]);
+            p_phase[s] ^= 1;
+            started[s] = true;
           }
-        }
-        auto takes = [&](const Item &x, int s, const KeyTiles<kN> &k, int t) {
-          return p.paired || x.range[s].touches(k.first(t), k.end(t));
-        };
-        auto next = [&] {
-          if (++stage == Sh::stages) stage = 0, phase ^= 1;
-        };
-        // the stage of K_0 is now, V_t and K_{t+1} follow in turn
-        if (!need(bar_wait(&bars.kv_full[stage], phase, stop, p.error))) break;
-        fence_after();
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-          if (takes(it, s, tiles, 0)) scores(s, stage, it.last[s] == 0);
-        mma_commit(mm.leader, &bars.kv_empty[stage]);
-        next();
-        for (int t = 0; t < tiles.n; ++t) {
-          const int v_stage = stage;
-          if (!need(bar_wait(&bars.kv_full[stage], phase, stop, p.error))) break;
-          next();
-          const int k_stage = stage;
-          const bool more = t + 1 < tiles.n;
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            if (takes(it, s, tiles, t)) {
-              if (!need(bar_wait(&bars.p_full[s], p_phase[s], stop, p.error))) break;
-              p_phase[s] ^= 1;
-              fence_after();
-              mm.sums(tmem + 256 + s * 128, tmem + s * kN, kv_addr + v_stage * Sh::tile, started[s]);
-              started[s] = true;
-              if (t == it.last[s]) mma_commit(mm.leader, &bars.o_full[s]);
-            }
-            if (s == 1) mma_commit(mm.leader, &bars.kv_empty[v_stage]);
-            if (more) {
-              if (s == 0) {
-                if (!need(bar_wait(&bars.kv_full[k_stage], phase, stop, p.error))) break;
-                fence_after();
-              }
-              if (takes(it, s, tiles, t + 1)) scores(s, k_stage, it.last[s] == t + 1);
-              if (s == 1) mma_commit(mm.leader, &bars.kv_empty[k_stage]);
-            }
+          if (s == 0 && more) {
+            need(warp_wait(&bars.kv_full[k_stage], phase, stop, p.error));
+            fence_after();
           }
-          if (!ok) break;
-          if (more) next();
+          if (then[s]) scores(s, k_stage, it.last[s] == t + 1);
         }
+        mma_commit(mm.leader, &bars.step[steps++ & 7]);
+        if (more) next();
       }
     }
   } else {
-    // ---- softmax: two threads for each query row, 64 of its columns each --------
-    const int s = (warp - 2) >> 3, half = (warp - 2) >> 2 & 1, row = (warp & 3) * 32 + lane;
-    const int pair_bar = 1 + s * 4 + (warp & 3);  // named barrier of the two warps of these rows
+    // ---- softmax, a query row for each thread ------------------------------------
+    const int s = (warp - 2) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-    const uint32_t t_s = tmem + s * kN + half * 64 + lanes, t_o = tmem + 256 + s * 128 + half * DB * 32 + lanes;
+    const uint32_t t_s = tmem + s * kN + lanes, t_o = tmem + 256 + s * 128 + lanes;
     const float c = w.c.scale * kLog2e;
     uint32_t s_phase = 0, o_phase = 0;
-    // These warps meet at barriers of their own, so none leaves early: a wait that
-    // gave up makes the rest run through on whatever is there.
-    auto swap = [&](float x) {  // the other thread's x
-      bars.row[s][half][row] = x;
-      pair_sync(pair_bar);
-      const float y = bars.row[s][half ^ 1][row];
-      pair_sync(pair_bar);
-      return y;
-    };
-    for (int64_t n = blockIdx.x; n < p.items; n += gridDim.x) {
+    bool ok = true;
+    for (int64_t n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
       const Item it = item_of(p, n);
       const KeyTiles<kN> tiles(it.both);
       const KeyRange range = s ? it.range[1] : it.range[0];
       const int i = (s ? it.i0[1] : it.i0[0]) + row, h = s ? it.head[1] : it.head[0];
       const QuerySpan span = query_span(w, it.b, i);
-      // the keys that all 32 rows of this warp see: tiles inside need no mask
+      // the keys that all 32 rows of this warp see: halves inside need no mask
       const int all_low = __reduce_max_sync(~0u, span.p < 0 ? INT_MAX : span.low);
       const int all_end = __reduce_min_sync(~0u, span.p < 0 ? -1 : span.p) + 1;
       float m = -INFINITY, l = 0.f;
       bool started = false;
-      for (int t = 0; t < tiles.n; ++t) {
+      for (int t = 0; ok && t < tiles.n; ++t) {
         if (!p.paired && !range.touches(tiles.first(t), tiles.end(t))) continue;
-        const int j0 = tiles.first(t) + half * 64, j1 = tiles.end(t);
-        bar_wait(&bars.s_full[s], s_phase, stop, p.error);
-        s_phase ^= 1;
+        if (!(ok = warp_wait(&bars.s_full[s], s_phase, stop, p.error))) break;
         fence_after();
-        const bool masked = !(j0 >= all_low && j0 + 64 <= all_end && j1 - j0 >= 64);
-        uint32_t seen[2] = {~0u, ~0u};
-        if (masked) {
+        const int j0 = tiles.first(t), j1 = tiles.end(t);
+        const bool masked = !(j0 >= all_low && j0 + kN <= all_end && j1 - j0 >= kN);
+        uint32_t pk[kN / 2];
+        // Scores of the tile: their maximum and, with EXP, their exponentials over the
+        // maximum in use, packed, and their sum.
+        auto tile = [&](auto exp, auto mask) {
+          const float base = m == -INFINITY ? 0.f : m * c;
+          const float2 base2 = make_float2(-base, -base), c2 = make_float2(c, c);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           const int b0 = span.low - j0, b1 = min(span.p + 1, j1) - j0, s0 = span.start - j0,
                     s1 = min(span.sink_end, j1) - j0;
-          seen[0] = bits(b0, b1, 0) | bits(s0, s1, 0), seen[1] = bits(b0, b1, 32) | bits(s0, s1, 32);
-        }
-        uint32_t pk[32];
-        float2 sum[2];
-        float tops[4];
-        // Scores of 16 keys, loaded into `z` beforehand: their maximum and, with
-        // EXP, their exponentials over the maximum in use, packed.
-        auto part = [&](auto exp, uint32_t *z, int x, float2 base2) {
-          tie16(z);
-          if (masked) {
 #pragma unroll
-            for (int y = 0; y < 16; ++y)
-              if (!(seen[x >> 1] >> ((x & 1) * 16 + y) & 1)) z[y] = 0xff800000u;  // -inf
-          }
+          for (int x = 0; x < kN; x += 32) {
+            uint32_t z[32];
+            tmem_ld16(t_s + x, z), tmem_ld16(t_s + x + 16, z + 16);
+            wait_ld();
+            tie32(z);
+            if (mask) {
+              const uint32_t seen = bits(b0, b1, x) | bits(s0, s1, x);
 #pragma unroll
-          for (int y = 0; y < 16; ++y) tops[y & 3] = fmaxf(tops[y & 3], __uint_as_float(z[y]));
-          if (decltype(exp)::value) {
+              for (int y = 0; y < 32; ++y)
+                if (!(seen >> y & 1)) z[y] = 0xff800000u;  // -inf
+            }
 #pragma unroll
-            for (int y = 0; y < 8; ++y) {
-              float2 e = fma2(make_float2(__uint_as_float(z[2 * y]), __uint_as_float(z[2 * y + 1])), make_float2(c, c),
-                              base2);
-              e.x = exp2_fast(e.x), e.y = exp2_fast(e.y);
-              sum[y & 1] = add2(sum[y & 1], e);
-              pk[x * 8 + y] = pack2<BF16>(e.x, e.y);
+            for (int y = 0; y < 32; y += 2)
+              tops[y >> 1 & 3] = max3(tops[y >> 1 & 3], __uint_as_float(z[y]), __uint_as_float(z[y + 1]));
+            if (exp) {
+#pragma unroll
+              for (int y = 0; y < 16; ++y) {
+                float2 e = fma2(make_float2(__uint_as_float(z[2 * y]), __uint_as_float(z[2 * y + 1])), c2, base2);
+                e.x = exp2_fast(e.x), e.y = exp2_fast(e.y);
+                sum[y & 1] = add2(sum[y & 1], e);
+                pk[x / 2 + y] = pack2<BF16>(e.x, e.y);
+              }
             }
           }
+          return make_float2(fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]),
+                             (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
         };
-        auto tile = [&](auto exp) {
-          uint32_t z[2][16];
-          const float base = m == -INFINITY ? 0.f : m * c;
-          const float2 base2 = make_float2(-base, -base);
-          sum[0] = sum[1] = make_float2(0.f, 0.f);
-          tops[0] = tops[1] = tops[2] = tops[3] = -INFINITY;
-          tmem_ld16(t_s, z[0]);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            wait_ld();
-            if (x < 3) tmem_ld16(t_s + (x + 1) * 16, z[(x + 1) & 1]);
-            part(exp, z[x & 1], x, base2);
-          }
-          return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        };
-        // Later tiles rarely raise the maximum in use: their exponentials are
-        // taken at once and only taken again where it had to rise.
-        float top = started ? tile(std::true_type{}) : tile(std::false_type{});
-        if (pair_any(pair_bar, !started || (top - m) * c > 8.f)) {
-          top = fmaxf(top, swap(top));
-          const bool raise = (top - m) * c > 8.f;
-          const float keep = raise ? (m == -INFINITY ? 0.f : exp2_fast((m - top) * c)) : 1.f;
+        constexpr std::true_type yes{};
+        constexpr std::false_type no{};
+        // Later tiles rarely raise the maximum in use: their exponentials are taken
+        // at once and only taken again where it had to rise.
+        float2 r = !started ? tile(no, yes) : masked ? tile(yes, yes) : tile(yes, no);
+        const bool raise = (r.x - m) * c > 8.f;
+        if (!started || __any_sync(~0u, raise)) {
+          const float keep = raise ? (m == -INFINITY ? 0.f : exp2_fast((m - r.x) * c)) : 1.f;
           l *= keep;
-          if (raise) m = top;
-          if (started) {
+          if (raise) m = r.x;
+          if (started) {  // the tiles before are in the output: these scores were computed after them
 #pragma unroll 1
-            for (int x = 0; x < DB * 32; x += 16) {
+            for (int x = 0; x < DB * 64; x += 16) {
               uint32_t o[16];
               tmem_ld16(t_o + x, o);
               wait_ld();
@@ -396,50 +370,42 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
               tmem_st16(t_o + x, o);
             }
           }
-          tile(std::true_type{});
+          r = tile(yes, yes);
         }
-        tmem_st32(t_s, pk);
-        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        tmem_st32(t_s, pk), tmem_st32(t_s + kHalf, pk + 32);
+        l += r.y;
         wait_st();
         fence_before();
         __syncwarp();
         if (lane == 0) bar_arrive(&bars.p_full[s]);
         started = true;
+        s_phase ^= 1;
       }
+      if (!ok) break;
       if (started) {
-        bar_wait(&bars.o_full[s], o_phase, stop, p.error);
+        if (!(ok = warp_wait(&bars.o_full[s], o_phase, stop, p.error))) break;
         o_phase ^= 1;
         fence_after();
       }
-      l += swap(l);
       const bool inside = i < w.c.q_len, empty = span.empty();
       const float inv = empty ? 0.f : 1.f / l;
-      const int d0 = half * DB * 32;  // this thread's share of the head
-      T *out = static_cast<T *>(w.c.out) + ((it.b * w.c.q_len + i) * w.c.q_heads + h) * w.c.dim;
+      T *out = static_cast<T *>(w.c.out) + ((it.b * w.c.q_len + i - lane) * w.c.q_heads + h) * w.c.dim;
       bool bad = false;
 #pragma unroll 1
-      for (int x = 0; x < DB * 32; x += 16) {
-        uint32_t o[16];
+      for (int x = 0; x < DB * 64; x += 32) {
+        uint32_t o[32];
         if (started) {
-          tmem_ld16(t_o + x, o);
+          tmem_ld16(t_o + x, o), tmem_ld16(t_o + x + 16, o + 16);
           wait_ld();
-          tie16(o);
+          tie32(o);
         }
+        if (!started || empty) {
 #pragma unroll
-        for (int y = 0; y < 16; y += 8) {
-          uint32_t v[4];
-#pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            const float e0 = empty ? 0.f : __uint_as_float(o[y + 2 * z]) * inv;
-            const float e1 = empty ? 0.f : __uint_as_float(o[y + 2 * z + 1]) * inv;
-            bad = bad || (d0 + x + y < w.c.dim && !(fabsf(e0) < INFINITY && fabsf(e1) < INFINITY));
-            v[z] = pack2<BF16>(e0, e1);
-          }
-          if (inside && d0 + x + y < w.c.dim)
-            *reinterpret_cast<uint4 *>(out + d0 + x + y) = make_uint4(v[0], v[1], v[2], v[3]);
+          for (int y = 0; y < 32; ++y) o[y] = 0;
         }
+        bad = store32<T>(out, (int64_t)w.c.q_heads * w.c.dim, o, inv, x, w.c.dim, (int)w.c.q_len - (i - lane)) || bad;
       }
-      if (inside && half == 0 && w.c.lse)
+      if (inside && w.c.lse)
         w.c.lse[((int64_t)it.b * w.c.q_heads + h) * w.lse_row + i] = empty ? INFINITY : m * c + log2f(l);
       if (__any_sync(~0u, bad && inside)) {
         // What the row sees may be at fault; recompute it only if something not
@@ -459,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
           }
         }
         for (unsigned left = __ballot_sync(~0u, bad && inside && hidden); left; left &= left - 1)
-          repair_row<T>(w, it.b, h, i - lane + __ffs(left) - 1, d0, d0 + DB * 32);
+          repair_row<T>(w, it.b, h, i - lane + __ffs(left) - 1);
       }
     }
   }

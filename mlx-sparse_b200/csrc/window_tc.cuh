@@ -37,6 +37,42 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+// The largest of three numbers; NaNs are left out.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n"
+      " mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// 2^x of two numbers on the FMA and integer units, for x < 128; NaN stays NaN,
+// below -126 the result is 2^-126. x = n + f with n the nearest integer (read off
+// the low bits of x + 1.5 2^23) and |f| <= 1/2; 2^f is a polynomial of degree 4,
+// the minimax one for the relative error (2.6e-6, a hundredth of float16's half
+// rounding step), found by Remez' exchange.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+  const float2 t = add2(x, make_float2(12582912.f, 12582912.f));
+  const float2 n = add2(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 p = make_float2(9.570102207e-03f, 9.570102207e-03f);
+  p = fma2(p, f, make_float2(5.591785908e-02f, 5.591785908e-02f));
+  p = fma2(p, f, make_float2(2.402474433e-01f, 2.402474433e-01f));
+  p = fma2(p, f, make_float2(6.931217909e-01f, 6.931217909e-01f));
+  p = fma2(p, f, make_float2(9.999992847e-01f, 9.999992847e-01f));
+  const float2 scale = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                                   __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
+  return mul2(p, scale);
+}
+
 template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if (BF16) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -52,12 +88,16 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi, int from) {
   return hi <= lo ? 0u : (~0u >> (32 - hi)) & (~0u << lo);
 }
 
-// Products issued by a warp's leader, of tiles of 128 x 128 and head sizes covered by
-// DB boxes of 64 elements. Scores: both operands K-major in shared memory. Sums:
-// left operand in tensor memory, where each run of W columns of scores holds its
-// 16-bit values in its first W / 2 columns; right operand MN-major in shared
-// memory. Unrolled: the issuing warp is on the critical path of every tile.
-template <int DB, int W> struct Products {
+// Products issued by a warp's leader, of 128 x 128 tiles of scores (64 columns
+// would take nearly as long: 465 clocks against 530); DB boxes of 64 elements cover
+// the head size. Scores: both operands K-major in shared memory. Sums: the left
+// operand in tensor memory, where each run of 64 columns of scores holds its 16-bit
+// values in its first 32; the right operand MN-major in shared memory; half of the
+// 128 rows of it at a time. Unrolled: the issuing warp is on the critical path of
+// every tile.
+constexpr int kHalf = 64;                // columns of scores that are handled together
+constexpr int kHalfBytes = kHalf * 128;  // rows 64.. of a box
+template <int DB> struct Products {
   bool leader;
   int k_steps;
   uint32_t scores_desc, sums_desc;
@@ -74,13 +114,63 @@ template <int DB, int W> struct Products {
         tc::mma_ss(leader, d, x + off, y + off, scores_desc, k > 0);
       }
   }
-  __device__ __forceinline__ void sums(uint32_t d, uint32_t left, uint32_t b, bool add) const {
-    const uint32_t y = tc::desc_mn_major(b, kBox);
+  __device__ __forceinline__ void half_sums(uint32_t d, uint32_t left, uint32_t b, int u, bool add) const {
+    const uint32_t y = tc::desc_mn_major(b + u * kHalfBytes, kBox);
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      tc::mma_ts(leader, d, left + k * 16 / W * W + k * 16 % W / 2, y + (k * 2048 >> 4), sums_desc, add || k > 0);
+    for (int k = 0; k < kHalf / 16; ++k)
+      tc::mma_ts(leader, d, left + u * kHalf + k * 8, y + (k * 2048 >> 4), sums_desc, add || k > 0);
+  }
+  __device__ __forceinline__ void sums(uint32_t d, uint32_t left, uint32_t b, bool add) const {
+    half_sums(d, left, b, 0, add);
+    half_sums(d, left, b, 1, true);
   }
 };
+
+// Writes 32 accumulator columns [d0, d0 + 32) of a warp's 32 rows, scaled and
+// rounded; `first` is the first row, rows from `rows` on are left out. A thread
+// has a row's columns; 4 threads exchange 16-byte pieces so that they write 64
+// bytes of one row together (a row each would be 32 lines for each store: 4096
+// clocks for two slots' tiles). True where a value of this thread's own row is not
+// finite.
+template <typename T>
+__device__ __forceinline__ bool store32(T *first, int64_t row_stride, const uint32_t *o, float scale, int d0, int dim,
+                                        int rows) {
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  const int lane = threadIdx.x & 31, c = lane & 3;
+  float2 odd = make_float2(0.f, 0.f);  // 0 times an infinity or a NaN is NaN
+  uint32_t v[4][4];
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    const bool inside = d0 + 8 * y < dim;  // whole 16-byte pieces
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+      float2 a = make_float2(__uint_as_float(o[8 * y + 2 * z]), __uint_as_float(o[8 * y + 2 * z + 1]));
+      if (!inside) a = make_float2(0.f, 0.f);
+      a = mul2(a, make_float2(scale, scale));
+      odd = fma2(a, make_float2(0.f, 0.f), odd);
+      v[y][z] = pack2<BF16>(a.x, a.y);
+    }
+  }
+  const bool bad = !(odd.x + odd.y == 0.f);
+#pragma unroll
+  for (int bit = 1; bit < 4; bit *= 2)
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      if (!(y & bit)) {
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const uint32_t got = __shfl_xor_sync(~0u, c & bit ? v[y][z] : v[y | bit][z], bit);
+          if (c & bit) v[y][z] = got; else v[y | bit][z] = got;
+        }
+      }
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    const int r = (lane & ~3) + y, d = d0 + 8 * c;
+    if (r < rows && d < dim)
+      *reinterpret_cast<uint4 *>(first + r * row_stride + d) = make_uint4(v[y][0], v[y][1], v[y][2], v[y][3]);
+  }
+  return bad;
+}
 
 // Whether row t of a 16-bit matrix (dim elements from `p`, a multiple of 8,
 // 16-byte aligned) holds an infinity or a NaN; rows outside [0, limit) do not.
