@@ -84,20 +84,21 @@ struct KeyRange {
 
 __device__ __forceinline__ KeyRange key_range(const WindowProblem &w, int b, int first, int last) {
   const int shift = key_count(w, b) - (int)w.c.q_len;
-  int64_t lo = max(first, max(0, -shift)), hi = min(last, (int)w.c.q_len - 1);
+  int lo = max(first, max(0, -shift)), hi = min(last, (int)w.c.q_len - 1);
   if (w.c.indptr != nullptr) {
     const int64_t n = w.c.n_seq;
     auto at = [&](int64_t r) -> int64_t {
       return w.wide_ptr ? static_cast<const int64_t *>(w.c.indptr)[r]
                         : (int64_t) static_cast<const int32_t *>(w.c.indptr)[r];
     };
-    lo = max(lo, at(0)), hi = min(hi, at(n) - 1);
+    lo = (int)max((int64_t)lo, min(at(0), (int64_t)INT_MAX));
+    hi = (int)min((int64_t)hi, max(at(n), (int64_t)0) - 1);
   }
   KeyRange r{0, 0, 0, 0};
   if (lo > hi) return r;
-  const QuerySpan s = query_span(w, b, (int)lo);
+  const QuerySpan s = query_span(w, b, lo);
   if (s.p < 0) return r;
-  r.low = s.low, r.end = (int)hi + shift + 1;
+  r.low = s.low, r.end = hi + shift + 1;
   r.sink0 = s.start, r.sink_end = max(s.start, min(s.start + w.sinks, s.low));
   return r;
 }

@@ -43,8 +43,7 @@ constexpr int kStages = 4;
 struct Params {
   WindowProblem w;
   CUtensorMap q, k, v, g;
-  int64_t items;
-  int q_tiles;
+  int items, q_tiles;
   int *error;
 };
 
@@ -181,8 +180,14 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
   const int i_first = max(0, j0 - shift), i_stop = min((int)w.c.q_len, bars.last - shift + 1);
   const int t0 = i_first / kT, n_tiles = i_stop > i_first ? (i_stop - t0 * kT + kT - 1) / kT : 0;
   const int n = n_tiles * w.group;
-  auto head_of = [&](int it) { return hk * w.group + it / n_tiles; };
-  auto query_of = [&](int it) { return (t0 + it % n_tiles) * kT; };
+  // the pair (head, query tile) that comes next: all tiles of a head, then the next head's
+  struct Walk {
+    int h, t, first, end;
+    __device__ void next() {
+      if (++t == end) t = first, ++h;
+    }
+  };
+  const Walk start{hk * w.group, t0, t0, t0 + n_tiles};
 
   if (warp == 0) {
     if (lane == 0 && n > 0) {
@@ -192,9 +197,11 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
         tma_load_4d(v_tile + x * kBox, &p.v, &bars.kv_full, x * 64, j0, hk, b);
       }
       bool ok = true;
+      Walk at_pair = start;
       for (int e = 0; ok && e < 2 * n; ++e) {  // Q and dO of each pair in turn
         const int s = e % kStages, it = e >> 1;
-        const int h = head_of(it), i0 = query_of(it);
+        if (e > 0 && !(e & 1)) at_pair.next();
+        const int h = at_pair.h, i0 = at_pair.t * kT;
         if (!(ok = bar_wait(&bars.empty[s], (e / kStages & 1) ^ 1, stop, p.error))) break;
         if (e & 1) {
           bar_expect(&bars.full[s], kTile);
@@ -256,8 +263,9 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
     // the queries that all 32 keys of this warp are seen by
     const int all_first = __reduce_max_sync(~0u, key) - shift, all_last = __reduce_min_sync(~0u, own_last) - shift;
     bool ok = true;
-    for (int it = 0; ok && it < n; ++it) {
-      const int i0 = query_of(it) + half * 64;
+    Walk at_pair = start;
+    for (int it = 0; ok && it < n; ++it, at_pair.next()) {
+      const int i0 = at_pair.t * kT + half * 64;
       const float *lse = row_stats + (it & 1) * 2 * kT + half * 64, *delta = lse + kT;
       const bool masked = !(i0 >= all_first && i0 + 63 <= all_last);
       const int c0 = key - shift - i0, c1 = min(own_last - shift, (int)w.c.q_len - 1) - i0 + 1;
@@ -268,14 +276,14 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       fence_after();
       float2 pr[32];
       {
-        uint32_t z[2][16], pk[16];
-        tmem_ld16(t_s + at, z[0]);
+        uint32_t z[kHalf], pk[16];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tmem_ld16(t_s + at + x * 16, z + x * 16);
+        wait_ld();
+        tie32(z), tie32(z + 32);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          wait_ld();
-          if (x < 3) tmem_ld16(t_s + at + (x + 1) * 16, z[(x + 1) & 1]);
-          uint32_t *zz = z[x & 1];
-          tie16(zz);
+          const uint32_t *zz = z + x * 16;
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
             const int col = x * 16 + 2 * y;
@@ -299,14 +307,14 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       if (!(ok = warp_wait(&bars.dp_full, it & 1, stop, p.error))) break;
       fence_after();
       {
-        uint32_t z[2][16], pk[16];
-        tmem_ld16(t_dp + at, z[0]);
+        uint32_t z[kHalf], pk[16];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tmem_ld16(t_dp + at + x * 16, z + x * 16);
+        wait_ld();
+        tie32(z), tie32(z + 32);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          wait_ld();
-          if (x < 3) tmem_ld16(t_dp + at + (x + 1) * 16, z[(x + 1) & 1]);
-          uint32_t *zz = z[x & 1];
-          tie16(zz);
+          const uint32_t *zz = z + x * 16;
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
             const int col = x * 16 + 2 * y;
@@ -352,10 +360,11 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       }
       if (__any_sync(~0u, bad && inside)) {
         bool hidden = false;
-        for (int it = 0; it < n; ++it) {
-          const int i0 = query_of(it);
+        Walk look = start;
+        for (int it = 0; it < n; ++it, look.next()) {
+          const int i0 = look.t * kT;
           if (i0 >= all_first && i0 + kT - 1 <= all_last) continue;
-          const PairDots<T> row(w, b, head_of(it), 0, 0);
+          const PairDots<T> row(w, b, look.h, 0, 0);
           for (int x = 0; x < kT; x += 32) {
             const bool odd = half ? row_not_finite(row.q, w.c.q.token, i0 + x + lane, w.c.q_len, w.c.dim)
                                   : row_not_finite(row.g, (int64_t)w.c.q_heads * w.c.dim, i0 + x + lane, w.c.q_len, w.c.dim);
@@ -411,13 +420,13 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
   __syncthreads();
   fence_after();
   const uint32_t tmem = __shfl_sync(~0u, bars.tmem, 0), t_dp = tmem + 256, t_dq = tmem + 384;  // two score tiles before them
-  auto item = [&](int64_t x, int &b, int &h, int &i0) {  // heads of one key head side by side
-    const int g = (int)(x % w.group);
+  auto item = [&](int x, int &b, int &h, int &i0) {  // heads of one key head side by side
+    const int g = x % w.group;
     x /= w.group;
-    i0 = (int)(x % p.q_tiles) * kT;
+    i0 = x % p.q_tiles * kT;
     x /= p.q_tiles;
-    h = (int)(x % w.c.k_heads) * w.group + g;
-    b = (int)(x / w.c.k_heads);
+    h = x % w.c.k_heads * w.group + g;
+    b = x / w.c.k_heads;
   };
 
   if (warp == 0) {
@@ -425,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
       int stage = 0, b, h, i0;
       uint32_t phase = 1, q_phase = 1;
       bool ok = true;
-      for (int64_t x = blockIdx.x; ok && x < p.items; x += gridDim.x) {
+      for (int x = blockIdx.x; ok && x < p.items; x += gridDim.x) {
         item(x, b, h, i0);
         const KeyTiles<kT> tiles(key_range(w, b, i0, i0 + kT - 1));
         if (tiles.n == 0) continue;
@@ -450,28 +459,28 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
     {
       const Products<DB> mm(BF16, w.c.dim);
       const uint32_t qa = smem_addr(q_tile), ga = smem_addr(g_tile), ra = smem_addr(ring);
-      int64_t done = 0;  // tile pairs of earlier items: K of pair t is ring entry 2 (done + t), V the next
+      uint32_t done = 0;  // tile pairs of earlier items: K of pair t is ring entry 2 (done + t), V the next
       uint32_t q_phase = 0;
       bool ok = true;
-      auto ready = [&](int64_t e) {
-        return ok = ok && warp_wait(&bars.full[e % kStages], (uint32_t)(e / kStages & 1), stop, p.error);
+      auto ready = [&](uint32_t e) {
+        return ok = ok && warp_wait(&bars.full[e % kStages], e / kStages & 1, stop, p.error);
       };
-      auto tile = [&](int64_t e) { return ra + (uint32_t)(e % kStages) * kTile; };
-      auto s_at = [&](int64_t t) { return tmem + (uint32_t)(t & 1) * 128; };
-      for (int64_t x = blockIdx.x; ok && x < p.items; x += gridDim.x) {
+      auto tile = [&](uint32_t e) { return ra + e % kStages * kTile; };
+      auto s_at = [&](uint32_t t) { return tmem + (t & 1) * 128; };
+      for (int x = blockIdx.x; ok && x < p.items; x += gridDim.x) {
         int b, h, i0;
         item(x, b, h, i0);
         const KeyTiles<kT> tiles(key_range(w, b, i0, i0 + kT - 1));
         if (tiles.n == 0) continue;
         if (!(ok = warp_wait(&bars.q_full, q_phase, stop, p.error))) break;
         q_phase ^= 1;
-        auto scores = [&](int64_t t) {
+        auto scores = [&](uint32_t t) {
           if (!ready(2 * t)) return;
           fence_after();
           mm.scores(s_at(t), qa, tile(2 * t));
           mma_commit(mm.leader, &bars.s_full[t & 1]);
         };
-        auto grads = [&](int64_t t, bool last) {
+        auto grads = [&](uint32_t t, bool last) {
           if (!ready(2 * t + 1)) return;
           fence_after();
           mm.scores(t_dp, ga, tile(2 * t + 1));
@@ -482,9 +491,9 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
         scores(done);
         grads(done, tiles.n == 1);
         for (int t = 0; ok && t < tiles.n; ++t) {
-          const int64_t e = done + t;
+          const uint32_t e = done + t;
           if (t + 1 < tiles.n) scores(e + 1);
-          if (!(ok = ok && warp_wait(&bars.ds_full, (uint32_t)(e & 1), stop, p.error))) break;
+          if (!(ok = ok && warp_wait(&bars.ds_full, e & 1, stop, p.error))) break;
           fence_after();
           mm.sums(t_dq, t_dp, tile(2 * e), t > 0);
           mma_commit(mm.leader, &bars.empty[2 * e % kStages]);
@@ -499,10 +508,10 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const float c = w.c.scale * kLog2e;
     const float2 minus_c = make_float2(-c, -c), minus_1 = make_float2(-1.f, -1.f);
-    int64_t done = 0;
+    uint32_t done = 0;
     uint32_t dq_phase = 0;
     bool ok = true;
-    for (int64_t x = blockIdx.x; ok && x < p.items; x += gridDim.x) {
+    for (int x = blockIdx.x; ok && x < p.items; x += gridDim.x) {
       int b, h, i0;
       item(x, b, h, i0);
       const KeyTiles<kT> tiles(key_range(w, b, i0, i0 + kT - 1));
@@ -515,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
       const float lse = inside ? w.c.lse[stat] : INFINITY, delta = inside ? w.c.delta[stat] : 0.f;
       const float2 lse2 = make_float2(lse, lse), delta2 = make_float2(delta, delta);
       for (int t = 0; t < tiles.n; ++t) {
-        const int64_t e = done + t;
+        const uint32_t e = done + t;
         const int j0 = tiles.first(t) + half * 64, j1 = tiles.end(t);
         const bool masked = !(j0 >= all_low && j0 + 64 <= all_end && j1 - j0 >= 64);
         uint32_t seen[2];
@@ -524,19 +533,19 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
                     s1 = min(span.sink_end, j1) - j0;
           seen[0] = bits(b0, b1, 0) | bits(s0, s1, 0), seen[1] = bits(b0, b1, 32) | bits(s0, s1, 32);
         }
-        if (!(ok = warp_wait(&bars.s_full[e & 1], (uint32_t)(e >> 1 & 1), stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.s_full[e & 1], e >> 1 & 1, stop, p.error))) break;
         fence_after();
-        const uint32_t t_s = tmem + (uint32_t)(e & 1) * 128 + lanes + half * 64, t_d = t_dp + lanes + half * 64;
+        const uint32_t t_s = tmem + (e & 1) * 128 + lanes + half * 64, t_d = t_dp + lanes + half * 64;
         float2 pr[32];
         {
-          uint32_t z[2][16];
-          tmem_ld16(t_s, z[0]);
+          uint32_t z[kHalf];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) tmem_ld16(t_s + y * 16, z + y * 16);
+          wait_ld();
+          tie32(z), tie32(z + 32);
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            wait_ld();
-            if (y < 3) tmem_ld16(t_s + (y + 1) * 16, z[(y + 1) & 1]);
-            uint32_t *zz = z[y & 1];
-            tie16(zz);
+            const uint32_t *zz = z + y * 16;
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
               const int col = y * 16 + 2 * u;
@@ -550,17 +559,17 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
             }
           }
         }
-        if (!(ok = warp_wait(&bars.dp_full, (uint32_t)(e & 1), stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.dp_full, e & 1, stop, p.error))) break;
         fence_after();
         {
-          uint32_t z[2][16], pk[16];
-          tmem_ld16(t_d, z[0]);
+          uint32_t z[kHalf], pk[16];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) tmem_ld16(t_d + y * 16, z + y * 16);
+          wait_ld();
+          tie32(z), tie32(z + 32);
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            wait_ld();
-            if (y < 3) tmem_ld16(t_d + (y + 1) * 16, z[(y + 1) & 1]);
-            uint32_t *zz = z[y & 1];
-            tie16(zz);
+            const uint32_t *zz = z + y * 16;
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
               const int col = y * 16 + 2 * u;
@@ -636,7 +645,7 @@ template <typename T, int DB> void launch(Params &p, cudaStream_t s) {
   if (w.c.dq && w.c.q_len > 0) {
     auto kernel = dq_tc_kernel<T, DB>;
     MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kQSmem<DB>));
-    kernel<<<(unsigned)std::min<int64_t>(p.items, num_sms()), kThreads, kQSmem<DB>, s>>>(p);
+    kernel<<<(unsigned)std::min(p.items, num_sms()), kThreads, kQSmem<DB>, s>>>(p);
     MSX_CHECK_LAUNCH();
   }
   if (w.c.dk) {
@@ -667,7 +676,9 @@ void window_backward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s)
   p.k = make_map(w.c.k, w.c.batch, w.c.k_len, w.c.k_heads, dim, bf16, kT);
   p.v = make_map(w.c.v, w.c.batch, w.c.k_len, w.c.k_heads, dim, bf16, kT);
   p.q_tiles = (int)ceil_div(w.c.q_len, kT);
-  p.items = w.c.batch * heads * p.q_tiles;
+  const int64_t items = w.c.batch * heads * p.q_tiles;
+  if (items > INT32_MAX / 2) fail(MSX_ERR_OVERFLOW, "window_attention has too many queries and heads for one call.");
+  p.items = (int)items;
   p.error = window_error_flag();
   if (bf16) {
     if (dim <= 64) launch<__nv_bfloat16, 1>(p, s); else launch<__nv_bfloat16, 2>(p, s);

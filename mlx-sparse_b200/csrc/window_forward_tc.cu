@@ -58,8 +58,7 @@ template <int DB> struct Shape {  // DB boxes of 64 elements cover the head size
 struct Params {
   WindowProblem w;
   CUtensorMap q, k, v;
-  int64_t items;
-  int q_tiles, paired;
+  int items, q_tiles, paired;
   int *error;
 };
 
@@ -71,28 +70,28 @@ struct Item {
   int last[2];  // the last tile of keys that a slot takes part in, -1: none
 };
 
-__device__ __forceinline__ Item item_of(const Params &p, int64_t n) {
+__device__ __forceinline__ Item item_of(const Params &p, int n) {
   const WindowProblem &w = p.w;
   Item it;
   if (p.paired) {
     const int pairs = w.group / 2;
-    const int pair = (int)(n % pairs);
+    const int pair = n % pairs;
     n /= pairs;
-    it.i0[0] = it.i0[1] = (int)(n % p.q_tiles) * kM;
+    it.i0[0] = it.i0[1] = n % p.q_tiles * kM;
     n /= p.q_tiles;
-    it.hk = (int)(n % w.c.k_heads);
-    it.b = (int)(n / w.c.k_heads);
+    it.hk = n % w.c.k_heads;
+    it.b = n / w.c.k_heads;
     it.head[0] = it.hk * w.group + 2 * pair;
     it.head[1] = it.head[0] + 1;
     it.both = it.range[0] = it.range[1] = key_range(w, it.b, it.i0[0], it.i0[0] + kM - 1);
     it.last[0] = it.last[1] = KeyTiles<kN>(it.both).n - 1;
   } else {
     const int blocks = (p.q_tiles + 1) / 2;
-    const int h = (int)(n / blocks % w.c.q_heads);
-    it.b = (int)(n / blocks / w.c.q_heads);
+    const int h = n / blocks % w.c.q_heads;
+    it.b = n / blocks / w.c.q_heads;
     it.hk = h / w.group;
     it.head[0] = it.head[1] = h;
-    it.i0[0] = (int)(n % blocks) * 2 * kM;
+    it.i0[0] = n % blocks * 2 * kM;
     it.i0[1] = it.i0[0] + kM;
     it.both = key_range(w, it.b, it.i0[0], it.i0[1] + kM - 1);
     const KeyTiles<kN> tiles(it.both);
@@ -195,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
       for (int x = 0; x < Sh::stages; ++x) freed[x] = -1;
       int stage = 0;
       bool ok = true;
-      for (int64_t n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
+      for (int n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
         const Item it = item_of(p, n);
         const KeyTiles<kN> tiles(it.both);
 #pragma unroll
@@ -234,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
     auto next = [&] {
       if (++stage == Sh::stages) stage = 0, phase ^= 1;
     };
-    for (int64_t n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
+    for (int n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
       const Item it = item_of(p, n);
       const KeyTiles<kN> tiles(it.both);
       if (tiles.n == 0) continue;
@@ -253,7 +252,6 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         }
       // the stage of K_0 is now, V_t and K_{t+1} follow in turn
       if (!need(warp_wait(&bars.kv_full[stage], phase, stop, p.error))) break;
-      fence_after();
 #pragma unroll
       for (int s = 0; s < 2; ++s)
         if (takes(s, 0)) scores(s, stage, it.last[s] == 0);
@@ -275,10 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
             p_phase[s] ^= 1;
             started[s] = true;
           }
-          if (s == 0 && more) {
-            need(warp_wait(&bars.kv_full[k_stage], phase, stop, p.error));
-            fence_after();
-          }
+          if (s == 0 && more) need(warp_wait(&bars.kv_full[k_stage], phase, stop, p.error));
           if (then[s]) scores(s, k_stage, it.last[s] == t + 1);
         }
         mma_commit(mm.leader, &bars.step[steps++ & 7]);
@@ -293,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
     const float c = w.c.scale * kLog2e;
     uint32_t s_phase = 0, o_phase = 0;
     bool ok = true;
-    for (int64_t n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
+    for (int n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
       const Item it = item_of(p, n);
       const KeyTiles<kN> tiles(it.both);
       const KeyRange range = s ? it.range[1] : it.range[0];
@@ -391,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
       const float inv = empty ? 0.f : 1.f / l;
       T *out = static_cast<T *>(w.c.out) + ((it.b * w.c.q_len + i - lane) * w.c.q_heads + h) * w.c.dim;
       bool bad = false;
-#pragma unroll 1
+#pragma unroll
       for (int x = 0; x < DB * 64; x += 32) {
         uint32_t o[32];
         if (started) {
@@ -443,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
 template <typename T, int DB> void launch(Params &p, cudaStream_t s) {
   auto kernel = forward_tc_kernel<T, DB>;
   MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DB>::smem));
-  kernel<<<(unsigned)std::min<int64_t>(p.items, num_sms()), kThreads, Shape<DB>::smem, s>>>(p);
+  kernel<<<(unsigned)std::min(p.items, num_sms()), kThreads, Shape<DB>::smem, s>>>(p);
   MSX_CHECK_LAUNCH();
 }
 
@@ -482,8 +477,10 @@ void window_forward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s) 
   p.v = make_map(w.c.v, w.c.batch, w.c.k_len, w.c.k_heads, w.c.dim, bf16, kN);
   p.q_tiles = (int)ceil_div(w.c.q_len, kM);
   p.paired = w.group % 2 == 0;
-  p.items = p.paired ? w.c.batch * w.c.k_heads * p.q_tiles * (w.group / 2)
-                     : w.c.batch * w.c.q_heads * ((p.q_tiles + 1) / 2);
+  const int64_t items = p.paired ? w.c.batch * w.c.k_heads * p.q_tiles * (w.group / 2)
+                                 : w.c.batch * w.c.q_heads * ((p.q_tiles + 1) / 2);
+  if (items > INT32_MAX / 2) fail(MSX_ERR_OVERFLOW, "window_attention has too many queries and heads for one call.");
+  p.items = (int)items;
   p.error = window_error_flag();
   if (bf16) {
     if (w.c.dim <= 64) launch<__nv_bfloat16, 1>(p, s); else launch<__nv_bfloat16, 2>(p, s);

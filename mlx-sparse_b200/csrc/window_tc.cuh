@@ -92,11 +92,9 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi, int from) {
 // would take nearly as long: 465 clocks against 530); DB boxes of 64 elements cover
 // the head size. Scores: both operands K-major in shared memory. Sums: the left
 // operand in tensor memory, where each run of 64 columns of scores holds its 16-bit
-// values in its first 32; the right operand MN-major in shared memory; half of the
-// 128 rows of it at a time. Unrolled: the issuing warp is on the critical path of
+// values in its first 32; the right operand MN-major in shared memory. Unrolled: the issuing warp is on the critical path of
 // every tile.
 constexpr int kHalf = 64;                // columns of scores that are handled together
-constexpr int kHalfBytes = kHalf * 128;  // rows 64.. of a box
 template <int DB> struct Products {
   bool leader;
   int k_steps;
@@ -114,15 +112,11 @@ template <int DB> struct Products {
         tc::mma_ss(leader, d, x + off, y + off, scores_desc, k > 0);
       }
   }
-  __device__ __forceinline__ void half_sums(uint32_t d, uint32_t left, uint32_t b, int u, bool add) const {
-    const uint32_t y = tc::desc_mn_major(b + u * kHalfBytes, kBox);
-#pragma unroll
-    for (int k = 0; k < kHalf / 16; ++k)
-      tc::mma_ts(leader, d, left + u * kHalf + k * 8, y + (k * 2048 >> 4), sums_desc, add || k > 0);
-  }
   __device__ __forceinline__ void sums(uint32_t d, uint32_t left, uint32_t b, bool add) const {
-    half_sums(d, left, b, 0, add);
-    half_sums(d, left, b, 1, true);
+    const uint32_t y = tc::desc_mn_major(b, kBox);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      tc::mma_ts(leader, d, left + (k >> 2) * kHalf + (k & 3) * 8, y + (k * 2048 >> 4), sums_desc, add || k > 0);
   }
 };
 
