@@ -500,7 +500,13 @@ MSX_API int msx_csr_distill_forward_backward(
  * out, grad_out, dq are contiguous like q; dk, dv like k. lse: float (batch,
  * q_heads, q_len rounded up to a multiple of 128), 16-byte aligned, written by
  * forward (null: not wanted), read by backward;
- * delta: float workspace of the same size. backward reads forward's out. */
+ * workspace: *floats of msx_window_attention_workspace, 16-byte aligned, for
+ * backward alone. backward reads forward's out. */
+MSX_API int msx_window_attention_workspace(int64_t batch, int64_t q_len,
+                                           int64_t k_len, int64_t q_heads,
+                                           int64_t k_heads, int64_t dim,
+                                           int64_t window, int64_t sinks,
+                                           int64_t *floats);
 MSX_API int msx_window_attention_forward(
     int value_dtype, const void *q, const int64_t *q_strides, const void *k,
     const int64_t *k_strides, const void *v, const int64_t *v_strides,
@@ -514,7 +520,7 @@ MSX_API int msx_window_attention_backward(
     int64_t batch, int64_t q_len, int64_t k_len, int64_t q_heads,
     int64_t k_heads, int64_t dim, int64_t window, int64_t sinks, float scale,
     int index_dtype, const void *indptr, int64_t n_seq, const void *out,
-    const float *lse, const void *grad_out, float *delta, void *dq, void *dk,
+    const float *lse, const void *grad_out, float *workspace, void *dq, void *dk,
     void *dv, void *stream);
 /* One query for each batch entry, at the end of that entry's cache: q (batch,
  * q_heads, dim) with strides {batch, heads}; caches (batch, max_len, k_heads,

@@ -679,6 +679,17 @@ static void window_packed(WindowCall &c, const void *indptr, int64_t n_seq) {
   c.indptr = indptr, c.n_seq = n_seq;
 }
 
+int msx_window_attention_workspace(int64_t batch, int64_t q_len, int64_t k_len, int64_t q_heads, int64_t k_heads,
+                                   int64_t dim, int64_t window, int64_t sinks, int64_t *floats) {
+  return guarded([&] {
+    const int64_t none[3] = {0, 0, 0};
+    require(floats != nullptr, MSX_ERR_INVALID, "window_attention floats must not be null.");
+    const int some = 0;  // stands for operands that this call does not read
+    *floats = window_backward_floats(window_checked(MSX_F32, &some, none, &some, none, &some, none, batch, q_len, k_len,
+                                                    q_heads, k_heads, dim, window, sinks, 1.f, MSX_I32));
+  });
+}
+
 int msx_window_attention_forward(int value_dtype, const void *q, const int64_t *q_strides, const void *k,
                                  const int64_t *k_strides, const void *v, const int64_t *v_strides, int64_t batch,
                                  int64_t q_len, int64_t k_len, int64_t q_heads, int64_t k_heads, int64_t dim,
@@ -699,7 +710,7 @@ int msx_window_attention_backward(int value_dtype, const void *q, const int64_t 
                                   int64_t q_len, int64_t k_len, int64_t q_heads, int64_t k_heads, int64_t dim,
                                   int64_t window, int64_t sinks, float scale, int index_dtype, const void *indptr,
                                   int64_t n_seq, const void *out, const float *lse, const void *grad_out,
-                                  float *delta, void *dq, void *dk, void *dv, void *stream) {
+                                  float *workspace, void *dq, void *dk, void *dv, void *stream) {
   return guarded([&] {
     WindowCall c = window_checked(value_dtype, q, q_strides, k, k_strides, v, v_strides, batch, q_len, k_len, q_heads,
                                   k_heads, dim, window, sinks, scale, index_dtype);
@@ -707,9 +718,9 @@ int msx_window_attention_backward(int value_dtype, const void *q, const int64_t 
     check_ptr(out, batch * q_len, "window_attention out");
     check_ptr(lse, batch * q_len, "window_attention lse");
     check_ptr(grad_out, batch * q_len, "window_attention grad_out");
-    check_ptr(delta, batch * q_len, "window_attention delta");
+    check_ptr(workspace, batch * q_len, "window_attention workspace");
     require((dk == nullptr) == (dv == nullptr), MSX_ERR_INVALID, "window_attention dk and dv come together.");
-    c.out = const_cast<void *>(out), c.lse = const_cast<float *>(lse), c.grad_out = grad_out, c.delta = delta;
+    c.out = const_cast<void *>(out), c.lse = const_cast<float *>(lse), c.grad_out = grad_out, c.delta = workspace;
     c.dq = dq, c.dk = dk, c.dv = dv;
     window_backward_run(value_dtype, c, as_stream(stream));
   });

@@ -56,7 +56,8 @@ void distill_run(int value_dtype, int index_dtype, const DistillCall &call, cuda
 // Windowed attention. q, k, v: (batch, tokens, heads, dim) with any batch,
 // token and head strides (in elements) and stride 1 along dim; out, grad_out and
 // the gradients are contiguous in that order. lse and delta: float (batch,
-// q_heads, q_len rounded up to a multiple of 128). A null dq (dk and dv) is not computed.
+// q_heads, q_len rounded up to a multiple of 128), delta followed by more workspace
+// (window_backward_floats in all). A null dq (dk and dv) is not computed.
 struct WindowTensor {
   const void *ptr;
   int64_t batch, token, head;
@@ -76,6 +77,7 @@ struct WindowCall {
   const void *lengths;  // keys of each batch entry (type indptr_dtype), or null: k_len
 };
 void window_forward_run(int value_dtype, const WindowCall &c, cudaStream_t s);
+int64_t window_backward_floats(const WindowCall &c);
 void window_decode_run(int value_dtype, const WindowCall &c, cudaStream_t s);
 bool window_take_error();  // reads and clears the device's wait error flag
 void window_backward_run(int value_dtype, const WindowCall &c, cudaStream_t s);

@@ -330,6 +330,11 @@ static WindowProblem problem(const WindowCall &c) {
   return w;
 }
 
+int64_t window_backward_floats(const WindowCall &c) {
+  const WindowProblem w = problem(c);
+  return c.batch * c.q_heads * w.lse_row + window_backward_floats_tc(w);
+}
+
 void window_forward_run(int value_dtype, const WindowCall &c, cudaStream_t s) {
   const WindowProblem w = problem(c);
   if (window_tc_ok(w, value_dtype))

@@ -133,6 +133,7 @@ void window_backward_general(const WindowProblem &w, int value_dtype, cudaStream
 bool window_tc_ok(const WindowProblem &w, int value_dtype);
 void window_forward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s);
 void window_backward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s);
+int64_t window_backward_floats_tc(const WindowProblem &w);  // workspace behind delta
 // One query for each sequence (window_decode.cu).
 void window_decode(const WindowProblem &w, int value_dtype, cudaStream_t s);
 void window_delta(const WindowProblem &w, int value_dtype, cudaStream_t s);

@@ -8,6 +8,14 @@
 //         every head that shares it: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO,
 //         dK += dS^T Q.
 //
+// A sink key is seen by every later query of its sequence. Where that would make a
+// few key tiles much longer than the rest, the queries are cut into chunks: the
+// key tile itself takes the queries of its band and of the chunk that the sequence
+// starts in, and every later chunk has a CTA of its own for the sinks of its first
+// query's sequence (a sequence that starts later in the chunk is in its own first
+// chunk). Their sums go to a workspace in fp32, a slot for each chunk, and the key
+// tile adds them in the order of the chunks.
+//
 // P = 2^(c S - lse) is recomputed from the forward pass's log-sum-exp. That is 7
 // products of 128 x 128 x dim for each tile pair where one kernel with atomic
 // sums of dQ would make 5; atomics would change results from run to run.
@@ -45,7 +53,31 @@ struct Params {
   CUtensorMap q, k, v, g;
   int items, q_tiles;
   int *error;
+  // far queries of the sinks: queries of a chunk (0: not cut), chunks, and sums
+  // [batch][key head][chunk][sink][dV, dK][dim]
+  int chunk, n_chunks;
+  float *far;
 };
+
+// The first chunk that takes a sequence's queries away from the key tiles.
+__device__ __forceinline__ int first_far_chunk(const Params &p, int start) {
+  const int i = start - p.w.offset;
+  return i < 0 ? 0 : i / p.chunk + 1;
+}
+
+// The last query position that a key's own tile takes (at least; it takes whole
+// tiles of queries).
+__device__ __forceinline__ int last_near_query(const Params &p, int j) {
+  const WindowProblem &w = p.w;
+  if (p.chunk == 0) return last_query(w, j);
+  if (j >= w.c.k_len) return -1;
+  int start, end;
+  sequence_of(w, j, start, end);
+  if (start >= end) return -1;
+  int last = j + w.window - 1;
+  if (j - start < w.sinks) last = max(last, first_far_chunk(p, start) * p.chunk - 1 + w.offset);
+  return min(end - 1, last);
+}
 
 // The score of one pair times log2(e) and dO_i . V_j, from global memory.
 template <typename T> struct PairDots {
@@ -139,9 +171,13 @@ struct KvBars {
   int stop, last;
 };
 
+// Key tiles that a sequence's sinks can touch.
+__host__ __device__ inline int far_key_tiles(const WindowProblem &w) { return (w.sinks + kT - 2) / kT + 1; }
+
 template <int DB> constexpr int kKvSmem = 1024 + (2 + kStages) * DB * kBox + 2 * 2 * kT * 4;
 
-template <typename T, int DB>
+// FAR: the sinks of one sequence against one chunk of queries.
+template <typename T, int DB, bool FAR>
 __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_constant__ Params p) {
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kTile = DB * kBox;
@@ -152,10 +188,23 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
   float *row_stats = reinterpret_cast<float *>(ring + kStages * kTile);  // two of {lse[128], delta[128]}
   const WindowProblem &w = p.w;
   const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int hk = (int)(blockIdx.x % w.c.k_heads);
-  const int b = (int)(blockIdx.x / w.c.k_heads % w.c.batch);
-  const int j0 = (int)(blockIdx.x / w.c.k_heads / w.c.batch) * kT;
   const int shift = w.offset;
+  int x = (int)blockIdx.x;
+  const int hk = x % w.c.k_heads;
+  x /= w.c.k_heads;
+  const int b = x % (int)w.c.batch;
+  x /= (int)w.c.batch;
+  int j0, chunk = 0, far_start = 0, far_end = 0;
+  if (FAR) {
+    const int n_tiles = far_key_tiles(w);
+    chunk = x / n_tiles;
+    const int p0 = chunk * p.chunk + shift;
+    if (p0 >= 0) sequence_of(w, p0, far_start, far_end);
+    j0 = (far_start / kT + x % n_tiles) * kT;
+    if (far_start >= far_end || first_far_chunk(p, far_start) > chunk || j0 >= min(far_start + w.sinks, far_end)) return;
+  } else {
+    j0 = x * kT;
+  }
   volatile int *stop = &bars.stop;
   if (threadIdx.x == 0) {
     bar_init(&bars.kv_full, 1);
@@ -165,21 +214,31 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
     bars.stop = 0, bars.last = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  __syncthreads();
+  // the tiles of queries that see any of these keys
+  const int key = j0 + (warp & 3) * 32 + lane;
+  if (warp >= 4 && warp < 8) {
+    const int top = __reduce_max_sync(~0u, last_near_query(p, key));
+    if (lane == 0) atomicMax(&bars.last, top);
+  }
+  __syncthreads();
+  const int i_first = max(0, j0 - shift), i_stop = min((int)w.c.q_len, bars.last - shift + 1);
+  int t0 = i_first / kT, n_tiles = i_stop > i_first ? (i_stop - t0 * kT + kT - 1) / kT : 0;
+  const int near_end = (t0 + n_tiles) * kT;  // queries from here on are the chunks'
+  int first_i = key - shift, last_i = min(last_query(w, key) - shift, (int)w.c.q_len - 1);
+  if (FAR) {
+    const int from = max(chunk * p.chunk, near_end), to = min((chunk + 1) * p.chunk, far_end - shift);
+    if (from >= to) return;
+    t0 = from / kT, n_tiles = (to - from + kT - 1) / kT;
+    const bool sink = key >= far_start && key < min(far_start + w.sinks, far_end);
+    first_i = sink ? from : INT_MAX, last_i = sink ? to - 1 : -1;
+  }
+  const int n = n_tiles * w.group;
   if (warp == 2) tmem_alloc(&bars.tmem, 512);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = __shfl_sync(~0u, bars.tmem, 0), t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
-  // the tiles of queries that see any of these keys
-  const int key = j0 + (warp & 3) * 32 + lane, own_last = last_query(w, key);
-  if (warp >= 4 && warp < 8) {
-    const int top = __reduce_max_sync(~0u, own_last);
-    if (lane == 0) atomicMax(&bars.last, top);
-  }
-  __syncthreads();
-  const int i_first = max(0, j0 - shift), i_stop = min((int)w.c.q_len, bars.last - shift + 1);
-  const int t0 = i_first / kT, n_tiles = i_stop > i_first ? (i_stop - t0 * kT + kT - 1) / kT : 0;
-  const int n = n_tiles * w.group;
   // the pair (head, query tile) that comes next: all tiles of a head, then the next head's
   struct Walk {
     int h, t, first, end;
@@ -187,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       if (++t == end) t = first, ++h;
     }
   };
-  const Walk start{hk * w.group, t0, t0, t0 + n_tiles};
+  const Walk first_pair{hk * w.group, t0, t0, t0 + n_tiles};
 
   if (warp == 0) {
     if (lane == 0 && n > 0) {
@@ -197,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
         tma_load_4d(v_tile + x * kBox, &p.v, &bars.kv_full, x * 64, j0, hk, b);
       }
       bool ok = true;
-      Walk at_pair = start;
+      Walk at_pair = first_pair;
       for (int e = 0; ok && e < 2 * n; ++e) {  // Q and dO of each pair in turn
         const int s = e % kStages, it = e >> 1;
         if (e > 0 && !(e & 1)) at_pair.next();
@@ -261,21 +320,21 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
     const float c = w.c.scale * kLog2e;
     const float2 minus_c = make_float2(-c, -c), minus_1 = make_float2(-1.f, -1.f);
     // the queries that all 32 keys of this warp are seen by
-    const int all_first = __reduce_max_sync(~0u, key) - shift, all_last = __reduce_min_sync(~0u, own_last) - shift;
+    const int all_first = __reduce_max_sync(~0u, first_i), all_last = __reduce_min_sync(~0u, last_i);
     bool ok = true;
-    Walk at_pair = start;
+    Walk at_pair = first_pair;
     for (int it = 0; ok && it < n; ++it, at_pair.next()) {
       const int i0 = at_pair.t * kT + half * 64;
       const float *lse = row_stats + (it & 1) * 2 * kT + half * 64, *delta = lse + kT;
       const bool masked = !(i0 >= all_first && i0 + 63 <= all_last);
-      const int c0 = key - shift - i0, c1 = min(own_last - shift, (int)w.c.q_len - 1) - i0 + 1;
-      const uint32_t seen[2] = {bits(c0, c1, 0), bits(c0, c1, 32)};
+      const uint32_t seen[2] = {first_i > last_i ? 0 : bits(first_i - i0, last_i + 1 - i0, 0),
+                                first_i > last_i ? 0 : bits(first_i - i0, last_i + 1 - i0, 32)};
       // lse and delta came with Q's tile, which the products of s_full have read
       if (!(ok = warp_wait(&bars.full[2 * it % kStages], 2 * it / kStages & 1, stop, p.error))) break;
       if (!(ok = warp_wait(&bars.s_full, it & 1, stop, p.error))) break;
       fence_after();
       float2 pr[32];
-      {
+      auto weights = [&](auto mask) {
         uint32_t z[kHalf], pk[16];
 #pragma unroll
         for (int x = 0; x < 4; ++x) tmem_ld16(t_s + at + x * 16, z + x * 16);
@@ -290,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
             float2 e = fma2(make_float2(__uint_as_float(zz[2 * y]), __uint_as_float(zz[2 * y + 1])), minus_c,
                             *reinterpret_cast<const float2 *>(lse + col));
             e.x = exp2_fast(-e.x), e.y = exp2_fast(-e.y);
-            if (masked) {
+            if (mask) {
               if (!(seen[col >> 5] >> (col & 31) & 1)) e.x = 0.f;
               if (!(seen[col >> 5] >> (col & 31) & 2)) e.y = 0.f;
             }
@@ -299,14 +358,15 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
           }
           if (x & 1) tmem_st16(t_s + at + (x >> 1) * 16, pk);
         }
-      }
+      };
+      if (masked) weights(std::true_type{}); else weights(std::false_type{});
       wait_st();
       fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive(&bars.p_full);
       if (!(ok = warp_wait(&bars.dp_full, it & 1, stop, p.error))) break;
       fence_after();
-      {
+      auto grads = [&](auto mask) {
         uint32_t z[kHalf], pk[16];
 #pragma unroll
         for (int x = 0; x < 4; ++x) tmem_ld16(t_dp + at + x * 16, z + x * 16);
@@ -322,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
             float2 e = fma2(make_float2(__uint_as_float(zz[2 * y]), __uint_as_float(zz[2 * y + 1])), minus_1,
                             *reinterpret_cast<const float2 *>(delta + col));
             e = mul2(e, pr[x * 8 + y]);
-            if (masked) {
+            if (mask) {
               if (!(seen[col >> 5] >> (col & 31) & 1)) e.x = 0.f;
               if (!(seen[col >> 5] >> (col & 31) & 2)) e.y = 0.f;
             }
@@ -330,7 +390,8 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
           }
           if (x & 1) tmem_st16(t_dp + at + (x >> 1) * 16, pk);
         }
-      }
+      };
+      if (masked) grads(std::true_type{}); else grads(std::false_type{});
       wait_st();
       fence_before();
       __syncwarp();
@@ -341,39 +402,76 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       fence_after();
       // the first warpgroup writes dV, the second dK
       const bool inside = key < w.c.k_len;
-      T *out = static_cast<T *>(half ? w.c.dk : w.c.dv) + ((b * w.c.k_len + key - lane) * w.c.k_heads + hk) * w.c.dim;
       const uint32_t from = (half ? t_dk : t_dv) + ((uint32_t)(warp & 3) << 21);
+      const float scale = half ? -w.c.scale : 1.f;
+      int start = 0, end = 0, c0 = 0, c1 = 0;  // the chunks that have sums for this key
+      if (p.chunk && inside) {
+        sequence_of(w, key, start, end);
+        if (key < min(start + w.sinks, end) && near_end < end - shift) {
+          c0 = max(first_far_chunk(p, start), near_end / p.chunk);
+          c1 = min(p.n_chunks, (end - shift + p.chunk - 1) / p.chunk);
+        }
+      }
+      float *far = nullptr;  // the sums of a chunk: far + chunk * far_step
+      const int64_t far_step = (int64_t)w.sinks * 2 * w.c.dim;
+      if (p.chunk) far = p.far + ((((int64_t)b * w.c.k_heads + hk) * p.n_chunks * w.sinks + key - start) * 2 + half) * w.c.dim;
+      T *out = static_cast<T *>(half ? w.c.dk : w.c.dv) + ((b * w.c.k_len + key - lane) * w.c.k_heads + hk) * w.c.dim;
       bool bad = false;
 #pragma unroll 1
-      for (int x = 0; x < DB * 64; x += 32) {
+      for (int d = 0; d < DB * 64; d += 32) {
         uint32_t o[32];
         if (n > 0) {
-          tmem_ld32(from + x, o);
+          tmem_ld16(from + d, o), tmem_ld16(from + d + 16, o + 16);
           wait_ld();
           tie32(o);
         } else {
 #pragma unroll
           for (int y = 0; y < 32; ++y) o[y] = 0;
         }
-        bad = store32<T>(out, (int64_t)w.c.k_heads * w.c.dim, o, half ? -w.c.scale : 1.f, x, w.c.dim,
-                         (int)w.c.k_len - (key - lane)) || bad;
+        if (FAR) {
+          if (first_i <= last_i)
+#pragma unroll
+            for (int y = 0; y < 32; y += 4)
+              if (d + y < w.c.dim)
+                *reinterpret_cast<float4 *>(far + chunk * far_step + d + y) =
+                    make_float4(__uint_as_float(o[y]), __uint_as_float(o[y + 1]), __uint_as_float(o[y + 2]),
+                                __uint_as_float(o[y + 3]));
+          continue;
+        }
+        for (int c = c0; c < c1; ++c)
+#pragma unroll
+          for (int y = 0; y < 32; y += 4)
+            if (d + y < w.c.dim) {
+              const float4 f = *reinterpret_cast<const float4 *>(far + c * far_step + d + y);
+              o[y] = __float_as_uint(__uint_as_float(o[y]) + f.x);
+              o[y + 1] = __float_as_uint(__uint_as_float(o[y + 1]) + f.y);
+              o[y + 2] = __float_as_uint(__uint_as_float(o[y + 2]) + f.z);
+              o[y + 3] = __float_as_uint(__uint_as_float(o[y + 3]) + f.w);
+            }
+        bad = store32<T>(out, (int64_t)w.c.k_heads * w.c.dim, o, scale, d, w.c.dim, (int)w.c.k_len - (key - lane)) || bad;
       }
-      if (__any_sync(~0u, bad && inside)) {
+      if (!FAR && __any_sync(~0u, bad && inside)) {
         bool hidden = false;
-        Walk look = start;
-        for (int it = 0; it < n; ++it, look.next()) {
-          const int i0 = look.t * kT;
-          if (i0 >= all_first && i0 + kT - 1 <= all_last) continue;
-          const PairDots<T> row(w, b, look.h, 0, 0);
-          for (int x = 0; x < kT; x += 32) {
-            const bool odd = half ? row_not_finite(row.q, w.c.q.token, i0 + x + lane, w.c.q_len, w.c.dim)
-                                  : row_not_finite(row.g, (int64_t)w.c.q_heads * w.c.dim, i0 + x + lane, w.c.q_len, w.c.dim);
+        auto look_at = [&](int h, int i0, int first, int last) {
+          const PairDots<T> row(w, b, h, 0, 0);
+          for (int y = 0; y < kT; y += 32) {
+            const bool odd = half ? row_not_finite(row.q, w.c.q.token, i0 + y + lane, w.c.q_len, w.c.dim)
+                                  : row_not_finite(row.g, (int64_t)w.c.q_heads * w.c.dim, i0 + y + lane, w.c.q_len, w.c.dim);
             for (unsigned left = __ballot_sync(~0u, odd); left; left &= left - 1) {
-              const int i = i0 + x + __ffs(left) - 1;
-              hidden = hidden || i < key - shift || i > own_last - shift;
+              const int i = i0 + y + __ffs(left) - 1;
+              hidden = hidden || i < first || i > last;
             }
           }
-        }
+        };
+        Walk look = first_pair;
+        for (int it = 0; it < n; ++it, look.next())
+          if (!(look.t * kT >= all_first && look.t * kT + kT - 1 <= all_last)) look_at(look.h, look.t * kT, first_i, last_i);
+        // of a sink's far queries' tiles only the sequence's last holds other queries
+        const int stop_i = c0 < c1 ? end - shift : 0, most = __reduce_max_sync(~0u, stop_i);
+        if (most > 0)
+          for (int h = hk * w.group; h < (hk + 1) * w.group; ++h)
+            look_at(h, (most - 1) / kT * kT, 0, stop_i > 0 ? stop_i - 1 : INT_MAX);
+        if (stop_i > 0 && stop_i < most) hidden = true;
         for (unsigned left = __ballot_sync(~0u, bad && inside && hidden); left; left &= left - 1)
           repair_dkv<T>(w, b, hk, key - lane + __ffs(left) - 1, half != 0);
       }
@@ -537,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
         fence_after();
         const uint32_t t_s = tmem + (e & 1) * 128 + lanes + half * 64, t_d = t_dp + lanes + half * 64;
         float2 pr[32];
-        {
+        auto weights = [&](auto mask) {
           uint32_t z[kHalf];
 #pragma unroll
           for (int y = 0; y < 4; ++y) tmem_ld16(t_s + y * 16, z + y * 16);
@@ -551,17 +649,18 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
               const int col = y * 16 + 2 * u;
               float2 f = fma2(make_float2(__uint_as_float(zz[2 * u]), __uint_as_float(zz[2 * u + 1])), minus_c, lse2);
               f.x = exp2_fast(-f.x), f.y = exp2_fast(-f.y);
-              if (masked) {
+              if (mask) {
                 if (!(seen[col >> 5] >> (col & 31) & 1)) f.x = 0.f;
                 if (!(seen[col >> 5] >> (col & 31) & 2)) f.y = 0.f;
               }
               pr[y * 8 + u] = f;
             }
           }
-        }
+        };
+        if (masked) weights(std::true_type{}); else weights(std::false_type{});
         if (!(ok = warp_wait(&bars.dp_full, e & 1, stop, p.error))) break;
         fence_after();
-        {
+        auto grads = [&](auto mask) {
           uint32_t z[kHalf], pk[16];
 #pragma unroll
           for (int y = 0; y < 4; ++y) tmem_ld16(t_d + y * 16, z + y * 16);
@@ -576,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
               // delta - dP: minus dS; the sign goes at the end
               float2 f = fma2(make_float2(__uint_as_float(zz[2 * u]), __uint_as_float(zz[2 * u + 1])), minus_1, delta2);
               f = mul2(f, pr[y * 8 + u]);
-              if (masked) {
+              if (mask) {
                 if (!(seen[col >> 5] >> (col & 31) & 1)) f.x = 0.f;
                 if (!(seen[col >> 5] >> (col & 31) & 2)) f.y = 0.f;
               }
@@ -584,7 +683,8 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
             }
             if (y & 1) tmem_st16(t_d + (y >> 1) * 16, pk);
           }
-        }
+        };
+        if (masked) grads(std::true_type{}); else grads(std::false_type{});
         wait_st();
         fence_before();
         __syncwarp();
@@ -649,18 +749,35 @@ template <typename T, int DB> void launch(Params &p, cudaStream_t s) {
     MSX_CHECK_LAUNCH();
   }
   if (w.c.dk) {
-    auto kernel = dkv_tc_kernel<T, DB>;
-    // The tiles of the first keys come first: sinks are seen by all that follow,
-    // so theirs are the longest.
-    const int64_t grid = ceil_div(w.c.k_len, kT) * w.c.batch * w.c.k_heads;
-    if (grid > INT32_MAX) fail(MSX_ERR_OVERFLOW, "window_attention has too many key tiles for one call.");
-    MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKvSmem<DB>));
-    kernel<<<(unsigned)grid, kThreads, kKvSmem<DB>, s>>>(p);
-    MSX_CHECK_LAUNCH();
+    auto run = [&](auto kernel, int64_t grid) {
+      grid *= w.c.batch * w.c.k_heads;
+      if (grid > INT32_MAX) fail(MSX_ERR_OVERFLOW, "window_attention has too many key tiles for one call.");
+      MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKvSmem<DB>));
+      kernel<<<(unsigned)grid, kThreads, kKvSmem<DB>, s>>>(p);
+      MSX_CHECK_LAUNCH();
+    };
+    if (p.chunk) run(dkv_tc_kernel<T, DB, true>, (int64_t)p.n_chunks * far_key_tiles(w));
+    run(dkv_tc_kernel<T, DB, false>, ceil_div(w.c.k_len, kT));
   }
 }
 
+// Queries of a chunk, a multiple of the tile: about 256 chunks over all sequences
+// and key heads, of two tiles at least. 0 where one chunk would hold all queries,
+// where no query lies outside the window, or with more sinks than a tile of keys
+// (then their tiles are several, and the products over them no longer mostly idle).
+int pick_chunk(const WindowProblem &w) {
+  if (w.sinks == 0 || w.sinks > kT || w.window >= w.c.k_len) return 0;
+  const int64_t tiles = ceil_div(w.c.q_len, kT);
+  const int64_t n = std::max<int64_t>(2, ceil_div(tiles * w.c.batch * w.c.k_heads, 256));
+  return n >= tiles ? 0 : (int)n * kT;
+}
+
 }  // namespace
+
+int64_t window_backward_floats_tc(const WindowProblem &w) {
+  const int chunk = pick_chunk(w);
+  return chunk ? w.c.batch * w.c.k_heads * ceil_div(w.c.q_len, chunk) * w.sinks * 2 * w.c.dim : 0;
+}
 
 void window_backward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s) {
   if (w.c.batch == 0) return;
@@ -680,6 +797,9 @@ void window_backward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s)
   if (items > INT32_MAX / 2) fail(MSX_ERR_OVERFLOW, "window_attention has too many queries and heads for one call.");
   p.items = (int)items;
   p.error = window_error_flag();
+  p.chunk = pick_chunk(w);
+  p.n_chunks = p.chunk ? (int)ceil_div(w.c.q_len, p.chunk) : 0;
+  p.far = w.c.delta + w.c.batch * heads * w.lse_row;
   if (bf16) {
     if (dim <= 64) launch<__nv_bfloat16, 1>(p, s); else launch<__nv_bfloat16, 2>(p, s);
   } else {

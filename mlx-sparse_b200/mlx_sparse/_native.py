@@ -93,6 +93,7 @@ def extension():
         window = [c_int, p, p, p, p, p, p, i64, i64, i64, i64, i64, i64, i64, i64, c_float, c_int, p, i64]
         L.msx_window_attention_forward.argtypes = window + [p, p, p]
         L.msx_window_attention_backward.argtypes = window + [p, p, p, p, p, p, p, p]
+        L.msx_window_attention_workspace.argtypes = [i64] * 8 + [ctypes.POINTER(i64)]
         L.msx_window_attention_decode.argtypes = [c_int, p, p, p, p, p, p, i64, i64, i64, i64, i64, i64, i64, c_float,
                                                   c_int, p, p, p]
         L.msx_cg_context_create.argtypes = [c_int, p, p, p, i64, i64, i64, c_int, c_int, c_int, c_int, p, c_int, p,
@@ -676,12 +677,15 @@ def window_attention_backward(q, k, v, out, lse, grad, window, sinks, scale, ind
     q, k, v = heads_of(q), heads_of(k), heads_of(v)
     indptr = None if indptr is None else indptr.contiguous()
     grad = heads_of(grad.contiguous())
-    delta = torch.empty_like(lse)
+    floats = ctypes.c_int64()
+    check(L.msx_window_attention_workspace(*q.shape[:2], k.shape[1], q.shape[2], k.shape[2], q.shape[3], window, sinks,
+                                           ctypes.byref(floats)))
+    work = lse.new_empty(floats.value)
     dq = q.new_empty(q.shape) if want_q else None
     dk, dv = (k.new_empty(k.shape), k.new_empty(k.shape)) if want_kv else (None, None)
     args, _keep = _window_args(q, k, v, window, sinks, scale, indptr)
     with _on(dev):
-        check(L.msx_window_attention_backward(*args, out.data_ptr(), lse.data_ptr(), grad.data_ptr(), delta.data_ptr(),
+        check(L.msx_window_attention_backward(*args, out.data_ptr(), lse.data_ptr(), grad.data_ptr(), work.data_ptr(),
                                               _p(dq), _p(dk), _p(dv), _stream(dev)))
     return dq, dk, dv
 
