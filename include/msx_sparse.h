@@ -498,8 +498,8 @@ MSX_API int msx_csr_distill_forward_backward(
  * q_len = k_len) sequences lie one after another along the tokens; tokens
  * outside all of them see nothing and get zeros.
  * out, grad_out, dq are contiguous like q; dk, dv like k. lse: float (batch,
- * q_heads, q_len rounded up to a multiple of 128), 16-byte aligned, written by
- * forward (null: not wanted), read by backward;
+ * q_heads, q_len rounded up to a multiple of 128), 16-byte aligned, minus
+ * the log-sum-exp in base 2, written by forward (null: not wanted), read by backward;
  * workspace: *floats of msx_window_attention_workspace, 16-byte aligned, for
  * backward alone. backward reads forward's out. */
 MSX_API int msx_window_attention_workspace(int64_t batch, int64_t q_len,

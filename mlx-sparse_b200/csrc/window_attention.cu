@@ -106,13 +106,13 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) forward_ker
       if (d < dim)
         out[((b * w.c.q_len + i) * w.c.q_heads + h) * dim + d] = VT<T>::store(empty ? 0.f : acc[r][x] * inv);
     }
-    // an empty row's +inf makes its probabilities 0 in the backward pass
+    // an empty row's -inf makes its probabilities 0 in the backward pass
     if (w.c.lse && lane == 0)
-      w.c.lse[((int64_t)b * w.c.q_heads + h) * w.lse_row + i] = empty ? INFINITY : m[r] + log2f(l[r]);
+      w.c.lse[((int64_t)b * w.c.q_heads + h) * w.lse_row + i] = empty ? -INFINITY : -(m[r] + log2f(l[r]));
   }
 }
 
-// delta_i = dO_i . O_i, 16 lanes for each row and head, VEC elements at a time.
+// -delta_i = -dO_i . O_i, 16 lanes for each row and head, VEC elements at a time.
 // O is the rounded output: the error that brings (half a step of O's type, times
 // dO) is of the size of the rounding of the gradients themselves.
 template <typename T, int VEC> __global__ void delta_kernel(const WindowProblem w) {
@@ -137,7 +137,7 @@ template <typename T, int VEC> __global__ void delta_kernel(const WindowProblem 
 #pragma unroll
   for (int d = 8; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
   const int64_t h = x % w.c.q_heads, bi = x / w.c.q_heads, b = bi / w.c.q_len, i = bi % w.c.q_len;
-  if (inside && lane == 0) w.c.delta[(b * w.c.q_heads + h) * w.lse_row + i] = s;
+  if (inside && lane == 0) w.c.delta[(b * w.c.q_heads + h) * w.lse_row + i] = -s;
 }
 
 template <typename T> __global__ void __launch_bounds__(kWarps * 32) dq_kernel(const WindowProblem w) {
@@ -161,7 +161,7 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) dq_kernel(c
     const int i = i0 + warp * kRowsPerWarp + r;
     span[r] = query_span(w, b, i);
     const int64_t at = ((int64_t)b * w.c.q_heads + h) * w.lse_row + i;
-    lse[r] = i < w.c.q_len ? w.c.lse[at] : INFINITY;
+    lse[r] = i < w.c.q_len ? w.c.lse[at] : -INFINITY;
     delta[r] = i < w.c.q_len ? w.c.delta[at] : 0.f;
 #pragma unroll
     for (int x = 0; x < kRegs; ++x) acc[r][x] = 0.f;
@@ -181,7 +181,7 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) dq_kernel(c
       if (seen) {
         const int row = warp * kRowsPerWarp + r;
         const float s = dot(sq + row * dim, sk + lane * ks, dim) * (w.c.scale * kLog2e);
-        ds = exp2f(s - lse[r]) * (dot(sg + row * dim, sv + lane * ks, dim) - delta[r]);
+        ds = exp2f(s + lse[r]) * (dot(sg + row * dim, sv + lane * ks, dim) + delta[r]);
       }
       for (unsigned left = who; left; left &= left - 1) {
         const int kk = __ffs(left) - 1;
@@ -235,7 +235,7 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) dkv_kernel(
       load_rows(sg, ks, g, (int64_t)w.c.q_heads * dim, i0, (int)w.c.q_len, kTile, dim);
       __syncthreads();
       const int i = i0 + lane, p = i + w.offset;
-      const float lse = i < w.c.q_len ? w.c.lse[at + i] : INFINITY, delta = i < w.c.q_len ? w.c.delta[at + i] : 0.f;
+      const float lse = i < w.c.q_len ? w.c.lse[at + i] : -INFINITY, delta = i < w.c.q_len ? w.c.delta[at + i] : 0.f;
 #pragma unroll
       for (int r = 0; r < kRowsPerWarp; ++r) {
         const int row = warp * kRowsPerWarp + r;
@@ -244,8 +244,8 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) dkv_kernel(
         if (!who) continue;
         float pr = 0.f, ds = 0.f;
         if (seen) {
-          pr = exp2f(dot(sk + row * dim, sq + lane * ks, dim) * (w.c.scale * kLog2e) - lse);
-          ds = pr * (dot(sv + row * dim, sg + lane * ks, dim) - delta);
+          pr = exp2f(dot(sk + row * dim, sq + lane * ks, dim) * (w.c.scale * kLog2e) + lse);
+          ds = pr * (dot(sv + row * dim, sg + lane * ks, dim) + delta);
         }
         for (unsigned left = who; left; left &= left - 1) {
           const int ii = __ffs(left) - 1;

@@ -19,7 +19,7 @@ struct WindowProblem {
   int offset;   // position of query 0
   int wide_ptr; // indptr or lengths are int64
   int window, sinks;  // clamped to k_len
-  int64_t lse_row;    // floats of lse (delta) for each head: q_len rounded up to whole tiles
+  int64_t lse_row;    // floats of lse (delta) for each head: q_len rounded up to whole tiles; both negated
 };
 
 // Sequence of a position: [start, end), empty (start = end) outside all.

@@ -95,8 +95,8 @@ template <typename T> struct PairDots {
       s = fmaf(VT<T>::load(q[d]), VT<T>::load(k[d]), s);
       dp = fmaf(VT<T>::load(g[d]), VT<T>::load(v[d]), dp);
     }
-    p = exp2f(s * (w.c.scale * kLog2e) - lse);
-    ds = p * (dp - delta);
+    p = exp2f(s * (w.c.scale * kLog2e) + lse);
+    ds = p * (dp + delta);
   }
 };
 
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
     const int half = (warp - 4) >> 2;
     const uint32_t at = ((uint32_t)(warp & 3) << 21) + half * 64;
     const float c = w.c.scale * kLog2e;
-    const float2 minus_c = make_float2(-c, -c), minus_1 = make_float2(-1.f, -1.f);
+    const float2 c2 = make_float2(c, c);
     // the queries that all 32 keys of this warp are seen by
     const int all_first = __reduce_max_sync(~0u, first_i), all_last = __reduce_min_sync(~0u, last_i);
     bool ok = true;
@@ -343,12 +343,14 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const uint32_t *zz = z + x * 16;
+          float4 stat;
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
             const int col = x * 16 + 2 * y;
-            float2 e = fma2(make_float2(__uint_as_float(zz[2 * y]), __uint_as_float(zz[2 * y + 1])), minus_c,
-                            *reinterpret_cast<const float2 *>(lse + col));
-            e.x = exp2_fast(-e.x), e.y = exp2_fast(-e.y);
+            if (!(y & 1)) stat = *reinterpret_cast<const float4 *>(lse + col);
+            float2 e = fma2(make_float2(__uint_as_float(zz[2 * y]), __uint_as_float(zz[2 * y + 1])), c2,
+                            y & 1 ? make_float2(stat.z, stat.w) : make_float2(stat.x, stat.y));
+            e.x = exp2_fast(e.x), e.y = exp2_fast(e.y);
             if (mask) {
               if (!(seen[col >> 5] >> (col & 31) & 1)) e.x = 0.f;
               if (!(seen[col >> 5] >> (col & 31) & 2)) e.y = 0.f;
@@ -375,12 +377,13 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const uint32_t *zz = z + x * 16;
+          float4 stat;
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
             const int col = x * 16 + 2 * y;
-            // delta - dP: minus dS comes out, and dK takes the sign back at the end
-            float2 e = fma2(make_float2(__uint_as_float(zz[2 * y]), __uint_as_float(zz[2 * y + 1])), minus_1,
-                            *reinterpret_cast<const float2 *>(delta + col));
+            if (!(y & 1)) stat = *reinterpret_cast<const float4 *>(delta + col);
+            float2 e = add2(make_float2(__uint_as_float(zz[2 * y]), __uint_as_float(zz[2 * y + 1])),
+                            y & 1 ? make_float2(stat.z, stat.w) : make_float2(stat.x, stat.y));
             e = mul2(e, pr[x * 8 + y]);
             if (mask) {
               if (!(seen[col >> 5] >> (col & 31) & 1)) e.x = 0.f;
@@ -403,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       // the first warpgroup writes dV, the second dK
       const bool inside = key < w.c.k_len;
       const uint32_t from = (half ? t_dk : t_dv) + ((uint32_t)(warp & 3) << 21);
-      const float scale = half ? -w.c.scale : 1.f;
+      const float scale = half ? w.c.scale : 1.f;
       int start = 0, end = 0, c0 = 0, c1 = 0;  // the chunks that have sums for this key
       if (p.chunk && inside) {
         sequence_of(w, key, start, end);
@@ -605,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
     const int half = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const float c = w.c.scale * kLog2e;
-    const float2 minus_c = make_float2(-c, -c), minus_1 = make_float2(-1.f, -1.f);
+    const float2 c2 = make_float2(c, c);
     uint32_t done = 0;
     uint32_t dq_phase = 0;
     bool ok = true;
@@ -619,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
       const int all_low = __reduce_max_sync(~0u, span.p < 0 ? INT_MAX : span.low);
       const int all_end = __reduce_min_sync(~0u, span.p < 0 ? -1 : span.p) + 1;
       const int64_t stat = ((int64_t)b * w.c.q_heads + h) * w.lse_row + i;
-      const float lse = inside ? w.c.lse[stat] : INFINITY, delta = inside ? w.c.delta[stat] : 0.f;
+      const float lse = inside ? w.c.lse[stat] : -INFINITY, delta = inside ? w.c.delta[stat] : 0.f;
       const float2 lse2 = make_float2(lse, lse), delta2 = make_float2(delta, delta);
       for (int t = 0; t < tiles.n; ++t) {
         const uint32_t e = done + t;
@@ -647,8 +650,8 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
               const int col = y * 16 + 2 * u;
-              float2 f = fma2(make_float2(__uint_as_float(zz[2 * u]), __uint_as_float(zz[2 * u + 1])), minus_c, lse2);
-              f.x = exp2_fast(-f.x), f.y = exp2_fast(-f.y);
+              float2 f = fma2(make_float2(__uint_as_float(zz[2 * u]), __uint_as_float(zz[2 * u + 1])), c2, lse2);
+              f.x = exp2_fast(f.x), f.y = exp2_fast(f.y);
               if (mask) {
                 if (!(seen[col >> 5] >> (col & 31) & 1)) f.x = 0.f;
                 if (!(seen[col >> 5] >> (col & 31) & 2)) f.y = 0.f;
@@ -672,8 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
               const int col = y * 16 + 2 * u;
-              // delta - dP: minus dS; the sign goes at the end
-              float2 f = fma2(make_float2(__uint_as_float(zz[2 * u]), __uint_as_float(zz[2 * u + 1])), minus_1, delta2);
+              float2 f = add2(make_float2(__uint_as_float(zz[2 * u]), __uint_as_float(zz[2 * u + 1])), delta2);
               f = mul2(f, pr[y * 8 + u]);
               if (mask) {
                 if (!(seen[col >> 5] >> (col & 31) & 1)) f.x = 0.f;
@@ -711,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
 #pragma unroll
           for (int y = 0; y < 32; ++y) o[y] = 0;
         }
-        bad = store32<T>(dq, (int64_t)w.c.q_heads * w.c.dim, o, -w.c.scale, d, w.c.dim, (int)w.c.q_len - (i - lane)) || bad;
+        bad = store32<T>(dq, (int64_t)w.c.q_heads * w.c.dim, o, w.c.scale, d, w.c.dim, (int)w.c.q_len - (i - lane)) || bad;
       }
       if (__any_sync(~0u, bad && inside)) {
         bool hidden = false;

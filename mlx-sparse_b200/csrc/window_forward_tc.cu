@@ -148,7 +148,7 @@ __device__ __noinline__ void repair_row(const WindowProblem &w, int b, int h, in
 #pragma unroll
   for (int x = 0; x < 4; ++x)
     if (x * 32 + lane < dim) out[x * 32 + lane] = VT<T>::store(acc[x] / l);
-  if (w.c.lse && lane == 0) w.c.lse[((int64_t)b * w.c.q_heads + h) * w.lse_row + i] = m + log2f(l);
+  if (w.c.lse && lane == 0) w.c.lse[((int64_t)b * w.c.q_heads + h) * w.lse_row + i] = -(m + log2f(l));
 }
 
 template <typename T, int DB>
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         bad = store32<T>(out, (int64_t)w.c.q_heads * w.c.dim, o, inv, x, w.c.dim, (int)w.c.q_len - (i - lane)) || bad;
       }
       if (inside && w.c.lse)
-        w.c.lse[((int64_t)it.b * w.c.q_heads + h) * w.lse_row + i] = empty ? INFINITY : m * c + log2f(l);
+        w.c.lse[((int64_t)it.b * w.c.q_heads + h) * w.lse_row + i] = empty ? -INFINITY : -(m * c + log2f(l));
       if (__any_sync(~0u, bad && inside)) {
         // What the row sees may be at fault; recompute it only if something not
         // finite hides among the tiles' other keys.
