@@ -21,8 +21,8 @@
 // sums of dQ would make 5; atomics would change results from run to run.
 //
 // As in the forward pass one warp loads tiles by TMA, one thread issues
-// tcgen05.mma, and two warpgroups do the arithmetic in between, straight from
-// tensor memory, 64 columns of every row each. P and dS, rounded to the inputs'
+// tcgen05.mma, and some warpgroups do the arithmetic in between, straight from
+// tensor memory, 32 or 64 columns of every row each. P and dS, rounded to the inputs'
 // type for the second products (half a step each; the sums are fp32), take the
 // place of the scores they came from. The products of one tile pair are issued
 // between those of its neighbours, so that the tensor cores work while the
@@ -45,7 +45,11 @@ using namespace tc;
 namespace {
 
 constexpr int kT = 128;        // rows and columns of a tile pair
-constexpr int kThreads = 384;  // loads, products, one warp for tensor memory, one idle; 8 warps of arithmetic
+// Columns of a tile for each warpgroup of arithmetic. dQ of head sizes over 64 is
+// 4% faster with fewer, busier warps, everything else up to 8% slower.
+constexpr int kKvCols = 32;
+template <int DB> constexpr int kQCols = DB == 2 ? 64 : 32;
+constexpr int threads_for(int cols) { return 64 + kT / cols * 128; }  // loads, products, arithmetic
 constexpr int kStages = 4;
 
 struct Params {
@@ -130,9 +134,9 @@ __device__ __noinline__ void repair_dq(const WindowProblem &w, int b, int h, int
   }
 }
 
-// One row of dK (keys) or dV again.
+// One row of dK (keys) or dV again, columns [d0, d1).
 template <typename T>
-__device__ __noinline__ void repair_dkv(const WindowProblem &w, int b, int hk, int j, bool keys) {
+__device__ __noinline__ void repair_dkv(const WindowProblem &w, int b, int hk, int j, bool keys, int d0, int d1) {
   const int lane = threadIdx.x & 31, shift = key_count(w, b) - (int)w.c.q_len;
   const int i0 = max(0, j - shift), i1 = min((int)w.c.q_len, last_query(w, j) - shift + 1);
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -154,8 +158,10 @@ __device__ __noinline__ void repair_dkv(const WindowProblem &w, int b, int hk, i
   }
   T *out = static_cast<T *>(keys ? w.c.dk : w.c.dv) + ((b * w.c.k_len + j) * w.c.k_heads + hk) * w.c.dim;
 #pragma unroll
-  for (int y = 0; y < 4; ++y)
-    if (y * 32 + lane < w.c.dim) out[y * 32 + lane] = VT<T>::store(acc[y] * (keys ? w.c.scale : 1.f));
+  for (int y = 0; y < 4; ++y) {
+    const int d = y * 32 + lane;
+    if (d >= d0 && d < d1 && d < w.c.dim) out[d] = VT<T>::store(acc[y] * (keys ? w.c.scale : 1.f));
+  }
 }
 
 __device__ __forceinline__ void drain(uint64_t *bars, int n) {
@@ -178,9 +184,9 @@ template <int DB> constexpr int kKvSmem = 1024 + (2 + kStages) * DB * kBox + 2 *
 
 // FAR: the sinks of one sequence against one chunk of queries.
 template <typename T, int DB, bool FAR>
-__global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(threads_for(kKvCols), 1) dkv_tc_kernel(const __grid_constant__ Params p) {
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr int kTile = DB * kBox;
+  constexpr int kTile = DB * kBox, kCols = kKvCols;
   extern __shared__ unsigned char raw[];
   unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   __shared__ KvBars bars;
@@ -210,14 +216,14 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
     bar_init(&bars.kv_full, 1);
     for (int s = 0; s < kStages; ++s) bar_init(&bars.full[s], 1), bar_init(&bars.empty[s], 1);
     bar_init(&bars.s_full, 1), bar_init(&bars.dp_full, 1), bar_init(&bars.done, 1);
-    bar_init(&bars.p_full, 8), bar_init(&bars.ds_full, 8);
+    bar_init(&bars.p_full, 4 * kT / kCols), bar_init(&bars.ds_full, 4 * kT / kCols);
     bars.stop = 0, bars.last = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
   // the tiles of queries that see any of these keys
   const int key = j0 + (warp & 3) * 32 + lane;
-  if (warp >= 4 && warp < 8) {
+  if (warp >= 2 && warp < 6) {
     const int top = __reduce_max_sync(~0u, last_near_query(p, key));
     if (lane == 0) atomicMax(&bars.last, top);
   }
@@ -234,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
     first_i = sink ? from : INT_MAX, last_i = sink ? to - 1 : -1;
   }
   const int n = n_tiles * w.group;
-  if (warp == 2) tmem_alloc(&bars.tmem, 512);
+  if (warp == 1) tmem_alloc(&bars.tmem, 512);
   fence_before();
   __syncthreads();
   fence_after();
@@ -277,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
     }
   } else if (warp == 1) {
     if (n > 0) {
-      const Products<DB> mm(BF16, w.c.dim);
+      const Products<DB, kCols> mm(BF16, w.c.dim);
       const uint32_t ka = smem_addr(k_tile), va = smem_addr(v_tile), ra = smem_addr(ring);
       bool ok = warp_wait(&bars.kv_full, 0, stop, p.error);
       auto ready = [&](int e) { return ok = ok && warp_wait(&bars.full[e % kStages], e / kStages & 1, stop, p.error); };
@@ -314,9 +320,9 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       }
       mma_commit(mm.leader, &bars.done);
     }
-  } else if (warp >= 4) {
-    const int half = (warp - 4) >> 2;
-    const uint32_t at = ((uint32_t)(warp & 3) << 21) + half * 64;
+  } else {
+    const int part = (warp - 2) >> 2;
+    const uint32_t at = ((uint32_t)(warp & 3) << 21) + part * kCols;
     const float c = w.c.scale * kLog2e;
     const float2 c2 = make_float2(c, c);
     // the queries that all 32 keys of this warp are seen by
@@ -324,24 +330,23 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
     bool ok = true;
     Walk at_pair = first_pair;
     for (int it = 0; ok && it < n; ++it, at_pair.next()) {
-      const int i0 = at_pair.t * kT + half * 64;
-      const float *lse = row_stats + (it & 1) * 2 * kT + half * 64, *delta = lse + kT;
-      const bool masked = !(i0 >= all_first && i0 + 63 <= all_last);
-      const uint32_t seen[2] = {first_i > last_i ? 0 : bits(first_i - i0, last_i + 1 - i0, 0),
-                                first_i > last_i ? 0 : bits(first_i - i0, last_i + 1 - i0, 32)};
+      const int i0 = at_pair.t * kT + part * kCols;
+      const float *lse = row_stats + (it & 1) * 2 * kT + part * kCols, *delta = lse + kT;
+      const bool masked = !(i0 >= all_first && i0 + kCols - 1 <= all_last);
+      const uint32_t seen = first_i > last_i ? 0 : bits(first_i - i0, last_i + 1 - i0, 0);
       // lse and delta came with Q's tile, which the products of s_full have read
       if (!(ok = warp_wait(&bars.full[2 * it % kStages], 2 * it / kStages & 1, stop, p.error))) break;
       if (!(ok = warp_wait(&bars.s_full, it & 1, stop, p.error))) break;
       fence_after();
-      float2 pr[32];
+      float2 pr[kCols / 2];
       auto weights = [&](auto mask) {
-        uint32_t z[kHalf], pk[16];
+        uint32_t z[kCols], pk[kCols / 2];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) tmem_ld16(t_s + at + x * 16, z + x * 16);
+        for (int x = 0; x < 2; ++x) tmem_ld16(t_s + at + x * 16, z + x * 16);
         wait_ld();
-        tie32(z), tie32(z + 32);
+        tie32(z);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < 2; ++x) {
           const uint32_t *zz = z + x * 16;
           float4 stat;
 #pragma unroll
@@ -352,14 +357,14 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
                             y & 1 ? make_float2(stat.z, stat.w) : make_float2(stat.x, stat.y));
             e.x = exp2_fast(e.x), e.y = exp2_fast(e.y);
             if (mask) {
-              if (!(seen[col >> 5] >> (col & 31) & 1)) e.x = 0.f;
-              if (!(seen[col >> 5] >> (col & 31) & 2)) e.y = 0.f;
+              if (!(seen >> col & 1)) e.x = 0.f;
+              if (!(seen >> col & 2)) e.y = 0.f;
             }
             pr[x * 8 + y] = e;
-            pk[(x & 1) * 8 + y] = pack2<BF16>(e.x, e.y);
+            pk[x * 8 + y] = pack2<BF16>(e.x, e.y);
           }
-          if (x & 1) tmem_st16(t_s + at + (x >> 1) * 16, pk);
         }
+        tmem_st16(t_s + at, pk);
       };
       if (masked) weights(std::true_type{}); else weights(std::false_type{});
       wait_st();
@@ -369,13 +374,13 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       if (!(ok = warp_wait(&bars.dp_full, it & 1, stop, p.error))) break;
       fence_after();
       auto grads = [&](auto mask) {
-        uint32_t z[kHalf], pk[16];
+        uint32_t z[kCols], pk[kCols / 2];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) tmem_ld16(t_dp + at + x * 16, z + x * 16);
+        for (int x = 0; x < 2; ++x) tmem_ld16(t_dp + at + x * 16, z + x * 16);
         wait_ld();
-        tie32(z), tie32(z + 32);
+        tie32(z);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < 2; ++x) {
           const uint32_t *zz = z + x * 16;
           float4 stat;
 #pragma unroll
@@ -386,13 +391,13 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
                             y & 1 ? make_float2(stat.z, stat.w) : make_float2(stat.x, stat.y));
             e = mul2(e, pr[x * 8 + y]);
             if (mask) {
-              if (!(seen[col >> 5] >> (col & 31) & 1)) e.x = 0.f;
-              if (!(seen[col >> 5] >> (col & 31) & 2)) e.y = 0.f;
+              if (!(seen >> col & 1)) e.x = 0.f;
+              if (!(seen >> col & 2)) e.y = 0.f;
             }
-            pk[(x & 1) * 8 + y] = pack2<BF16>(e.x, e.y);
+            pk[x * 8 + y] = pack2<BF16>(e.x, e.y);
           }
-          if (x & 1) tmem_st16(t_dp + at + (x >> 1) * 16, pk);
         }
+        tmem_st16(t_dp + at, pk);
       };
       if (masked) grads(std::true_type{}); else grads(std::false_type{});
       wait_st();
@@ -403,7 +408,8 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
     if (ok && n > 0) ok = warp_wait(&bars.done, 0, stop, p.error);
     if (ok) {
       fence_after();
-      // the first warpgroup writes dV, the second dK
+      // the first two warpgroups write dV, the others dK, half of the columns each
+      const int half = part >> 1, d0 = (part & 1) * DB * 32;
       const bool inside = key < w.c.k_len;
       const uint32_t from = (half ? t_dk : t_dv) + ((uint32_t)(warp & 3) << 21);
       const float scale = half ? w.c.scale : 1.f;
@@ -421,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       T *out = static_cast<T *>(half ? w.c.dk : w.c.dv) + ((b * w.c.k_len + key - lane) * w.c.k_heads + hk) * w.c.dim;
       bool bad = false;
 #pragma unroll 1
-      for (int d = 0; d < DB * 64; d += 32) {
+      for (int d = d0; d < d0 + DB * 32; d += 32) {
         uint32_t o[32];
         if (n > 0) {
           tmem_ld16(from + d, o), tmem_ld16(from + d + 16, o + 16);
@@ -476,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
             look_at(h, (most - 1) / kT * kT, 0, stop_i > 0 ? stop_i - 1 : INT_MAX);
         if (stop_i > 0 && stop_i < most) hidden = true;
         for (unsigned left = __ballot_sync(~0u, bad && inside && hidden); left; left &= left - 1)
-          repair_dkv<T>(w, b, hk, key - lane + __ffs(left) - 1, half != 0);
+          repair_dkv<T>(w, b, hk, key - lane + __ffs(left) - 1, half != 0, d0, d0 + DB * 32);
       }
     }
   }
@@ -485,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
   fence_after();
   if (threadIdx.x == 0 && *stop) drain(bars.full, kStages);
   __syncthreads();
-  if (warp == 2) tmem_free(tmem, 512);
+  if (warp == 1) tmem_free(tmem, 512);
 }
 
 // ---- dQ ---------------------------------------------------------------------------
@@ -498,9 +504,9 @@ struct QBars {
 template <int DB> constexpr int kQSmem = 1024 + (2 + kStages) * DB * kBox;
 
 template <typename T, int DB>
-__global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(threads_for(kQCols<DB>), 1) dq_tc_kernel(const __grid_constant__ Params p) {
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr int kTile = DB * kBox;
+  constexpr int kTile = DB * kBox, kCols = kQCols<DB>;
   extern __shared__ unsigned char raw[];
   unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   __shared__ QBars bars;
@@ -512,11 +518,11 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
     bar_init(&bars.q_full, 1), bar_init(&bars.q_empty, 1);
     for (int s = 0; s < kStages; ++s) bar_init(&bars.full[s], 1), bar_init(&bars.empty[s], 1);
     bar_init(&bars.s_full[0], 1), bar_init(&bars.s_full[1], 1);
-    bar_init(&bars.dp_full, 1), bar_init(&bars.ds_full, 8), bar_init(&bars.dq_full, 1);
+    bar_init(&bars.dp_full, 1), bar_init(&bars.ds_full, 4 * kT / kCols), bar_init(&bars.dq_full, 1);
     bars.stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 2) tmem_alloc(&bars.tmem, 512);
+  if (warp == 1) tmem_alloc(&bars.tmem, 512);
   fence_before();
   __syncthreads();
   fence_after();
@@ -558,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
     }
   } else if (warp == 1) {
     {
-      const Products<DB> mm(BF16, w.c.dim);
+      const Products<DB, kCols> mm(BF16, w.c.dim);
       const uint32_t qa = smem_addr(q_tile), ga = smem_addr(g_tile), ra = smem_addr(ring);
       uint32_t done = 0;  // tile pairs of earlier items: K of pair t is ring entry 2 (done + t), V the next
       uint32_t q_phase = 0;
@@ -604,8 +610,8 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
         done += tiles.n;
       }
     }
-  } else if (warp >= 4) {
-    const int half = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+  } else {
+    const int part = (warp - 2) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const float c = w.c.scale * kLog2e;
     const float2 c2 = make_float2(c, c);
@@ -626,26 +632,29 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
       const float2 lse2 = make_float2(lse, lse), delta2 = make_float2(delta, delta);
       for (int t = 0; t < tiles.n; ++t) {
         const uint32_t e = done + t;
-        const int j0 = tiles.first(t) + half * 64, j1 = tiles.end(t);
-        const bool masked = !(j0 >= all_low && j0 + 64 <= all_end && j1 - j0 >= 64);
-        uint32_t seen[2];
+        const int j0 = tiles.first(t) + part * kCols, j1 = tiles.end(t);
+        const bool masked = !(j0 >= all_low && j0 + kCols <= all_end && j1 - j0 >= kCols);
+        uint32_t seen[kCols / 32];
         {
           const int b0 = span.low - j0, b1 = min(span.p + 1, j1) - j0, s0 = span.start - j0,
                     s1 = min(span.sink_end, j1) - j0;
-          seen[0] = bits(b0, b1, 0) | bits(s0, s1, 0), seen[1] = bits(b0, b1, 32) | bits(s0, s1, 32);
+          
+#pragma unroll
+          for (int y = 0; y < kCols / 32; ++y) seen[y] = bits(b0, b1, y * 32) | bits(s0, s1, y * 32);
         }
         if (!(ok = warp_wait(&bars.s_full[e & 1], e >> 1 & 1, stop, p.error))) break;
         fence_after();
-        const uint32_t t_s = tmem + (e & 1) * 128 + lanes + half * 64, t_d = t_dp + lanes + half * 64;
-        float2 pr[32];
+        const uint32_t t_s = tmem + (e & 1) * 128 + lanes + part * kCols, t_d = t_dp + lanes + part * kCols;
+        float2 pr[kCols / 2];
         auto weights = [&](auto mask) {
-          uint32_t z[kHalf];
+          uint32_t z[kCols];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) tmem_ld16(t_s + y * 16, z + y * 16);
+          for (int y = 0; y < kCols; y += 16) tmem_ld16(t_s + y, z + y);
           wait_ld();
-          tie32(z), tie32(z + 32);
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
+          for (int y = 0; y < kCols; y += 32) tie32(z + y);
+#pragma unroll
+          for (int y = 0; y < kCols / 16; ++y) {
             const uint32_t *zz = z + y * 16;
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
@@ -664,13 +673,14 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
         if (!(ok = warp_wait(&bars.dp_full, e & 1, stop, p.error))) break;
         fence_after();
         auto grads = [&](auto mask) {
-          uint32_t z[kHalf], pk[16];
+          uint32_t z[kCols], pk[kCols / 2];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) tmem_ld16(t_d + y * 16, z + y * 16);
+          for (int y = 0; y < kCols; y += 16) tmem_ld16(t_d + y, z + y);
           wait_ld();
-          tie32(z), tie32(z + 32);
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
+          for (int y = 0; y < kCols; y += 32) tie32(z + y);
+#pragma unroll
+          for (int y = 0; y < kCols / 16; ++y) {
             const uint32_t *zz = z + y * 16;
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
@@ -681,10 +691,11 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
                 if (!(seen[col >> 5] >> (col & 31) & 1)) f.x = 0.f;
                 if (!(seen[col >> 5] >> (col & 31) & 2)) f.y = 0.f;
               }
-              pk[(y & 1) * 8 + u] = pack2<BF16>(f.x, f.y);
+              pk[y * 8 + u] = pack2<BF16>(f.x, f.y);
             }
-            if (y & 1) tmem_st16(t_d + (y >> 1) * 16, pk);
           }
+#pragma unroll
+          for (int y = 0; y < kCols / 2; y += 16) tmem_st16(t_d + y, pk + y);
         };
         if (masked) grads(std::true_type{}); else grads(std::false_type{});
         wait_st();
@@ -700,10 +711,12 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
         fence_after();
       }
       T *dq = static_cast<T *>(w.c.dq) + ((b * w.c.q_len + i - lane) * w.c.q_heads + h) * w.c.dim;
-      const int d0 = half * DB * 32;
+      // this warpgroup's columns of dQ; of four only two have some at head sizes up to 64
+      constexpr int kOut = DB == 2 ? DB * 64 * kCols / kT : 32;
+      const int d0 = part * kOut;
       bool bad = false;
 #pragma unroll 1
-      for (int d = d0; d < d0 + DB * 32; d += 32) {
+      for (int d = d0; d < d0 + kOut && d < DB * 64; d += 32) {
         uint32_t o[32];
         if (tiles.n > 0) {
           tmem_ld32(t_dq + lanes + d, o);
@@ -730,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
           }
         }
         for (unsigned left = __ballot_sync(~0u, bad && inside && hidden); left; left &= left - 1)
-          repair_dq<T>(w, b, h, i - lane + __ffs(left) - 1, d0, d0 + DB * 32);
+          repair_dq<T>(w, b, h, i - lane + __ffs(left) - 1, d0, d0 + kOut);
       }
     }
   }
@@ -739,7 +752,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
   fence_after();
   if (threadIdx.x == 0 && *stop) drain(bars.full, kStages);
   __syncthreads();
-  if (warp == 2) tmem_free(tmem, 512);
+  if (warp == 1) tmem_free(tmem, 512);
 }
 
 template <typename T, int DB> void launch(Params &p, cudaStream_t s) {
@@ -747,7 +760,7 @@ template <typename T, int DB> void launch(Params &p, cudaStream_t s) {
   if (w.c.dq && w.c.q_len > 0) {
     auto kernel = dq_tc_kernel<T, DB>;
     MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kQSmem<DB>));
-    kernel<<<(unsigned)std::min(p.items, num_sms()), kThreads, kQSmem<DB>, s>>>(p);
+    kernel<<<(unsigned)std::min(p.items, num_sms()), threads_for(kQCols<DB>), kQSmem<DB>, s>>>(p);
     MSX_CHECK_LAUNCH();
   }
   if (w.c.dk) {
@@ -755,7 +768,7 @@ template <typename T, int DB> void launch(Params &p, cudaStream_t s) {
       grid *= w.c.batch * w.c.k_heads;
       if (grid > INT32_MAX) fail(MSX_ERR_OVERFLOW, "window_attention has too many key tiles for one call.");
       MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKvSmem<DB>));
-      kernel<<<(unsigned)grid, kThreads, kKvSmem<DB>, s>>>(p);
+      kernel<<<(unsigned)grid, threads_for(kKvCols), kKvSmem<DB>, s>>>(p);
       MSX_CHECK_LAUNCH();
     };
     if (p.chunk) run(dkv_tc_kernel<T, DB, true>, (int64_t)p.n_chunks * far_key_tiles(w));

@@ -91,11 +91,11 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi, int from) {
 // Products issued by a warp's leader, of 128 x 128 tiles of scores (64 columns
 // would take nearly as long: 465 clocks against 530); DB boxes of 64 elements cover
 // the head size. Scores: both operands K-major in shared memory. Sums: the left
-// operand in tensor memory, where each run of 64 columns of scores holds its 16-bit
-// values in its first 32; the right operand MN-major in shared memory. Unrolled: the issuing warp is on the critical path of
+// operand in tensor memory, where each run of W columns of scores holds its 16-bit
+// values in its first W / 2; the right operand MN-major in shared memory. Unrolled: the issuing warp is on the critical path of
 // every tile.
 constexpr int kHalf = 64;                // columns of scores that are handled together
-template <int DB> struct Products {
+template <int DB, int W = 64> struct Products {
   bool leader;
   int k_steps;
   uint32_t scores_desc, sums_desc;
@@ -116,7 +116,7 @@ template <int DB> struct Products {
     const uint32_t y = tc::desc_mn_major(b, kBox);
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      tc::mma_ts(leader, d, left + (k >> 2) * kHalf + (k & 3) * 8, y + (k * 2048 >> 4), sums_desc, add || k > 0);
+      tc::mma_ts(leader, d, left + k * 16 / W * W + k * 16 % W / 2, y + (k * 2048 >> 4), sums_desc, add || k > 0);
   }
 };
 
