@@ -12,10 +12,11 @@
 // the gradient is rounded once, to the logits' type.
 //
 // Bound: HBM. Forward reads the logits once, the backward pass reads them
-// again and writes the gradient; the one-pass form keeps a row's logits in
-// shared memory (spread over a cluster when one SM's is too small) between
-// the sum of the exponentials and the gradient, so it reads once and writes
-// once, two thirds of the bytes of the two passes.
+// again and writes the gradient. The one-pass form reads HBM once and writes
+// once, two thirds of the bytes of the two passes: a row's logits stay on chip
+// between the sum of the exponentials and the gradient, in shared memory where
+// they fit (spread over a cluster where there are too few rows to fill the SMs),
+// else in L2, from where the CTA that summed the row reads it again.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -36,7 +37,9 @@ struct RowStats {
   float t_max, t_inv;  // the same of the teacher's entries
 };
 
-constexpr int kMaxKept = 200 * 1024;  // shared memory of a slice, at most
+constexpr int kMaxKept = 200 * 1024;  // dynamic shared memory, at most
+constexpr int kKeepMost = 64 * 1024;  // slices up to this are kept in shared memory
+constexpr int kRereadThreads = 384;
 
 struct DistillArgs {
   const void *logits;
@@ -298,13 +301,18 @@ template <int N> __device__ __forceinline__ void cp_async_wait() {
 constexpr int kThreads = 256;
 constexpr int kGroups = 4;  // commit groups of a slice: the sums start when the first quarter is there
 
-// One cluster for each row, one slice of the row for each CTA. KEEP: the slice
-// stays in shared memory and the gradient is written from it; else the forward
-// pass alone, straight from registers.
-template <typename T, typename I, bool KEEP>
-__global__ void __launch_bounds__(kThreads) distill_row_kernel(const DistillArgs a) {
+// What a CTA does with its slice of a row after the sum: nothing (the forward
+// pass alone), or the gradient, from the slice in shared memory or from a second
+// read of it.
+enum class Grad { none, kept, reread };
+constexpr int kBackwardTable = 1024;  // columns at a time of repeated entries' sums
+
+// One cluster for each row, one slice of the row for each CTA.
+template <typename T, typename I, Grad MODE, int TH>
+__global__ void __launch_bounds__(TH, MODE == Grad::kept ? 1024 / TH : 1536 / TH) distill_row_kernel(const DistillArgs a) {
+  constexpr bool KEEP = MODE == Grad::kept;
   extern __shared__ __align__(16) unsigned char dyn[];
-  __shared__ float2 part[kThreads / 32];
+  __shared__ float2 part[TH / 32];
   __shared__ float2 ranks[16];
   constexpr int N = Vec<T>::n;
   cg::cluster_group cluster = cg::this_cluster();
@@ -314,13 +322,13 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const DistillArgs
   int64_t lo, hi;
   row_range<I>(a, row, lo, hi);
   const int64_t c0 = min(a.vocab, (int64_t)rank * a.slice), c1 = min(a.vocab, c0 + a.slice);
-  T *g = KEEP ? static_cast<T *>(a.grad) + row * a.vocab : nullptr;
+  T *g = MODE == Grad::none ? nullptr : static_cast<T *>(a.grad) + row * a.vocab;
   if (lo == hi) {  // every CTA of the cluster leaves
     if (rank == 0 && threadIdx.x == 0) {
       a.loss[row] = 0.f;
       if (a.stats) a.stats[row] = RowStats{0.f, 0.f, 0.f, 0.f};
     }
-    if (KEEP) zero_slice(g + c0, c1 - c0);
+    if (MODE != Grad::none) zero_slice(g + c0, c1 - c0);
     return;
   }
   const T *z = static_cast<const T *>(a.logits) + row * a.ld;
@@ -336,11 +344,11 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const DistillArgs
   const bool has_loose = tid < sh.head + sh.tail;
   if (has_loose) loose = VT<T>::load(z[loose_col]);
   if (KEEP) {
-    const int per = (sh.nvec + kThreads * kGroups - 1) / (kThreads * kGroups);
+    const int per = (sh.nvec + TH * kGroups - 1) / (TH * kGroups);
 #pragma unroll
     for (int q = 0; q < kGroups; ++q) {
       for (int it = q * per; it < (q + 1) * per; ++it) {
-        const int i = tid + it * kThreads;
+        const int i = tid + it * TH;
         if (i < sh.nvec) cp_async16(kept + i, src + i);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -348,7 +356,7 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const DistillArgs
     // each thread reads back only what it copied itself, so its own wait is enough
     auto take = [&](int q) {
       for (int it = q * per; it < (q + 1) * per; ++it) {
-        const int i = tid + it * kThreads;
+        const int i = tid + it * TH;
         if (i < sh.nvec) {
           float f[N];
           Vec<T>::unpack(kept[i], f);
@@ -363,10 +371,10 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const DistillArgs
   } else {
     constexpr int U = 4;  // 16-byte loads in flight for each thread
     int i = tid;
-    for (; i + (U - 1) * kThreads < sh.nvec; i += U * kThreads) {
+    for (; i + (U - 1) * TH < sh.nvec; i += U * TH) {
       uint4 v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = __ldcs(src + i + u * kThreads);
+      for (int u = 0; u < U; ++u) v[u] = MODE == Grad::none ? __ldcs(src + i + u * TH) : src[i + u * TH];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float f[N];
@@ -374,9 +382,9 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const DistillArgs
         ms.add<N>(f, a.c);
       }
     }
-    for (; i < sh.nvec; i += kThreads) {
+    for (; i < sh.nvec; i += TH) {
       float f[N];
-      Vec<T>::unpack(__ldcs(src + i), f);
+      Vec<T>::unpack(src[i], f);
       ms.add<N>(f, a.c);
     }
   }
@@ -398,7 +406,7 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const DistillArgs
       if (a.stats) a.stats[row] = st;
     }
   }
-  if (!KEEP) return;
+  if (MODE == Grad::none) return;
   const float w = a.cot ? a.cot[row] : 1.f;
   if (w == 0.f) {
     zero_slice(g + c0, c1 - c0);
@@ -408,24 +416,36 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const DistillArgs
   const float qs = st.z_inv * scale;
   T *dst = g + c0 + sh.head;
   const bool aligned = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
-  for (int i = tid; i < sh.nvec; i += kThreads) {
+  auto put = [&](int i, const uint4 &v) {
     float f[N];
-    Vec<T>::unpack(kept[i], f);
+    Vec<T>::unpack(v, f);
 #pragma unroll
     for (int u = 0; u < N; ++u) f[u] = exp2_fast(fmaf(f[u], a.c, -st.z_max)) * qs;
     store_vec(dst + (int64_t)i * N, f, aligned);
+  };
+  if (KEEP) {
+    for (int i = tid; i < sh.nvec; i += TH) put(i, kept[i]);
+  } else {
+    constexpr int U = 4;
+    int i = tid;
+    for (; i + (U - 1) * TH < sh.nvec; i += U * TH) {
+      uint4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = __ldcs(src + i + u * TH);
+#pragma unroll
+      for (int u = 0; u < U; ++u) put(i + u * TH, v[u]);
+    }
+    for (; i < sh.nvec; i += TH) put(i, __ldcs(src + i));
   }
   if (has_loose) g[loose_col] = VT<T>::store(exp2_fast(fmaf(loose, a.c, -st.z_max)) * qs);
   __syncthreads();  // the slice in shared memory is done with: its space serves the teacher's entries
-  const int64_t words = (c1 - c0 + 31) / 32 * 4;
-  const int64_t bits_bytes = (words + 15) / 16 * 16;
+  const int64_t bits_bytes = (c1 - c0 + 127) / 128 * 16;
+  const int64_t table = KEEP ? (a.slice * (int64_t)sizeof(T) - bits_bytes) / 8 : kBackwardTable;
   subtract_teacher<T, I>(a, z, g, lo, hi, c0, c1, st, scale, reinterpret_cast<uint32_t *>(dyn),
-                         reinterpret_cast<unsigned long long *>(dyn + bits_bytes),
-                         (a.slice * (int64_t)sizeof(T) - bits_bytes) / 8);
+                         reinterpret_cast<unsigned long long *>(dyn + bits_bytes), table);
 }
 
 // The backward pass from the forward's statistics: one CTA for each slice.
-constexpr int kBackwardTable = 1024;
 
 template <typename T, typename I>
 __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const DistillArgs a) {
@@ -475,13 +495,13 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const Distil
 }
 
 template <typename K>
-void launch_rows(K kernel, const DistillArgs &a, size_t smem, cudaStream_t s) {
+void launch_rows(K kernel, const DistillArgs &a, int threads, size_t smem, cudaStream_t s) {
   const int64_t grid = a.rows * a.n_slices;
   if (grid > INT32_MAX) fail(MSX_ERR_OVERFLOW, "csr_distillation has too many rows for one call.");
   MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKept));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -522,23 +542,21 @@ template <typename T, typename I> void run_typed(const DistillCall &call, cudaSt
     distill_backward_kernel<T, I><<<(unsigned)(a.rows * a.n_slices), kThreads, smem, s>>>(a);
     MSX_CHECK_LAUNCH();
   };
+  // Short rows have few vectors for each thread and gain from more CTAs.
+  const bool small = row_bytes <= 40960;
   if (call.loss == nullptr) return backward();
   if (call.grad == nullptr) {
     split(pick_slices(a.rows, row_bytes, INT64_MAX, 8));
-    return launch_rows(distill_row_kernel<T, I, false>, a, 0, s);
+    if (small) return launch_rows(distill_row_kernel<T, I, Grad::none, 128>, a, 128, 0, s);
+    return launch_rows(distill_row_kernel<T, I, Grad::none, kThreads>, a, kThreads, 0, s);
   }
-  split(pick_slices(a.rows, row_bytes, 65536, 8));
+  split(pick_slices(a.rows, row_bytes, INT64_MAX, 8));
   const int64_t kept = a.slice * (int64_t)sizeof(T);
-  if (kept <= kMaxKept) return launch_rows(distill_row_kernel<T, I, true>, a, (size_t)kept, s);
-  // a row that a cluster's shared memory cannot hold: two passes
-  Scratch stats(sizeof(RowStats) * (size_t)a.rows, s);
-  a.stats = stats.as<RowStats>();
-  split(8);
-  void *grad = a.grad;
-  a.grad = nullptr;
-  launch_rows(distill_row_kernel<T, I, false>, a, 0, s);
-  a.grad = grad;
-  backward();
+  if (kept > kKeepMost)
+    return launch_rows(distill_row_kernel<T, I, Grad::reread, kRereadThreads>, a, kRereadThreads,
+                       (size_t)(ceil_div(a.slice, 128) * 16 + kBackwardTable * 8), s);
+  if (small) return launch_rows(distill_row_kernel<T, I, Grad::kept, 128>, a, 128, (size_t)kept, s);
+  launch_rows(distill_row_kernel<T, I, Grad::kept, kThreads>, a, kThreads, (size_t)kept, s);
 }
 
 }  // namespace
