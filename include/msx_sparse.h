@@ -497,7 +497,8 @@ MSX_API int msx_csr_distill_forward_backward(
  * k_len - q_len. With indptr (n_seq + 1 boundaries on the device, batch 1,
  * q_len = k_len) sequences lie one after another along the tokens; tokens
  * outside all of them see nothing and get zeros.
- * out, grad_out, dq are contiguous like q; dk, dv like k. lse: float (batch,
+ * out, grad_out, dq are contiguous like q; dk, dv like k. out_low, like out:
+ * what rounding out to a 16-bit type took off, for backward; may be null. lse: float (batch,
  * q_heads, q_len rounded up to a multiple of 128), 16-byte aligned, minus
  * the log-sum-exp in base 2, written by forward (null: not wanted), read by backward;
  * workspace: *floats of msx_window_attention_workspace, 16-byte aligned, for
@@ -512,15 +513,15 @@ MSX_API int msx_window_attention_forward(
     const int64_t *k_strides, const void *v, const int64_t *v_strides,
     int64_t batch, int64_t q_len, int64_t k_len, int64_t q_heads,
     int64_t k_heads, int64_t dim, int64_t window, int64_t sinks, float scale,
-    int index_dtype, const void *indptr, int64_t n_seq, void *out, float *lse,
-    void *stream);
+    int index_dtype, const void *indptr, int64_t n_seq, void *out, void *out_low,
+    float *lse, void *stream);
 MSX_API int msx_window_attention_backward(
     int value_dtype, const void *q, const int64_t *q_strides, const void *k,
     const int64_t *k_strides, const void *v, const int64_t *v_strides,
     int64_t batch, int64_t q_len, int64_t k_len, int64_t q_heads,
     int64_t k_heads, int64_t dim, int64_t window, int64_t sinks, float scale,
     int index_dtype, const void *indptr, int64_t n_seq, const void *out,
-    const float *lse, const void *grad_out, float *workspace, void *dq, void *dk,
+    const void *out_low, const float *lse, const void *grad_out, float *workspace, void *dq, void *dk,
     void *dv, void *stream);
 /* One query for each batch entry, at the end of that entry's cache: q (batch,
  * q_heads, dim) with strides {batch, heads}; caches (batch, max_len, k_heads,

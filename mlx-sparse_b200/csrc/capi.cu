@@ -694,13 +694,13 @@ int msx_window_attention_forward(int value_dtype, const void *q, const int64_t *
                                  const int64_t *k_strides, const void *v, const int64_t *v_strides, int64_t batch,
                                  int64_t q_len, int64_t k_len, int64_t q_heads, int64_t k_heads, int64_t dim,
                                  int64_t window, int64_t sinks, float scale, int index_dtype, const void *indptr,
-                                 int64_t n_seq, void *out, float *lse, void *stream) {
+                                 int64_t n_seq, void *out, void *out_low, float *lse, void *stream) {
   return guarded([&] {
     WindowCall c = window_checked(value_dtype, q, q_strides, k, k_strides, v, v_strides, batch, q_len, k_len, q_heads,
                                   k_heads, dim, window, sinks, scale, index_dtype);
     window_packed(c, indptr, n_seq);
     check_ptr(out, batch * q_len, "window_attention out");
-    c.out = out, c.lse = lse;
+    c.out = out, c.out_low = value_dtype == MSX_F32 ? nullptr : out_low, c.lse = lse;
     window_forward_run(value_dtype, c, as_stream(stream));
   });
 }
@@ -709,7 +709,8 @@ int msx_window_attention_backward(int value_dtype, const void *q, const int64_t 
                                   const int64_t *k_strides, const void *v, const int64_t *v_strides, int64_t batch,
                                   int64_t q_len, int64_t k_len, int64_t q_heads, int64_t k_heads, int64_t dim,
                                   int64_t window, int64_t sinks, float scale, int index_dtype, const void *indptr,
-                                  int64_t n_seq, const void *out, const float *lse, const void *grad_out,
+                                  int64_t n_seq, const void *out, const void *out_low, const float *lse,
+                                  const void *grad_out,
                                   float *workspace, void *dq, void *dk, void *dv, void *stream) {
   return guarded([&] {
     WindowCall c = window_checked(value_dtype, q, q_strides, k, k_strides, v, v_strides, batch, q_len, k_len, q_heads,
@@ -720,6 +721,7 @@ int msx_window_attention_backward(int value_dtype, const void *q, const int64_t 
     check_ptr(grad_out, batch * q_len, "window_attention grad_out");
     check_ptr(workspace, batch * q_len, "window_attention workspace");
     require((dk == nullptr) == (dv == nullptr), MSX_ERR_INVALID, "window_attention dk and dv come together.");
+    c.out_low = value_dtype == MSX_F32 ? nullptr : const_cast<void *>(out_low);
     c.out = const_cast<void *>(out), c.lse = const_cast<float *>(lse), c.grad_out = grad_out, c.delta = workspace;
     c.dq = dq, c.dk = dk, c.dv = dv;
     window_backward_run(value_dtype, c, as_stream(stream));

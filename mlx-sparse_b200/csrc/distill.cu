@@ -39,6 +39,11 @@ struct RowStats {
 
 constexpr int kMaxKept = 200 * 1024;  // dynamic shared memory, at most
 constexpr int kKeepMost = 64 * 1024;  // slices up to this are kept in shared memory
+// Longer ones are read again, in slices of 128 KB: four CTAs an SM then have few
+// enough bytes between their two reads for L2 (8192 x 128000 bf16: 860 us with a
+// cluster of two, 947 with whole rows, all of whose second reads miss, 1095 with
+// four slices and their waits).
+constexpr int kRereadMost = 128 * 1024;
 constexpr int kRereadThreads = 384;
 
 struct DistillArgs {
@@ -114,27 +119,29 @@ template <> struct Vec<__nv_bfloat16> {
   }
 };
 
-// Running maximum m of the logits and sum of 2^((z - m) c). A sum that is still
-// empty has m = -inf and sum 0; a NaN ends up in the sum.
+// Running maximum m of the logits and sum of 2^(z c - b) with b = m c rounded. A sum
+// that is still empty has m = -inf, b = 0 and sum 0; a NaN ends up in the sum. Sums
+// over different maxima are joined by the difference of their rounded b: the
+// product of an unrounded m c would leave the rounding's error in the sum, once
+// for every join.
 struct MaxSum {
-  float m = kNegInf, s = 0.f;
-  __device__ static float base(float m, float c) { return m == kNegInf ? 0.f : m * c; }
+  float m = kNegInf, b = 0.f, s = 0.f;
+  __device__ void raise(float top, float c) {
+    const float up = __fmul_rn(top, c);
+    if (m != kNegInf) s *= exp2_fast(b - up);
+    m = top, b = up;
+  }
   template <int N> __device__ void add(const float *z, float c) {
     float top = z[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) top = fmaxf(top, z[i]);
-    if (top > m) {
-      s *= exp2_fast(fmaf(m, c, -base(top, c)));
-      m = top;
-    }
-    const float b = base(m, c);
+    if (top > m) raise(top, c);
 #pragma unroll
     for (int i = 0; i < N; ++i) s += exp2_fast(fmaf(z[i], c, -b));
   }
   __device__ void join(float m2, float s2, float c) {
-    const float top = fmaxf(m, m2), b = base(top, c);
-    s = s * exp2_fast(fmaf(m, c, -b)) + s2 * exp2_fast(fmaf(m2, c, -b));
-    m = top;
+    if (m2 > m) raise(m2, c);
+    s += m2 == m || m2 == kNegInf ? s2 : s2 * exp2_fast(__fmul_rn(m2, c) - b);
   }
 };
 
@@ -398,7 +405,7 @@ __global__ void __launch_bounds__(TH, MODE == Grad::kept ? 1024 / TH : 1536 / TH
     all = MaxSum();
     for (int r = 0; r < n_ranks; ++r) all.join(ranks[r].x, ranks[r].y, a.c);
   }
-  const RowStats st{all.m * a.c, 1.f / all.s, ts.m * a.c, 1.f / ts.s};
+  const RowStats st{all.b, 1.f / all.s, ts.b, 1.f / ts.s};
   if (rank == 0) {
     const float loss = row_loss<T, I>(a, z, lo, hi, st, all.s, ts.s, reinterpret_cast<float *>(part));
     if (tid == 0) {
@@ -550,7 +557,7 @@ template <typename T, typename I> void run_typed(const DistillCall &call, cudaSt
     if (small) return launch_rows(distill_row_kernel<T, I, Grad::none, 128>, a, 128, 0, s);
     return launch_rows(distill_row_kernel<T, I, Grad::none, kThreads>, a, kThreads, 0, s);
   }
-  split(pick_slices(a.rows, row_bytes, INT64_MAX, 8));
+  split(pick_slices(a.rows, row_bytes, kRereadMost, 8));
   const int64_t kept = a.slice * (int64_t)sizeof(T);
   if (kept > kKeepMost)
     return launch_rows(distill_row_kernel<T, I, Grad::reread, kRereadThreads>, a, kRereadThreads,

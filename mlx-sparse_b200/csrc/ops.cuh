@@ -66,6 +66,7 @@ struct WindowCall {
   WindowTensor q, k, v;
   const void *grad_out;
   void *out, *dq, *dk, *dv;
+  void *out_low;  // what rounding out to its 16-bit type took off, in that type; may be null
   float *lse, *delta;
   int64_t batch, q_len, k_len;
   int q_heads, k_heads, dim;

@@ -103,8 +103,11 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) forward_ker
 #pragma unroll
     for (int x = 0; x < kRegs; ++x) {
       const int d = x * 32 + lane;
-      if (d < dim)
-        out[((b * w.c.q_len + i) * w.c.q_heads + h) * dim + d] = VT<T>::store(empty ? 0.f : acc[r][x] * inv);
+      if (d >= dim) continue;
+      const int64_t at = ((b * w.c.q_len + i) * w.c.q_heads + h) * dim + d;
+      const float o = empty ? 0.f : acc[r][x] * inv;
+      out[at] = VT<T>::store(o);
+      if (w.c.out_low) static_cast<T *>(w.c.out_low)[at] = VT<T>::store(o - VT<T>::load(out[at]));
     }
     // an empty row's -inf makes its probabilities 0 in the backward pass
     if (w.c.lse && lane == 0)
@@ -113,8 +116,9 @@ template <typename T> __global__ void __launch_bounds__(kWarps * 32) forward_ker
 }
 
 // -delta_i = -dO_i . O_i, 16 lanes for each row and head, VEC elements at a time.
-// O is the rounded output: the error that brings (half a step of O's type, times
-// dO) is of the size of the rounding of the gradients themselves.
+// Of a 16-bit output what its rounding took off is added back: the same error of
+// delta reaches every key of a row, which would cost dQ and dK as much as all their
+// other roundings where a row sees few keys.
 template <typename T, int VEC> __global__ void delta_kernel(const WindowProblem w) {
   const int64_t x = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
   const int lane = threadIdx.x & 15;
@@ -122,16 +126,18 @@ template <typename T, int VEC> __global__ void delta_kernel(const WindowProblem 
   float s = 0.f;
   if (inside) {
     const T *o = static_cast<const T *>(w.c.out) + x * w.c.dim, *g = static_cast<const T *>(w.c.grad_out) + x * w.c.dim;
+    const T *l = w.c.out_low ? static_cast<const T *>(w.c.out_low) + x * w.c.dim : nullptr;
     for (int d = lane * VEC; d < w.c.dim; d += 16 * VEC) {
-      alignas(16) T a[VEC], b[VEC];
+      alignas(16) T a[VEC], b[VEC], c[VEC];
       if (VEC > 1) {
         *reinterpret_cast<uint4 *>(a) = __ldcs(reinterpret_cast<const uint4 *>(o + d));
         *reinterpret_cast<uint4 *>(b) = __ldcs(reinterpret_cast<const uint4 *>(g + d));
+        *reinterpret_cast<uint4 *>(c) = l ? __ldcs(reinterpret_cast<const uint4 *>(l + d)) : make_uint4(0, 0, 0, 0);
       } else {
-        a[0] = o[d], b[0] = g[d];
+        a[0] = o[d], b[0] = g[d], c[0] = l ? l[d] : VT<T>::store(0.f);
       }
 #pragma unroll
-      for (int y = 0; y < VEC; ++y) s = fmaf(VT<T>::load(a[y]), VT<T>::load(b[y]), s);
+      for (int y = 0; y < VEC; ++y) s = fmaf(VT<T>::load(a[y]) + VT<T>::load(c[y]), VT<T>::load(b[y]), s);
     }
   }
 #pragma unroll
@@ -297,7 +303,8 @@ void window_forward_general(const WindowProblem &w, int value_dtype, cudaStream_
 void window_delta(const WindowProblem &w, int value_dtype, cudaStream_t s) {
   const int64_t rows = w.c.batch * w.c.q_len * w.c.q_heads;
   if (rows == 0) return;
-  const uintptr_t at = reinterpret_cast<uintptr_t>(w.c.out) | reinterpret_cast<uintptr_t>(w.c.grad_out);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(w.c.out) | reinterpret_cast<uintptr_t>(w.c.grad_out) |
+                       reinterpret_cast<uintptr_t>(w.c.out_low);
   dispatch_value(value_dtype, [&](auto v) {
     using T = decltype(v);
     constexpr int kVec = 16 / sizeof(T);

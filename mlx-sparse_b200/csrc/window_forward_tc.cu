@@ -144,10 +144,15 @@ __device__ __noinline__ void repair_row(const WindowProblem &w, int b, int h, in
       }
     }
   }
-  T *out = static_cast<T *>(w.c.out) + ((b * w.c.q_len + i) * w.c.q_heads + h) * dim;
+  const int64_t at = ((b * w.c.q_len + i) * w.c.q_heads + h) * dim;
+  T *out = static_cast<T *>(w.c.out) + at;
 #pragma unroll
-  for (int x = 0; x < 4; ++x)
-    if (x * 32 + lane < dim) out[x * 32 + lane] = VT<T>::store(acc[x] / l);
+  for (int x = 0; x < 4; ++x) {
+    const int d = x * 32 + lane;
+    if (d >= dim) continue;
+    out[d] = VT<T>::store(acc[x] / l);
+    if (w.c.out_low) static_cast<T *>(w.c.out_low)[at + d] = VT<T>::store(acc[x] / l - VT<T>::load(out[d]));
+  }
   if (w.c.lse && lane == 0) w.c.lse[((int64_t)b * w.c.q_heads + h) * w.lse_row + i] = -(m + log2f(l));
 }
 
@@ -384,7 +389,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
       }
       const bool inside = i < w.c.q_len, empty = span.empty();
       const float inv = empty ? 0.f : 1.f / l;
-      T *out = static_cast<T *>(w.c.out) + ((it.b * w.c.q_len + i - lane) * w.c.q_heads + h) * w.c.dim;
+      const int64_t first = ((it.b * w.c.q_len + i - lane) * w.c.q_heads + h) * w.c.dim;
+      T *out = static_cast<T *>(w.c.out) + first;
       bool bad = false;
 #pragma unroll
       for (int x = 0; x < DB * 64; x += 32) {
@@ -399,6 +405,15 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
           for (int y = 0; y < 32; ++y) o[y] = 0;
         }
         bad = store32<T>(out, (int64_t)w.c.q_heads * w.c.dim, o, inv, x, w.c.dim, (int)w.c.q_len - (i - lane)) || bad;
+        if (w.c.out_low) {
+#pragma unroll
+          for (int y = 0; y < 32; ++y) {
+            const float e = __uint_as_float(o[y]) * inv;
+            o[y] = __float_as_uint(e - VT<T>::load(VT<T>::store(e)));
+          }
+          store32<T>(static_cast<T *>(w.c.out_low) + first, (int64_t)w.c.q_heads * w.c.dim, o, 1.f, x, w.c.dim,
+                     (int)w.c.q_len - (i - lane));
+        }
       }
       if (inside && w.c.lse)
         w.c.lse[((int64_t)it.b * w.c.q_heads + h) * w.lse_row + i] = empty ? -INFINITY : -(m * c + log2f(l));

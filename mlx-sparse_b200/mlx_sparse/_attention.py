@@ -68,7 +68,7 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, scale=None, indptr
 
         out = WindowAttention.apply(q, k, v, int(window), int(sinks), scale, indptr)
     else:
-        out, _ = _native.window_attention_forward(q, k, v, int(window), int(sinks), scale, indptr, with_lse=False)
+        out = _native.window_attention_forward(q, k, v, int(window), int(sinks), scale, indptr, with_lse=False)[0]
     return out if indptr is None else out.squeeze(0)
 
 

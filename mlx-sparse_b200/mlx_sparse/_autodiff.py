@@ -74,21 +74,22 @@ class CsrDistillation(torch.autograd.Function):
 
 class WindowAttention(torch.autograd.Function):
     """Windowed attention on rank-4 operands, differentiable once in ``q``,
-    ``k`` and ``v``. Keeps the output and each row's log-sum-exp."""
+    ``k`` and ``v``. Keeps the output, what its rounding took off, and each row's
+    log-sum-exp."""
 
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, scale, indptr):
-        out, lse = _native.window_attention_forward(q, k, v, window, sinks, scale, indptr, with_lse=True)
+        out, low, lse = _native.window_attention_forward(q, k, v, window, sinks, scale, indptr, with_lse=True)
         ctx.args = (window, sinks, scale, indptr)
-        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.save_for_backward(q, k, v, out, low, lse)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, low, lse = ctx.saved_tensors
         need_q, need_kv = ctx.needs_input_grad[0], any(ctx.needs_input_grad[1:3])
-        dq, dk, dv = _native.window_attention_backward(q, k, v, out, lse, grad, *ctx.args, want_q=need_q,
+        dq, dk, dv = _native.window_attention_backward(q, k, v, out, low, lse, grad, *ctx.args, want_q=need_q,
                                                        want_kv=need_kv)
         return (dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None,
                 None)

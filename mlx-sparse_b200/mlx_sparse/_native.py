@@ -91,8 +91,8 @@ def extension():
         L.msx_csr_distill_backward.argtypes = distill + [p, p, p, p]
         L.msx_csr_distill_forward_backward.argtypes = distill + [p, p, p, p]
         window = [c_int, p, p, p, p, p, p, i64, i64, i64, i64, i64, i64, i64, i64, c_float, c_int, p, i64]
-        L.msx_window_attention_forward.argtypes = window + [p, p, p]
-        L.msx_window_attention_backward.argtypes = window + [p, p, p, p, p, p, p, p]
+        L.msx_window_attention_forward.argtypes = window + [p, p, p, p]
+        L.msx_window_attention_backward.argtypes = window + [p, p, p, p, p, p, p, p, p]
         L.msx_window_attention_workspace.argtypes = [i64] * 8 + [ctypes.POINTER(i64)]
         L.msx_window_attention_decode.argtypes = [c_int, p, p, p, p, p, p, i64, i64, i64, i64, i64, i64, i64, c_float,
                                                   c_int, p, p, p]
@@ -655,22 +655,25 @@ def _window_args(q, k, v, window, sinks, scale, indptr):
 
 
 def window_attention_forward(q, k, v, window, sinks, scale, indptr=None, *, with_lse: bool):
-    """Rank-4 ``q``, ``k``, ``v``; returns ``(out, lse)`` (lse None unless wanted)."""
+    """Rank-4 ``q``, ``k``, ``v``; returns ``(out, low, lse)``. ``low`` and
+    ``lse`` are for the backward call and None unless ``with_lse``: what rounding
+    ``out`` to a 16-bit type took off, and each row's log-sum-exp."""
     L = extension()
     dev = require_cuda(q, k, v) if indptr is None else require_cuda(q, k, v, indptr)
     q, k, v = heads_of(q), heads_of(k), heads_of(v)
     indptr = None if indptr is None else indptr.contiguous()
     out = q.new_empty(q.shape)
-    lse = None
-    if with_lse:  # the kernels read whole tiles of it
+    low = lse = None
+    if with_lse:  # the kernels read whole tiles of lse
+        low = q.new_empty(q.shape) if q.element_size() == 2 else None
         lse = torch.empty((q.shape[0], q.shape[2], (q.shape[1] + 127) // 128 * 128), dtype=torch.float32, device=dev)
     args, _keep = _window_args(q, k, v, window, sinks, scale, indptr)
     with _on(dev):
-        check(L.msx_window_attention_forward(*args, out.data_ptr(), _p(lse), _stream(dev)))
-    return out, lse
+        check(L.msx_window_attention_forward(*args, out.data_ptr(), _p(low), _p(lse), _stream(dev)))
+    return out, low, lse
 
 
-def window_attention_backward(q, k, v, out, lse, grad, window, sinks, scale, indptr=None, *, want_q=True,
+def window_attention_backward(q, k, v, out, low, lse, grad, window, sinks, scale, indptr=None, *, want_q=True,
                               want_kv=True):
     L = extension()
     dev = require_cuda(q, k, v, out, lse, grad)
@@ -685,7 +688,7 @@ def window_attention_backward(q, k, v, out, lse, grad, window, sinks, scale, ind
     dk, dv = (k.new_empty(k.shape), k.new_empty(k.shape)) if want_kv else (None, None)
     args, _keep = _window_args(q, k, v, window, sinks, scale, indptr)
     with _on(dev):
-        check(L.msx_window_attention_backward(*args, out.data_ptr(), lse.data_ptr(), grad.data_ptr(), work.data_ptr(),
+        check(L.msx_window_attention_backward(*args, out.data_ptr(), _p(low), lse.data_ptr(), grad.data_ptr(), work.data_ptr(),
                                               _p(dq), _p(dk), _p(dv), _stream(dev)))
     return dq, dk, dv
 

@@ -73,7 +73,7 @@ def test_window_entry_points():
     def forward(vt=2, strides=st, batch=0, q_len=4, k_len=4, hq=4, hk=2, dim=64, window=2, sinks=0, scale=1.0, it=0,
                 indptr=None, n_seq=0):
         return lib.msx_window_attention_forward(vt, None, strides, None, st, None, st, batch, q_len, k_len, hq, hk, dim,
-                                                window, sinks, scale, it, indptr, n_seq, None, None, None)
+                                                window, sinks, scale, it, indptr, n_seq, None, None, None, None)
 
     for bad in (dict(batch=-1), dict(q_len=-1), dict(hq=3), dict(hk=0), dict(dim=0), dict(dim=257), dict(window=-1),
                 dict(sinks=-1), dict(scale=float("nan")), dict(strides=None), dict(batch=1), dict(indptr=8, n_seq=1)):
