@@ -89,8 +89,9 @@ MSX_API int msx_compiled_sm(void);
  * call; off by default, plain loads measured faster on B200) wait on
  * shared-memory barriers with a bounded number of polls; if a wait
  * gives up, the kernel stops, records the event in a per-device flag and the
- * rows it had not reached stay unwritten. The flag is sticky: this call
- * synchronises `stream`, reads and clears the flag of the current device and
+ * rows it had not reached stay unwritten. The tensor-core kernels of windowed
+ * attention have such waits and a flag of their own. The flags are sticky: this call
+ * synchronises `stream`, reads and clears the flags of the current device and
  * returns MSX_ERR_RUNTIME if it was set. No counterpart in the reference,
  * whose CPU loops cannot time out. */
 MSX_API int msx_check_device_errors(void *stream);

@@ -33,7 +33,7 @@ __device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
 // A wait that gives up after `kWaitNs`, far beyond any run of these kernels: it
 // then sets the device's error flag and the CTA's `stop`, which makes every
 // other wait of the CTA give up too, so that all warps reach the kernel's end.
-constexpr unsigned long long kWaitNs = 4ull * 1000 * 1000 * 1000;
+constexpr unsigned long long kWaitNs = 20ull * 1000 * 1000 * 1000;
 __device__ __forceinline__ unsigned long long now_ns() {
   unsigned long long t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));

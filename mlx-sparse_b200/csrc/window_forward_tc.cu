@@ -47,6 +47,7 @@ struct Bars {
   uint64_t kv_full[8], step[8];
   uint32_t tmem;
   int stop;
+  float max1[kM], sum1[kM];  // the second slot's, where both share the queries
 };
 
 template <int DB> struct Shape {  // DB boxes of 64 elements cover the head size
@@ -70,10 +71,20 @@ struct Item {
   int last[2];  // the last tile of keys that a slot takes part in, -1: none
 };
 
-__device__ __forceinline__ Item item_of(const Params &p, int n) {
+template <bool SPLIT> __device__ __forceinline__ Item item_of(const Params &p, int n) {
   const WindowProblem &w = p.w;
   Item it;
-  if (p.paired) {
+  if (SPLIT) {
+    it.i0[0] = it.i0[1] = n % p.q_tiles * kM;
+    n /= p.q_tiles;
+    it.head[0] = it.head[1] = n % w.c.q_heads;
+    it.b = n / w.c.q_heads;
+    it.hk = it.head[0] / w.group;
+    it.both = it.range[0] = it.range[1] = key_range(w, it.b, it.i0[0], it.i0[0] + kM - 1);
+    const int tiles = KeyTiles<kN>(it.both).n;
+    it.last[0] = tiles == 0 ? -1 : (tiles - 1) & ~1;
+    it.last[1] = tiles < 2 ? -1 : (tiles - 2) | 1;
+  } else if (p.paired) {
     const int pairs = w.group / 2;
     const int pair = n % pairs;
     n /= pairs;
@@ -156,7 +167,9 @@ __device__ __noinline__ void repair_row(const WindowProblem &w, int b, int h, in
   if (w.c.lse && lane == 0) w.c.lse[((int64_t)b * w.c.q_heads + h) * w.lse_row + i] = -(m + log2f(l));
 }
 
-template <typename T, int DB>
+// SPLIT: both slots share the queries. LOW: what the rounding of the output takes
+// off is kept too. (As run-time branches the two cost the other calls 10%.)
+template <typename T, int DB, bool SPLIT, bool LOW>
 __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_constant__ Params p) {
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   using Sh = Shape<DB>;
@@ -200,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
       int stage = 0;
       bool ok = true;
       for (int n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
-        const Item it = item_of(p, n);
+        const Item it = item_of<SPLIT>(p, n);
         const KeyTiles<kN> tiles(it.both);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -239,10 +252,12 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
       if (++stage == Sh::stages) stage = 0, phase ^= 1;
     };
     for (int n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
-      const Item it = item_of(p, n);
+      const Item it = item_of<SPLIT>(p, n);
       const KeyTiles<kN> tiles(it.both);
       if (tiles.n == 0) continue;
-      auto takes = [&](int s, int t) { return p.paired || it.range[s].touches(tiles.first(t), tiles.end(t)); };
+      auto takes = [&](int s, int t) {
+        return SPLIT ? (t & 1) == s : p.paired || it.range[s].touches(tiles.first(t), tiles.end(t));
+      };
       auto scores = [&](int s, int st, bool last_one) {
         mm.scores(tmem + s * kN, q_addr + s * Sh::tile, kv_addr + st * Sh::tile);
         mma_commit(mm.leader, &bars.s_full[s]);
@@ -263,10 +278,35 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
       next();
       for (int t = 0; ok && t < tiles.n; ++t) {
         const int v_stage = stage;
+        const uint32_t v_phase = phase;
+        const bool more = t + 1 < tiles.n;
+        if (SPLIT) {
+          // the slots take turns: the other one's scores before this one's output
+          next();
+          if (more) {
+            if (!need(warp_wait(&bars.kv_full[stage], phase, stop, p.error))) break;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+              if ((t & 1) != s) scores(s, stage, it.last[s] == t + 1);
+          }
+          need(warp_wait(&bars.kv_full[v_stage], v_phase, stop, p.error));
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+            if ((t & 1) == s) {
+              need(warp_wait(&bars.p_full[s], p_phase[s], stop, p.error));
+              fence_after();
+              mm.sums(tmem + 256 + s * 128, tmem + s * kN, kv_addr + v_stage * Sh::tile, started[s]);
+              if (t == it.last[s]) mma_commit(mm.leader, &bars.o_full[s]);
+              p_phase[s] ^= 1;
+              started[s] = true;
+            }
+          mma_commit(mm.leader, &bars.step[steps++ & 7]);
+          if (more) next();
+          continue;
+        }
         if (!need(warp_wait(&bars.kv_full[stage], phase, stop, p.error))) break;
         next();
         const int k_stage = stage;
-        const bool more = t + 1 < tiles.n;
         const bool now[2] = {takes(0, t), takes(1, t)}, then[2] = {more && takes(0, t + 1), more && takes(1, t + 1)};
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -294,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
     uint32_t s_phase = 0, o_phase = 0;
     bool ok = true;
     for (int n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
-      const Item it = item_of(p, n);
+      const Item it = item_of<SPLIT>(p, n);
       const KeyTiles<kN> tiles(it.both);
       const KeyRange range = s ? it.range[1] : it.range[0];
       const int i = (s ? it.i0[1] : it.i0[0]) + row, h = s ? it.head[1] : it.head[0];
@@ -305,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
       float m = -INFINITY, l = 0.f;
       bool started = false;
       for (int t = 0; ok && t < tiles.n; ++t) {
-        if (!p.paired && !range.touches(tiles.first(t), tiles.end(t))) continue;
+        if (SPLIT ? (t & 1) != s : !p.paired && !range.touches(tiles.first(t), tiles.end(t))) continue;
         if (!(ok = warp_wait(&bars.s_full[s], s_phase, stop, p.error))) break;
         fence_after();
         const int j0 = tiles.first(t), j1 = tiles.end(t);
@@ -381,6 +421,21 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         started = true;
         s_phase ^= 1;
       }
+      float keep0 = 1.f, keep1 = 0.f;
+      if (SPLIT) {
+        // One item a CTA. The first slot's warps write the row; they read the second's
+        // output too. The barrier is met on every path.
+        if (s == 1) bars.max1[row] = m, bars.sum1[row] = l;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (s == 1 || !ok) break;
+        if (it.last[1] >= 0) {
+          if (!(ok = warp_wait(&bars.o_full[1], 0, stop, p.error))) break;
+          const float m1 = bars.max1[row], top = fmaxf(m, m1);
+          keep0 = m == -INFINITY ? 0.f : exp2_fast((m - top) * c);
+          keep1 = m1 == -INFINITY ? 0.f : exp2_fast((m1 - top) * c);
+          l = l * keep0 + bars.sum1[row] * keep1, m = top;
+        }
+      }
       if (!ok) break;
       if (started) {
         if (!(ok = warp_wait(&bars.o_full[s], o_phase, stop, p.error))) break;
@@ -399,13 +454,22 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
           tmem_ld16(t_o + x, o), tmem_ld16(t_o + x + 16, o + 16);
           wait_ld();
           tie32(o);
+          if (SPLIT && it.last[1] >= 0) {
+            uint32_t o1[32];
+            tmem_ld16(t_o + 128 + x, o1), tmem_ld16(t_o + 128 + x + 16, o1 + 16);
+            wait_ld();
+            tie32(o1);
+#pragma unroll
+            for (int y = 0; y < 32; ++y)
+              o[y] = __float_as_uint(__uint_as_float(o[y]) * keep0 + __uint_as_float(o1[y]) * keep1);
+          }
         }
         if (!started || empty) {
 #pragma unroll
           for (int y = 0; y < 32; ++y) o[y] = 0;
         }
         bad = store32<T>(out, (int64_t)w.c.q_heads * w.c.dim, o, inv, x, w.c.dim, (int)w.c.q_len - (i - lane)) || bad;
-        if (w.c.out_low) {
+        if (LOW) {
 #pragma unroll
           for (int y = 0; y < 32; ++y) {
             const float e = __uint_as_float(o[y]) * inv;
@@ -450,11 +514,17 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
   if (warp == 1) tmem_free(tmem, 512);
 }
 
-template <typename T, int DB> void launch(Params &p, cudaStream_t s) {
-  auto kernel = forward_tc_kernel<T, DB>;
-  MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DB>::smem));
-  kernel<<<(unsigned)std::min(p.items, num_sms()), kThreads, Shape<DB>::smem, s>>>(p);
-  MSX_CHECK_LAUNCH();
+template <typename T, int DB> void launch(Params &p, bool split, cudaStream_t s) {
+  auto run = [&](auto kernel) {
+    MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DB>::smem));
+    kernel<<<(unsigned)std::min(p.items, num_sms()), kThreads, Shape<DB>::smem, s>>>(p);
+    MSX_CHECK_LAUNCH();
+  };
+  const bool low = p.w.c.out_low != nullptr;
+  if (split)
+    low ? run(forward_tc_kernel<T, DB, true, true>) : run(forward_tc_kernel<T, DB, true, false>);
+  else
+    low ? run(forward_tc_kernel<T, DB, false, true>) : run(forward_tc_kernel<T, DB, false, false>);
 }
 
 }  // namespace
@@ -491,16 +561,18 @@ void window_forward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s) 
   p.k = make_map(w.c.k, w.c.batch, w.c.k_len, w.c.k_heads, w.c.dim, bf16, kN);
   p.v = make_map(w.c.v, w.c.batch, w.c.k_len, w.c.k_heads, w.c.dim, bf16, kN);
   p.q_tiles = (int)ceil_div(w.c.q_len, kM);
-  p.paired = w.group % 2 == 0;
-  const int64_t items = p.paired ? w.c.batch * w.c.k_heads * p.q_tiles * (w.group / 2)
+  const bool split = w.c.batch * w.c.q_heads * p.q_tiles <= num_sms();
+  p.paired = !split && w.group % 2 == 0;
+  const int64_t items = split ? w.c.batch * w.c.q_heads * p.q_tiles
+                        : p.paired ? w.c.batch * w.c.k_heads * p.q_tiles * (w.group / 2)
                                  : w.c.batch * w.c.q_heads * ((p.q_tiles + 1) / 2);
   if (items > INT32_MAX / 2) fail(MSX_ERR_OVERFLOW, "window_attention has too many queries and heads for one call.");
   p.items = (int)items;
   p.error = window_error_flag();
   if (bf16) {
-    if (w.c.dim <= 64) launch<__nv_bfloat16, 1>(p, s); else launch<__nv_bfloat16, 2>(p, s);
+    if (w.c.dim <= 64) launch<__nv_bfloat16, 1>(p, split, s); else launch<__nv_bfloat16, 2>(p, split, s);
   } else {
-    if (w.c.dim <= 64) launch<__half, 1>(p, s); else launch<__half, 2>(p, s);
+    if (w.c.dim <= 64) launch<__half, 1>(p, split, s); else launch<__half, 2>(p, split, s);
   }
 }
 

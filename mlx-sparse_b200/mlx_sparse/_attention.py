@@ -43,16 +43,18 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, scale=None, indptr
     dimension is strided, or whose 16-bit rows do not start on 16-byte
     boundaries, is copied first.
 
-    Differentiable (once) in ``q``, ``k`` and ``v``.
+    Differentiable (once) in ``q``, ``k`` and ``v``. A training step can be captured
+    into a CUDA graph under torch's rule for it: no eager graph of the same leaves
+    may be alive meanwhile.
     """
     q = ensure_array(q)
     k, v = ensure_array(k, device=q.device), ensure_array(v, device=q.device)
     if indptr is None:
-        scale = validate_window_inputs(q, k, v, window, sinks, scale, rank=4, name="window_attention")
+        window, sinks, scale = validate_window_inputs(q, k, v, window, sinks, scale, rank=4, name="window_attention")
         if q.shape[0] != k.shape[0]:
             raise ValueError(f"window_attention q and k must have one batch size, got {q.shape[0]} and {k.shape[0]}.")
     else:
-        scale = validate_window_inputs(q, k, v, window, sinks, scale, rank=3, name="window_attention")
+        window, sinks, scale = validate_window_inputs(q, k, v, window, sinks, scale, rank=3, name="window_attention")
         indptr = ensure_array(indptr, device=q.device)
         check_rank1("window_attention indptr", indptr)
         check_index_dtype("window_attention indptr", indptr)
@@ -66,9 +68,9 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, scale=None, indptr
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         from mlx_sparse._autodiff import WindowAttention
 
-        out = WindowAttention.apply(q, k, v, int(window), int(sinks), scale, indptr)
+        out = WindowAttention.apply(q, k, v, window, sinks, scale, indptr)
     else:
-        out = _native.window_attention_forward(q, k, v, int(window), int(sinks), scale, indptr, with_lse=False)[0]
+        out = _native.window_attention_forward(q, k, v, window, sinks, scale, indptr, with_lse=False)[0]
     return out if indptr is None else out.squeeze(0)
 
 
@@ -91,7 +93,8 @@ def window_attention_decode(q, k_cache, v_cache, lengths, *, window: int, sinks:
     if q.ndim != 3 or k_cache.ndim != 4 or v_cache.ndim != 4:
         raise ValueError(f"{name} expects q of rank 3 and caches of rank 4, got {q.ndim}, {k_cache.ndim} and "
                          f"{v_cache.ndim}.")
-    scale = validate_window_inputs(q.unsqueeze(1), k_cache, v_cache, window, sinks, scale, rank=4, name=name)
+    window, sinks, scale = validate_window_inputs(q.unsqueeze(1), k_cache, v_cache, window, sinks, scale, rank=4,
+                                                  name=name)
     check_rank1(f"{name} lengths", lengths)
     check_index_dtype(f"{name} lengths", lengths)
     if not q.shape[0] == k_cache.shape[0] == lengths.shape[0]:
@@ -99,4 +102,4 @@ def window_attention_decode(q, k_cache, v_cache, lengths, *, window: int, sinks:
                          f"{k_cache.shape[0]} and {lengths.shape[0]}.")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise ValueError(f"{name} has no gradient; use window_attention, or call it under torch.no_grad().")
-    return _native.window_attention_decode(q, k_cache, v_cache, lengths, int(window), int(sinks), scale)
+    return _native.window_attention_decode(q, k_cache, v_cache, lengths, window, sinks, scale)

@@ -171,8 +171,9 @@ def validate_distillation_inputs(data, indices, indptr, logits, shape, temperatu
         raise ValueError(f"csr_distillation temperature must be positive and finite, got {temperature}.")
 
 
-def validate_window_inputs(q, k, v, window, sinks, scale, *, rank, name) -> float:
-    """Shapes and types of windowed attention; returns the scale to use."""
+def validate_window_inputs(q, k, v, window, sinks, scale, *, rank, name) -> tuple[int, int, float]:
+    """Shapes and types of windowed attention; returns the window, the sinks
+    (both cut to 2**31, more than any sequence) and the scale to use."""
     if q.ndim != rank or k.ndim != rank or v.ndim != rank:
         raise ValueError(f"{name} got q of shape {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)}.")
     for label, t in (("q", q), ("k", k), ("v", v)):
@@ -199,4 +200,4 @@ def validate_window_inputs(q, k, v, window, sinks, scale, *, rank, name) -> floa
     scale = float(dim) ** -0.5 if scale is None else float(scale)
     if not np.isfinite(scale):
         raise ValueError(f"{name} scale must be finite, got {scale}.")
-    return scale
+    return min(int(window), 1 << 31), min(int(sinks), 1 << 31), scale

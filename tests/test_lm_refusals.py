@@ -51,7 +51,7 @@ def test_window_metadata():
     def check(q=q, k=k, w=k, window=3, sinks=0, scale=None, rank=4):
         return v.validate_window_inputs(q, k, w, window, sinks, scale, rank=rank, name="window_attention")
 
-    assert check() == 8 ** -0.5 and check(scale=2) == 2.0
+    assert check() == (3, 0, 8 ** -0.5) and check(scale=2, window=2 ** 70, sinks=5) == (2 ** 31, 5, 2.0)
     for bad in (dict(q=q[0]), dict(w=k[:, :3]), dict(q=q[..., :4]), dict(q=q[:, :, :3]), dict(q=q[:, :, :0]),
                 dict(window=-1), dict(sinks=-1), dict(scale=float("nan")), dict(rank=3),
                 dict(q=q.repeat(1, 1, 1, 40), k=k.repeat(1, 1, 1, 40), w=k.repeat(1, 1, 1, 40))):

@@ -125,6 +125,9 @@ SHAPES = [
     (1, 400, 400, 2, 2, 8, 64, 70),
     (1, 1, 900, 4, 2, 128, 1000, 0),
     (1, 1100, 1100, 2, 1, 128, 384, 16),
+    (1, 900, 500, 2, 1, 64, 60, 3),     # sinks with queries in several chunks: more queries than keys,
+    (2, 600, 1500, 4, 2, 64, 70, 4),   # fewer,
+    (1, 1100, 1100, 3, 1, 128, 30, 100),  # sinks over most of a tile of keys
     (1, 95, 95, 2, 1, 33, 20, 1),      # head sizes that are the general kernels'
     (1, 40, 40, 2, 1, 256, 11, 2),
     (1, 50, 50, 1, 1, 1, 7, 0),
@@ -163,6 +166,20 @@ def test_packed_sequences(ms, dtype, dim, index):
     for x, ref, name in zip(got, refs, ("out", "dq", "dk", "dv")):
         _check(x, ref, name)
         assert (x[:3] == 0).all() and (x[760:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bounds", [[0, 256, 900, 1030, 1800], [0, 250, 270, 1300, 1305, 1800], [100, 255, 257, 1700]])
+@pytest.mark.parametrize("sinks", [1, 5, 128])
+def test_sinks_of_long_packed_sequences(ms, dtype, bounds, sinks):
+    """Sequences that start at, before and behind the 256-query chunks in which
+    far queries reach their sinks."""
+    tokens, dim = 1850, 64
+    q, k, v, g = (_rand((tokens, 2, dim), dtype, s) for s in (1, 2, 3, 4))
+    refs = _reference(q[None], k[None], v[None], _mask(tokens, tokens, 40, sinks, bounds), dim ** -0.5, g[None])
+    got = _all(ms, q, k, v, g, window=40, sinks=sinks, indptr=torch.tensor(bounds).cuda())
+    for x, ref, name in zip(got, refs, ("out", "dq", "dk", "dv")):
+        _check(x, ref, name)
 
 
 @pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.bfloat16, 64), (torch.float16, 128)])
@@ -494,6 +511,9 @@ def test_nothing_to_do(ms, b, n, m):
     assert out.shape == q.shape and (out == 0).all()
     out.sum().backward()
     assert (q.grad == 0).all() and (k.grad == 0).all() and (v.grad == 0).all()
+    if n == 3:
+        none = ms.window_attention_decode(q[:, 0].detach(), k.detach(), v.detach(), torch.tensor([0, 7]).cuda(), window=2)
+        assert none.shape == (2, 2, 64) and (none == 0).all()
     if n == m == 5:
         empty = ms.window_attention_decode(q[:, 0].detach(), k.detach(), v.detach(), torch.zeros(0).cuda().int(), window=2)
         assert empty.shape == (0, 2, 64)
@@ -506,6 +526,15 @@ def test_boundaries_outside_the_tokens_do_not_reach_memory(ms):
         assert all(torch.isfinite(t).all() for t in got)
     want = ms.window_attention(q, k, v, window=9, sinks=2, indptr=torch.tensor([0, 50]).cuda())
     assert torch.equal(ms.window_attention(q, k, v, window=9, sinks=2, indptr=torch.tensor([0, 90]).cuda()), want)
+
+
+def test_windows_beyond_64_bits(ms):
+    q, k = _rand((1, 70, 2, 64), torch.bfloat16, 1), _rand((1, 70, 2, 64), torch.bfloat16, 2)
+    want = ms.window_attention(q, k, k, window=70, sinks=70)
+    assert torch.equal(ms.window_attention(q, k, k, window=2 ** 64, sinks=2 ** 65), want)
+    n = torch.tensor([70]).cuda()
+    assert torch.equal(ms.window_attention_decode(q[:, 0], k, k, n, window=2 ** 64),
+                       ms.window_attention_decode(q[:, 0], k, k, n, window=70))
 
 
 def test_refusals(ms):
