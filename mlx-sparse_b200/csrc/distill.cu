@@ -11,7 +11,9 @@
 // gradient. Everything is computed in base 2 (c = log2(e) / T) and in fp32;
 // the gradient is rounded once, to the logits' type.
 //
-// Bound: HBM. Forward reads the logits once, the backward pass reads them
+// Bound: HBM (8192 x 128000 bf16: forward 0.34 ms, backward 0.69 ms, both in one
+// pass 0.87 ms, where the special-function unit's two exponentials and a
+// conversion for each logit, 0.55 ms, are the next limit). Forward reads the logits once, the backward pass reads them
 // again and writes the gradient. The one-pass form reads HBM once and writes
 // once, two thirds of the bytes of the two passes: a row's logits stay on chip
 // between the sum of the exponentials and the gradient, in shared memory where
@@ -314,7 +316,9 @@ constexpr int kGroups = 4;  // commit groups of a slice: the sums start when the
 enum class Grad { none, kept, reread };
 constexpr int kBackwardTable = 1024;  // columns at a time of repeated entries' sums
 
-// One cluster for each row, one slice of the row for each CTA.
+// One cluster for each row, one slice of the row for each CTA. Registers are held to
+// what lets 48 warps run on an SM where the loads are waited for (forward alone: 0.33
+// ms against 0.37 at 32 warps).
 template <typename T, typename I, Grad MODE, int TH>
 __global__ void __launch_bounds__(TH, MODE == Grad::kept ? 1024 / TH : 1536 / TH) distill_row_kernel(const DistillArgs a) {
   constexpr bool KEEP = MODE == Grad::kept;
@@ -559,9 +563,16 @@ template <typename T, typename I> void run_typed(const DistillCall &call, cudaSt
   }
   split(pick_slices(a.rows, row_bytes, kRereadMost, 8));
   const int64_t kept = a.slice * (int64_t)sizeof(T);
-  if (kept > kKeepMost)
-    return launch_rows(distill_row_kernel<T, I, Grad::reread, kRereadThreads>, a, kRereadThreads,
-                       (size_t)(ceil_div(a.slice, 128) * 16 + kBackwardTable * 8), s);
+  if (kept > kKeepMost) {
+    const int64_t smem = ceil_div(a.slice, 128) * 16 + kBackwardTable * 8;
+    if (smem <= kMaxKept)
+      return launch_rows(distill_row_kernel<T, I, Grad::reread, kRereadThreads>, a, kRereadThreads, (size_t)smem, s);
+    // a bit for each column of a slice does not fit (over 12 million columns): two passes
+    Scratch stats(sizeof(RowStats) * (size_t)a.rows, s);
+    a.stats = stats.as<RowStats>();
+    launch_rows(distill_row_kernel<T, I, Grad::none, kThreads>, a, kThreads, 0, s);
+    return backward();
+  }
   if (small) return launch_rows(distill_row_kernel<T, I, Grad::kept, 128>, a, 128, (size_t)kept, s);
   launch_rows(distill_row_kernel<T, I, Grad::kept, kThreads>, a, kThreads, (size_t)kept, s);
 }

@@ -10,9 +10,8 @@
 // tensor memory. Scores and output of a slot stay there (S 128 columns, O 128, two
 // slots: all 512). The probabilities, rounded to the inputs' type for the second
 // product (half a step each, against sums held in fp32), take the place of the
-// scores and are read from there as its left operand, the first 64 of a tile
-// while the softmax of the last 64 goes on. While one slot's softmax runs, the
-// other slot's products do.
+// scores and are read from there as its left operand. While one slot's softmax
+// runs, the other slot's products do.
 //
 // The running maximum is only raised when a row's new maximum is 2^8 above the
 // one in use, so the output is rescaled in tensor memory a few times at most;
@@ -24,8 +23,9 @@
 // something not finite hides among their tiles' other keys.
 //
 // Bound: the products (2 x 520 clocks for 128 x 128 scores at head size 128) and
-// the exponentials (16 a clock and SM: 1024 clocks, less a share that is computed
-// as polynomials on the FMA units) take about the same time, side by side.
+// the exponentials (16 a clock and SM: 1024 clocks) take about the same time, side by
+// side; beside a busy softmax a product takes about 700 clocks. 32768 tokens, window
+// 4096, 32 / 8 heads of 128, bf16: 2.0 ms, 1030 TFLOP/s.
 #include <algorithm>
 
 #include "window_tc.cuh"

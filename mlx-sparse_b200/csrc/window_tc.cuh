@@ -52,27 +52,6 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return d;
 }
 
-// 2^x of two numbers on the FMA and integer units, for x < 128; NaN stays NaN,
-// below -126 the result is 2^-126. x = n + f with n the nearest integer (read off
-// the low bits of x + 1.5 2^23) and |f| <= 1/2; 2^f is a polynomial of degree 4,
-// the minimax one for the relative error (2.6e-6, a hundredth of float16's half
-// rounding step), found by Remez' exchange.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
-  const float2 t = add2(x, make_float2(12582912.f, 12582912.f));
-  const float2 n = add2(t, make_float2(-12582912.f, -12582912.f));
-  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
-  float2 p = make_float2(9.570102207e-03f, 9.570102207e-03f);
-  p = fma2(p, f, make_float2(5.591785908e-02f, 5.591785908e-02f));
-  p = fma2(p, f, make_float2(2.402474433e-01f, 2.402474433e-01f));
-  p = fma2(p, f, make_float2(6.931217909e-01f, 6.931217909e-01f));
-  p = fma2(p, f, make_float2(9.999992847e-01f, 9.999992847e-01f));
-  const float2 scale = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
-                                   __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
-  return mul2(p, scale);
-}
-
 template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if (BF16) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);

@@ -106,13 +106,26 @@ def test_loss_and_gradient(ms, shape, dtype):
         _check(ms.csr_distillation_loss(teacher, leaf, temperature=T), loss, bar, "loss without a graph")
 
 
-@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 900001), (torch.bfloat16, 300007)])
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 900001), (torch.bfloat16, 300007), (torch.float16, 13000003)])
 def test_rows_beyond_one_sm(ms, dtype, vocab):
-    """A row over a cluster's shared memory (two passes) and one that needs all of it."""
+    """Rows that are read twice, and one too long for a bit a column in shared memory."""
     parts, logits = _case(2, vocab, 40, dtype, seed=3)
     teacher = ms.csr_array(parts, shape=(2, vocab))
     loss, bar, grad, gbar = _reference(parts, logits, 1.0, torch.ones(2, dtype=torch.float64))
     got, got_grad = ms.csr_distillation_loss_and_grad(teacher, logits)
+    _check(got, loss, bar, "loss")
+    _check(got_grad, grad, gbar, "gradient")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_rows_beyond_shared_memory(ms, dtype):
+    """More rows than SMs: a cluster of two that reads each half row again."""
+    rows, vocab = 400, 70001
+    parts, logits = _case(rows, vocab, 12, dtype, seed=9, empty=(0, 17))
+    teacher = ms.csr_array(parts, shape=(rows, vocab))
+    w = torch.linspace(0.5, 1.0, rows)
+    loss, bar, grad, gbar = _reference(parts, logits, 1.0, w.double())
+    got, got_grad = ms.csr_distillation_loss_and_grad(teacher, logits, cotangent=w.cuda())
     _check(got, loss, bar, "loss")
     _check(got_grad, grad, gbar, "gradient")
 
