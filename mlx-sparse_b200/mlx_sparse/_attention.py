@@ -64,14 +64,11 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, scale=None, indptr
             raise ValueError(
                 f"window_attention with indptr needs as many queries as keys, got {q.shape[0]} and {k.shape[0]}."
             )
-        q, k, v = q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         from mlx_sparse._autodiff import WindowAttention
 
-        out = WindowAttention.apply(q, k, v, window, sinks, scale, indptr)
-    else:
-        out = _native.window_attention_forward(q, k, v, window, sinks, scale, indptr, with_lse=False)[0]
-    return out if indptr is None else out.squeeze(0)
+        return WindowAttention.apply(q, k, v, window, sinks, scale, indptr)
+    return _native.window_attention_forward(q, k, v, window, sinks, scale, indptr, with_lse=False)[0]
 
 
 def window_attention_decode(q, k_cache, v_cache, lengths, *, window: int, sinks: int = 0, scale=None):

@@ -73,9 +73,9 @@ class CsrDistillation(torch.autograd.Function):
 
 
 class WindowAttention(torch.autograd.Function):
-    """Windowed attention on rank-4 operands, differentiable once in ``q``,
-    ``k`` and ``v``. Keeps the output, what its rounding took off, and each row's
-    log-sum-exp."""
+    """Windowed attention, batched (rank 4) or packed (rank 3), differentiable
+    once in ``q``, ``k`` and ``v``. Keeps the output, what its rounding took off,
+    and each row's log-sum-exp."""
 
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, scale, indptr):
@@ -88,8 +88,7 @@ class WindowAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         q, k, v, out, low, lse = ctx.saved_tensors
-        need_q, need_kv = ctx.needs_input_grad[0], any(ctx.needs_input_grad[1:3])
-        dq, dk, dv = _native.window_attention_backward(q, k, v, out, low, lse, grad, *ctx.args, want_q=need_q,
-                                                       want_kv=need_kv)
-        return (dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None,
-                None)
+        need = ctx.needs_input_grad
+        dq, dk, dv = _native.window_attention_backward(q, k, v, out, low, lse, grad, *ctx.args, want_q=need[0],
+                                                       want_kv=need[1] or need[2])
+        return dq, dk if need[1] else None, dv if need[2] else None, None, None, None, None

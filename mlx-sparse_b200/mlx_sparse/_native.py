@@ -655,14 +655,17 @@ def _window_args(q, k, v, window, sinks, scale, indptr):
 
 
 def window_attention_forward(q, k, v, window, sinks, scale, indptr=None, *, with_lse: bool):
-    """Rank-4 ``q``, ``k``, ``v``; returns ``(out, low, lse)``. ``low`` and
-    ``lse`` are for the backward call and None unless ``with_lse``: what rounding
-    ``out`` to a 16-bit type took off, and each row's log-sum-exp."""
+    """Rank-4 ``q``, ``k``, ``v``, or rank 3 with ``indptr``; returns ``(out, low,
+    lse)``. ``low`` and ``lse`` are for the backward call and None unless
+    ``with_lse``: what rounding ``out`` to a 16-bit type took off, and each row's
+    log-sum-exp."""
     L = extension()
     dev = require_cuda(q, k, v) if indptr is None else require_cuda(q, k, v, indptr)
+    out = q.new_empty(q.shape)  # of q's own rank: a view could not be changed in place under autograd
+    if indptr is not None:
+        indptr = indptr.contiguous()
+        q, k, v = q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)
     q, k, v = heads_of(q), heads_of(k), heads_of(v)
-    indptr = None if indptr is None else indptr.contiguous()
-    out = q.new_empty(q.shape)
     low = lse = None
     if with_lse:  # the kernels read whole tiles of lse
         low = q.new_empty(q.shape) if q.element_size() == 2 else None
@@ -677,15 +680,17 @@ def window_attention_backward(q, k, v, out, low, lse, grad, window, sinks, scale
                               want_kv=True):
     L = extension()
     dev = require_cuda(q, k, v, out, lse, grad)
+    dq = q.new_empty(q.shape) if want_q else None
+    dk, dv = (k.new_empty(k.shape), k.new_empty(k.shape)) if want_kv else (None, None)
+    if indptr is not None:
+        indptr = indptr.contiguous()
+        q, k, v = q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)
     q, k, v = heads_of(q), heads_of(k), heads_of(v)
-    indptr = None if indptr is None else indptr.contiguous()
     grad = heads_of(grad.contiguous())
     floats = ctypes.c_int64()
     check(L.msx_window_attention_workspace(*q.shape[:2], k.shape[1], q.shape[2], k.shape[2], q.shape[3], window, sinks,
                                            ctypes.byref(floats)))
     work = lse.new_empty(floats.value)
-    dq = q.new_empty(q.shape) if want_q else None
-    dk, dv = (k.new_empty(k.shape), k.new_empty(k.shape)) if want_kv else (None, None)
     args, _keep = _window_args(q, k, v, window, sinks, scale, indptr)
     with _on(dev):
         check(L.msx_window_attention_backward(*args, out.data_ptr(), _p(low), lse.data_ptr(), grad.data_ptr(), work.data_ptr(),

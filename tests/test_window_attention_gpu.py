@@ -276,6 +276,27 @@ def test_some_gradients_and_twice(ms, dtype):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_packed_gradients_one_at_a_time_and_output_in_place(ms, dtype):
+    q, k, v = (_rand((200, heads, 64), dtype, s) for heads, s in ((4, 1), (2, 2), (2, 3)))
+    g = _rand(q.shape, dtype, 4)
+    args = dict(window=33, sinks=2, indptr=torch.tensor([0, 90, 200], device="cuda"))
+    full = _all(ms, q, k, v, g, **args)
+    for pick in range(3):
+        leaves = [t.clone() for t in (q, k, v)]
+        leaves[pick].requires_grad_()
+        out = ms.window_attention(*leaves, **args)
+        out.backward(g)
+        assert torch.equal(out, full[0]) and torch.equal(leaves[pick].grad, full[1 + pick])
+        # the output is a tensor of its own, not a view that refuses to be changed
+        ms.window_attention(*leaves, **args).add_(1)
+    fused = _rand((200, 8, 64), dtype, 5)
+    parts = fused.split((4, 2, 2), 1)
+    want = _all(ms, *(t.contiguous() for t in parts), g, **args)
+    for x, y in zip(_all(ms, *parts, g, **args), want):
+        assert torch.equal(x, y)
+
+
 def test_gradient_against_differences(ms):
     """float32, along random directions. Each side's value is off by the
     forward's bar; the third derivative of sum(g * out) along a direction of
