@@ -54,41 +54,41 @@ class CsrProduct(torch.autograd.Function):
 class CsrDistillation(torch.autograd.Function):
     """Per-row distillation losses, differentiable once in the logits; the
     teacher is a constant. The forward pass keeps four numbers a row, the
-    backward pass reads the logits again."""
+    backward pass reads the logits and the teacher again (saved, so that writing
+    to either in between is an error)."""
 
     @staticmethod
-    def forward(ctx, logits, a, temperature):
-        loss, stats = _native.csr_distill_forward(a.data, a.indices, a.indptr, logits, temperature, with_stats=True)
-        ctx.a, ctx.temperature = a, temperature
-        ctx.save_for_backward(logits, stats)
+    def forward(ctx, logits, data, indices, indptr, temperature):
+        loss, stats = _native.csr_distill_forward(data, indices, indptr, logits, temperature, with_stats=True)
+        ctx.temperature = temperature
+        ctx.save_for_backward(logits, data, indices, indptr, stats)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        logits, stats = ctx.saved_tensors
-        a = ctx.a
-        return (_native.csr_distill_backward(a.data, a.indices, a.indptr, logits, ctx.temperature, stats, grad), None,
-                None)
+        logits, data, indices, indptr, stats = ctx.saved_tensors
+        return (_native.csr_distill_backward(data, indices, indptr, logits, ctx.temperature, stats, grad), None, None,
+                None, None)
 
 
 class WindowAttention(torch.autograd.Function):
     """Windowed attention, batched (rank 4) or packed (rank 3), differentiable
-    once in ``q``, ``k`` and ``v``. Keeps the output, what its rounding took off,
-    and each row's log-sum-exp."""
+    once in ``q``, ``k`` and ``v``. Keeps the operands, the boundaries, the output,
+    what its rounding took off, and each row's log-sum-exp."""
 
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, scale, indptr):
         out, low, lse = _native.window_attention_forward(q, k, v, window, sinks, scale, indptr, with_lse=True)
-        ctx.args = (window, sinks, scale, indptr)
-        ctx.save_for_backward(q, k, v, out, low, lse)
+        ctx.args = (window, sinks, scale)
+        ctx.save_for_backward(q, k, v, indptr, out, low, lse)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        q, k, v, out, low, lse = ctx.saved_tensors
+        q, k, v, indptr, out, low, lse = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dq, dk, dv = _native.window_attention_backward(q, k, v, out, low, lse, grad, *ctx.args, want_q=need[0],
+        dq, dk, dv = _native.window_attention_backward(q, k, v, out, low, lse, grad, *ctx.args, indptr, want_q=need[0],
                                                        want_kv=need[1] or need[2])
         return dq, dk if need[1] else None, dv if need[2] else None, None, None, None, None

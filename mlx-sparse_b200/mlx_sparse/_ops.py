@@ -226,7 +226,7 @@ def csr_distillation_loss(teacher: CSRArray, logits, *, temperature: float = 1.0
     if _wants_grad(logits):
         from mlx_sparse._autodiff import CsrDistillation
 
-        return CsrDistillation.apply(logits, teacher, float(temperature))
+        return CsrDistillation.apply(logits, teacher.data, teacher.indices, teacher.indptr, float(temperature))
     return _native.csr_distill_forward(teacher.data, teacher.indices, teacher.indptr, logits, temperature,
                                        with_stats=False)[0]
 
