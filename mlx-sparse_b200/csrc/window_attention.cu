@@ -286,9 +286,11 @@ template <typename K>
 void launch_general(K kernel, const WindowProblem &w, int64_t rows, int64_t heads, int staged, cudaStream_t s) {
   const int64_t blocks = ceil_div(rows, kRows);
   if (blocks == 0 || heads == 0 || w.c.batch == 0) return;
-  const size_t smem = sizeof(float) * ((size_t)2 * kTile * (w.c.dim + 1) + (size_t)staged * kRows * w.c.dim);
-  MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kernel<<<dim3((unsigned)blocks, (unsigned)heads, (unsigned)w.c.batch), kWarps * 32, smem, s>>>(w);
+  auto bytes = [&](int dim) { return sizeof(float) * ((size_t)2 * kTile * (dim + 1) + (size_t)staged * kRows * dim); };
+  // The attribute is the kernel's, not the launch's: what the largest head size
+  // needs, so that another thread's call cannot lower it before this launch.
+  MSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(kMaxDim)));
+  kernel<<<dim3((unsigned)blocks, (unsigned)heads, (unsigned)w.c.batch), kWarps * 32, bytes(w.c.dim), s>>>(w);
   MSX_CHECK_LAUNCH();
 }
 
