@@ -503,7 +503,10 @@ MSX_API int msx_csr_distill_forward_backward(
  * q_heads, q_len rounded up to a multiple of 128), 16-byte aligned, minus
  * the log-sum-exp in base 2, written by forward (null: not wanted), read by backward;
  * workspace: *floats of msx_window_attention_workspace, 16-byte aligned, for
- * backward alone. backward reads forward's out. */
+ * backward alone. lse or a workspace that is not 16-byte aligned is refused; the
+ * other arrays may lie anywhere (16-bit arrays that are not 16-byte aligned take
+ * the general kernels, which do not use the tensor cores). backward reads
+ * forward's out. */
 MSX_API int msx_window_attention_workspace(int64_t batch, int64_t q_len,
                                            int64_t k_len, int64_t q_heads,
                                            int64_t k_heads, int64_t dim,

@@ -672,6 +672,11 @@ static WindowCall window_checked(int value_dtype, const void *q, const int64_t *
   return c;
 }
 
+// The kernels read and write these in 16-byte pieces.
+static void check_aligned16(const void *p, const char *name) {
+  require(reinterpret_cast<uintptr_t>(p) % 16 == 0, MSX_ERR_INVALID, std::string(name) + " must be 16-byte aligned.");
+}
+
 static void window_packed(WindowCall &c, const void *indptr, int64_t n_seq) {
   if (indptr == nullptr) return;
   require(c.batch == 1 && c.q_len == c.k_len && n_seq >= 0, MSX_ERR_INVALID,
@@ -700,6 +705,7 @@ int msx_window_attention_forward(int value_dtype, const void *q, const int64_t *
                                   k_heads, dim, window, sinks, scale, index_dtype);
     window_packed(c, indptr, n_seq);
     check_ptr(out, batch * q_len, "window_attention out");
+    check_aligned16(lse, "window_attention lse");
     c.out = out, c.out_low = value_dtype == MSX_F32 ? nullptr : out_low, c.lse = lse;
     window_forward_run(value_dtype, c, as_stream(stream));
   });
@@ -720,6 +726,8 @@ int msx_window_attention_backward(int value_dtype, const void *q, const int64_t 
     check_ptr(lse, batch * q_len, "window_attention lse");
     check_ptr(grad_out, batch * q_len, "window_attention grad_out");
     check_ptr(workspace, batch * q_len, "window_attention workspace");
+    check_aligned16(lse, "window_attention lse");
+    check_aligned16(workspace, "window_attention workspace");
     require((dk == nullptr) == (dv == nullptr), MSX_ERR_INVALID, "window_attention dk and dv come together.");
     c.out_low = value_dtype == MSX_F32 ? nullptr : const_cast<void *>(out_low);
     c.out = const_cast<void *>(out), c.lse = const_cast<float *>(lse), c.grad_out = grad_out, c.delta = workspace;

@@ -13,6 +13,8 @@
 // run from shared memory and bound the kernel.
 #include "window_attention.cuh"
 
+#include <initializer_list>
+
 namespace msx {
 namespace {
 
@@ -344,9 +346,16 @@ int64_t window_backward_floats(const WindowCall &c) {
   return c.batch * c.q_heads * w.lse_row + window_backward_floats_tc(w);
 }
 
+// The tensor-core kernels write 16 bytes at a time; the general ones any element.
+static bool aligned16(std::initializer_list<const void *> outputs) {
+  uintptr_t at = 0;
+  for (const void *p : outputs) at |= reinterpret_cast<uintptr_t>(p);
+  return at % 16 == 0;
+}
+
 void window_forward_run(int value_dtype, const WindowCall &c, cudaStream_t s) {
   const WindowProblem w = problem(c);
-  if (window_tc_ok(w, value_dtype))
+  if (window_tc_ok(w, value_dtype) && aligned16({c.out, c.out_low}))
     window_forward_tc(w, value_dtype, s);
   else
     window_forward_general(w, value_dtype, s);
@@ -358,7 +367,7 @@ void window_decode_run(int value_dtype, const WindowCall &c, cudaStream_t s) {
 
 void window_backward_run(int value_dtype, const WindowCall &c, cudaStream_t s) {
   const WindowProblem w = problem(c);
-  if (window_tc_ok(w, value_dtype) && reinterpret_cast<uintptr_t>(c.grad_out) % 16 == 0)
+  if (window_tc_ok(w, value_dtype) && aligned16({c.grad_out, c.dq, c.dk, c.dv}))
     window_backward_tc(w, value_dtype, s);
   else
     window_backward_general(w, value_dtype, s);
