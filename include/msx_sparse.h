@@ -99,6 +99,11 @@ MSX_API int msx_check_device_errors(void *stream);
  * (default 2^22; 0 makes every wait give up at once; negative restores the
  * default). Process-wide. */
 MSX_API int msx_debug_set_spmv_poll_limit(int64_t polls);
+/* Test hook: the nanoseconds that a wait of the windowed-attention kernels goes
+ * on before giving up (default 2e10; 0: every barrier that is not passed already
+ * is given up; negative restores the default). Process-wide, for launches from
+ * then on. */
+MSX_API int msx_debug_set_window_wait_limit(int64_t ns);
 
 /* ------------------------------------------------------------------------ */
 /* SpMV plan: row-length bins of a CSR matrix.                              */

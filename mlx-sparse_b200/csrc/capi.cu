@@ -102,6 +102,10 @@ int msx_debug_set_spmv_poll_limit(int64_t polls) {
   return guarded([&] { spmv_set_poll_limit(polls); });
 }
 
+int msx_debug_set_window_wait_limit(int64_t ns) {
+  return guarded([&] { window_set_wait_limit(ns); });
+}
+
 int msx_spmv_plan_create(int index_dtype, const void *indptr, int64_t n_rows, int64_t nnz, void *stream,
                          msx_spmv_plan **out) {
   return guarded([&] {

@@ -81,6 +81,7 @@ void window_forward_run(int value_dtype, const WindowCall &c, cudaStream_t s);
 int64_t window_backward_floats(const WindowCall &c);
 void window_decode_run(int value_dtype, const WindowCall &c, cudaStream_t s);
 bool window_take_error();  // reads and clears the device's wait error flag
+void window_set_wait_limit(long long ns);  // negative: the default
 void window_backward_run(int value_dtype, const WindowCall &c, cudaStream_t s);
 
 }  // namespace msx

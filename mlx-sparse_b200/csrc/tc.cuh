@@ -30,37 +30,65 @@ __device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
   return ok != 0;
 }
 
-// A wait that gives up after `kWaitNs`, far beyond any run of these kernels: it
-// then sets the device's error flag and the CTA's `stop`, which makes every
-// other wait of the CTA give up too, so that all warps reach the kernel's end.
-constexpr unsigned long long kWaitNs = 20ull * 1000 * 1000 * 1000;
+__device__ __forceinline__ bool bar_test(uint64_t *bar, uint32_t parity) {  // does not wait
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(ok)
+               : "r"(smem_addr(bar)), "r"(parity)
+               : "memory");
+  return ok != 0;
+}
+
+// What a wait goes by: `polls` tries at once, then until `limit_ns` have passed,
+// far beyond any run of these kernels. A wait that gives up sets the device's
+// error flag and the CTA's `stop`, which makes every other wait of the CTA give up
+// too, so that all warps reach the kernel's end. A limit of 0 (for tests) gives up
+// wherever a barrier is not passed already.
+struct Watch {
+  int *error;
+  unsigned long long limit_ns;
+  int polls;
+};
+constexpr long long kWaitNs = 20ll * 1000 * 1000 * 1000;
+constexpr unsigned long long kSettleNs = 1000ull * 1000 * 1000;
 __device__ __forceinline__ unsigned long long now_ns() {
   unsigned long long t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
   return t;
 }
-static __device__ __noinline__ bool bar_wait_slow(uint64_t *bar, uint32_t parity, volatile int *stop, int *error) {
-  const unsigned long long begin = now_ns();
-  while (!bar_try(bar, parity)) {
+static __device__ __noinline__ bool bar_wait_slow(uint64_t *bar, uint32_t parity, volatile int *stop, const Watch *w) {
+  const unsigned long long begin = now_ns(), limit = w->limit_ns;
+  while (!(limit ? bar_try(bar, parity) : bar_test(bar, parity))) {
     if (*stop) return false;
-    if (now_ns() - begin > kWaitNs) {
+    if (now_ns() - begin >= limit) {
       *stop = 1;
-      *error = 1;
+      *w->error = 1;
       return false;
     }
   }
   return true;
 }
-__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile int *stop, int *error) {
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile int *stop, const Watch *w) {
 #pragma unroll 1
-  for (int i = 0; i < 64; ++i)
+  for (int i = 0; i < w->polls; ++i)
     if (bar_try(bar, parity)) return true;
-  return bar_wait_slow(bar, parity, stop, error);
+  return bar_wait_slow(bar, parity, stop, w);
 }
 
 // The same by a whole warp, which goes on or gives up as one.
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *stop, int *error) {
-  return __all_sync(~0u, bar_wait(bar, parity, stop, error));
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *stop, const Watch *w) {
+  return __all_sync(~0u, bar_wait(bar, parity, stop, w));
+}
+
+// After a wait gave up: copies and products that were issued end by themselves,
+// and must have ended before the CTA's memory goes away. Waits, whatever `stop`
+// says and a second at most, until the barrier has passed the phase `parity`. Of a
+// barrier that copies arrive at, that is the phase armed last: a bit that starts as
+// 1, which a new barrier has passed, and turns with each arming.
+static __device__ __noinline__ void bar_settle(uint64_t *bar, uint32_t parity) {
+  const unsigned long long begin = now_ns();
+  while (!bar_try(bar, parity) && now_ns() - begin < kSettleNs) {
+  }
 }
 
 // ---- TMA -----------------------------------------------------------------------

@@ -137,6 +137,5 @@ int64_t window_backward_floats_tc(const WindowProblem &w);  // workspace behind 
 // One query for each sequence (window_decode.cu).
 void window_decode(const WindowProblem &w, int value_dtype, cudaStream_t s);
 void window_delta(const WindowProblem &w, int value_dtype, cudaStream_t s);
-int *window_error_flag();
 
 }  // namespace msx

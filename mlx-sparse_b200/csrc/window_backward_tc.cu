@@ -59,7 +59,7 @@ struct Params {
   WindowProblem w;
   CUtensorMap q, k, v, g;
   int items, q_tiles;
-  int *error;
+  Watch watch;
   // far queries of the sinks: queries of a chunk (0: not cut), chunks, and sums
   // [batch][key head][chunk][sink][dV, dK][dim]
   int chunk, n_chunks;
@@ -167,16 +167,22 @@ __device__ __noinline__ void repair_dkv(const WindowProblem &w, int b, int hk, i
   }
 }
 
-__device__ __forceinline__ void drain(uint64_t *bars, int n) {
-  for (int s = 0; s < n; ++s)
-    for (int x = 0; x < (1 << 16) && !bar_try(&bars[s], 0) && !bar_try(&bars[s], 1); ++x) {
-    }
+// After a wait gave up, by all threads at the kernel's end: see bar_settle. The
+// phases armed last of the ring's barriers and of `once` are the bits of `armed`.
+__device__ __forceinline__ void settle(uint64_t *ring, uint64_t *once, uint64_t *idle, uint32_t armed) {
+  const int warp = (int)threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) bar_settle(&ring[s], armed >> s & 1);
+    bar_settle(once, armed >> kStages & 1);
+  }
+  if (warp == 1) mma_commit((threadIdx.x & 31) == 0, idle), bar_settle(idle, 0);
 }
+constexpr uint32_t kNoneArmed = (2u << kStages) - 1;  // the ring's barriers, then the other one
 
 // ---- dK and dV -------------------------------------------------------------------
 struct KvBars {
-  uint64_t kv_full, full[kStages], empty[kStages], s_full, dp_full, p_full, ds_full, done;
-  uint32_t tmem;
+  uint64_t kv_full, full[kStages], empty[kStages], s_full, dp_full, p_full, ds_full, done, idle;
+  uint32_t tmem, armed;
   int stop, last;
 };
 
@@ -220,7 +226,8 @@ __global__ void __launch_bounds__(threads_for(kKvCols), 1) dkv_tc_kernel(const _
     for (int s = 0; s < kStages; ++s) bar_init(&bars.full[s], 1), bar_init(&bars.empty[s], 1);
     bar_init(&bars.s_full, 1), bar_init(&bars.dp_full, 1), bar_init(&bars.done, 1);
     bar_init(&bars.p_full, 4 * kT / kCols), bar_init(&bars.ds_full, 4 * kT / kCols);
-    bars.stop = 0, bars.last = -1;
+    bar_init(&bars.idle, 1);
+    bars.stop = 0, bars.last = -1, bars.armed = kNoneArmed;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
@@ -260,6 +267,7 @@ __global__ void __launch_bounds__(threads_for(kKvCols), 1) dkv_tc_kernel(const _
   if (warp == 0) {
     if (lane == 0 && n > 0) {
       bar_expect(&bars.kv_full, 2 * kTile);
+      uint32_t armed = kNoneArmed ^ 1u << kStages;
       for (int x = 0; x < DB; ++x) {
         tma_load_4d(k_tile + x * kBox, &p.k, &bars.kv_full, x * 64, j0, hk, b);
         tma_load_4d(v_tile + x * kBox, &p.v, &bars.kv_full, x * 64, j0, hk, b);
@@ -270,7 +278,8 @@ __global__ void __launch_bounds__(threads_for(kKvCols), 1) dkv_tc_kernel(const _
         const int s = e % kStages, it = e >> 1;
         if (e > 0 && !(e & 1)) at_pair.next();
         const int h = at_pair.h, i0 = at_pair.t * kT;
-        if (!(ok = bar_wait(&bars.empty[s], (e / kStages & 1) ^ 1, stop, p.error))) break;
+        if (!(ok = bar_wait(&bars.empty[s], (e / kStages & 1) ^ 1, stop, &p.watch))) break;
+        armed ^= 1u << s;
         if (e & 1) {
           bar_expect(&bars.full[s], kTile);
         } else {
@@ -283,13 +292,14 @@ __global__ void __launch_bounds__(threads_for(kKvCols), 1) dkv_tc_kernel(const _
         for (int x = 0; x < DB; ++x)
           tma_load_4d(ring + s * kTile + x * kBox, e & 1 ? &p.g : &p.q, &bars.full[s], x * 64, i0, h, b);
       }
+      bars.armed = armed;
     }
   } else if (warp == 1) {
     if (n > 0) {
       const Products<DB, kCols> mm(BF16, w.c.dim);
       const uint32_t ka = smem_addr(k_tile), va = smem_addr(v_tile), ra = smem_addr(ring);
-      bool ok = warp_wait(&bars.kv_full, 0, stop, p.error);
-      auto ready = [&](int e) { return ok = ok && warp_wait(&bars.full[e % kStages], e / kStages & 1, stop, p.error); };
+      bool ok = warp_wait(&bars.kv_full, 0, stop, &p.watch);
+      auto ready = [&](int e) { return ok = ok && warp_wait(&bars.full[e % kStages], e / kStages & 1, stop, &p.watch); };
       auto tile = [&](int e) { return ra + (e % kStages) * kTile; };
       if (ready(0)) {
         fence_after();
@@ -302,7 +312,7 @@ __global__ void __launch_bounds__(threads_for(kKvCols), 1) dkv_tc_kernel(const _
       }
       for (int it = 0; ok && it < n; ++it) {
         const int q = 2 * it, g = q + 1;
-        if (!(ok = warp_wait(&bars.p_full, it & 1, stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.p_full, it & 1, stop, &p.watch))) break;
         fence_after();
         mm.sums(t_dv, t_s, tile(g), it > 0);
         mma_commit(mm.leader, &bars.empty[g % kStages]);
@@ -311,7 +321,7 @@ __global__ void __launch_bounds__(threads_for(kKvCols), 1) dkv_tc_kernel(const _
           mm.scores(t_s, ka, tile(q + 2));
           mma_commit(mm.leader, &bars.s_full);
         }
-        if (!(ok = warp_wait(&bars.ds_full, it & 1, stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.ds_full, it & 1, stop, &p.watch))) break;
         fence_after();
         mm.sums(t_dk, t_dp, tile(q), it > 0);
         mma_commit(mm.leader, &bars.empty[q % kStages]);
@@ -338,8 +348,8 @@ __global__ void __launch_bounds__(threads_for(kKvCols), 1) dkv_tc_kernel(const _
       const bool masked = !(i0 >= all_first && i0 + kCols - 1 <= all_last);
       const uint32_t seen = first_i > last_i ? 0 : bits(first_i - i0, last_i + 1 - i0, 0);
       // lse and delta came with Q's tile, which the products of s_full have read
-      if (!(ok = warp_wait(&bars.full[2 * it % kStages], 2 * it / kStages & 1, stop, p.error))) break;
-      if (!(ok = warp_wait(&bars.s_full, it & 1, stop, p.error))) break;
+      if (!(ok = warp_wait(&bars.full[2 * it % kStages], 2 * it / kStages & 1, stop, &p.watch))) break;
+      if (!(ok = warp_wait(&bars.s_full, it & 1, stop, &p.watch))) break;
       fence_after();
       float2 pr[kCols / 2];
       auto weights = [&](auto mask) {
@@ -374,7 +384,7 @@ __global__ void __launch_bounds__(threads_for(kKvCols), 1) dkv_tc_kernel(const _
       fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive(&bars.p_full);
-      if (!(ok = warp_wait(&bars.dp_full, it & 1, stop, p.error))) break;
+      if (!(ok = warp_wait(&bars.dp_full, it & 1, stop, &p.watch))) break;
       fence_after();
       auto grads = [&](auto mask) {
         uint32_t z[kCols], pk[kCols / 2];
@@ -408,7 +418,7 @@ __global__ void __launch_bounds__(threads_for(kKvCols), 1) dkv_tc_kernel(const _
       __syncwarp();
       if (lane == 0) bar_arrive(&bars.ds_full);
     }
-    if (ok && n > 0) ok = warp_wait(&bars.done, 0, stop, p.error);
+    if (ok && n > 0) ok = warp_wait(&bars.done, 0, stop, &p.watch);
     if (ok) {
       fence_after();
       // the first two warpgroups write dV, the others dK, half of the columns each
@@ -492,15 +502,15 @@ __global__ void __launch_bounds__(threads_for(kKvCols), 1) dkv_tc_kernel(const _
   fence_before();
   __syncthreads();
   fence_after();
-  if (threadIdx.x == 0 && *stop) drain(bars.full, kStages);
+  if (*stop) settle(bars.full, &bars.kv_full, &bars.idle, bars.armed);
   __syncthreads();
   if (warp == 1) tmem_free(tmem, 512);
 }
 
 // ---- dQ ---------------------------------------------------------------------------
 struct QBars {
-  uint64_t q_full, q_empty, full[kStages], empty[kStages], s_full[2], dp_full, ds_full, dq_full;
-  uint32_t tmem;
+  uint64_t q_full, q_empty, full[kStages], empty[kStages], s_full[2], dp_full, ds_full, dq_full, idle;
+  uint32_t tmem, armed;
   int stop;
 };
 
@@ -522,7 +532,8 @@ __global__ void __launch_bounds__(threads_for(kQCols<DB>), 1) dq_tc_kernel(const
     for (int s = 0; s < kStages; ++s) bar_init(&bars.full[s], 1), bar_init(&bars.empty[s], 1);
     bar_init(&bars.s_full[0], 1), bar_init(&bars.s_full[1], 1);
     bar_init(&bars.dp_full, 1), bar_init(&bars.ds_full, 4 * kT / kCols), bar_init(&bars.dq_full, 1);
-    bars.stop = 0;
+    bar_init(&bars.idle, 1);
+    bars.stop = 0, bars.armed = kNoneArmed;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(&bars.tmem, 512);
@@ -542,28 +553,31 @@ __global__ void __launch_bounds__(threads_for(kQCols<DB>), 1) dq_tc_kernel(const
   if (warp == 0) {
     if (lane == 0) {
       int stage = 0, b, h, i0;
-      uint32_t phase = 1, q_phase = 1;
+      uint32_t phase = 1, q_phase = 1, armed = kNoneArmed;
       bool ok = true;
       for (int x = blockIdx.x; ok && x < p.items; x += gridDim.x) {
         item(x, b, h, i0);
         const KeyTiles<kT> tiles(key_range(w, b, i0, i0 + kT - 1));
         if (tiles.n == 0) continue;
-        if (!(ok = bar_wait(&bars.q_empty, q_phase, stop, p.error))) break;
+        if (!(ok = bar_wait(&bars.q_empty, q_phase, stop, &p.watch))) break;
         q_phase ^= 1;
         bar_expect(&bars.q_full, 2 * kTile);
+        armed ^= 1u << kStages;
         for (int d = 0; d < DB; ++d) {
           tma_load_4d(q_tile + d * kBox, &p.q, &bars.q_full, d * 64, i0, h, b);
           tma_load_4d(g_tile + d * kBox, &p.g, &bars.q_full, d * 64, i0, h, b);
         }
         for (int e = 0; ok && e < 2 * tiles.n; ++e) {
-          if (!(ok = bar_wait(&bars.empty[stage], phase, stop, p.error))) break;
+          if (!(ok = bar_wait(&bars.empty[stage], phase, stop, &p.watch))) break;
           bar_expect(&bars.full[stage], kTile);
+          armed ^= 1u << stage;
           for (int d = 0; d < DB; ++d)
             tma_load_4d(ring + stage * kTile + d * kBox, e & 1 ? &p.v : &p.k, &bars.full[stage], d * 64,
                         tiles.first(e >> 1), h / w.group, b);
           if (++stage == kStages) stage = 0, phase ^= 1;
         }
       }
+      bars.armed = armed;
     }
   } else if (warp == 1) {
     {
@@ -573,7 +587,7 @@ __global__ void __launch_bounds__(threads_for(kQCols<DB>), 1) dq_tc_kernel(const
       uint32_t q_phase = 0;
       bool ok = true;
       auto ready = [&](uint32_t e) {
-        return ok = ok && warp_wait(&bars.full[e % kStages], e / kStages & 1, stop, p.error);
+        return ok = ok && warp_wait(&bars.full[e % kStages], e / kStages & 1, stop, &p.watch);
       };
       auto tile = [&](uint32_t e) { return ra + e % kStages * kTile; };
       auto s_at = [&](uint32_t t) { return tmem + (t & 1) * 128; };
@@ -582,7 +596,7 @@ __global__ void __launch_bounds__(threads_for(kQCols<DB>), 1) dq_tc_kernel(const
         item(x, b, h, i0);
         const KeyTiles<kT> tiles(key_range(w, b, i0, i0 + kT - 1));
         if (tiles.n == 0) continue;
-        if (!(ok = warp_wait(&bars.q_full, q_phase, stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.q_full, q_phase, stop, &p.watch))) break;
         q_phase ^= 1;
         auto scores = [&](uint32_t t) {
           if (!ready(2 * t)) return;
@@ -603,7 +617,7 @@ __global__ void __launch_bounds__(threads_for(kQCols<DB>), 1) dq_tc_kernel(const
         for (int t = 0; ok && t < tiles.n; ++t) {
           const uint32_t e = done + t;
           if (t + 1 < tiles.n) scores(e + 1);
-          if (!(ok = ok && warp_wait(&bars.ds_full, e & 1, stop, p.error))) break;
+          if (!(ok = ok && warp_wait(&bars.ds_full, e & 1, stop, &p.watch))) break;
           fence_after();
           mm.sums(t_dq, t_dp, tile(2 * e), t > 0);
           mma_commit(mm.leader, &bars.empty[2 * e % kStages]);
@@ -645,7 +659,7 @@ __global__ void __launch_bounds__(threads_for(kQCols<DB>), 1) dq_tc_kernel(const
 #pragma unroll
           for (int y = 0; y < kCols / 32; ++y) seen[y] = bits(b0, b1, y * 32) | bits(s0, s1, y * 32);
         }
-        if (!(ok = warp_wait(&bars.s_full[e & 1], e >> 1 & 1, stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.s_full[e & 1], e >> 1 & 1, stop, &p.watch))) break;
         fence_after();
         const uint32_t t_s = tmem + (e & 1) * 128 + lanes + part * kCols, t_d = t_dp + lanes + part * kCols;
         float2 pr[kCols / 2];
@@ -673,7 +687,7 @@ __global__ void __launch_bounds__(threads_for(kQCols<DB>), 1) dq_tc_kernel(const
           }
         };
         if (masked) weights(std::true_type{}); else weights(std::false_type{});
-        if (!(ok = warp_wait(&bars.dp_full, e & 1, stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.dp_full, e & 1, stop, &p.watch))) break;
         fence_after();
         auto grads = [&](auto mask) {
           uint32_t z[kCols], pk[kCols / 2];
@@ -709,7 +723,7 @@ __global__ void __launch_bounds__(threads_for(kQCols<DB>), 1) dq_tc_kernel(const
       if (!ok) break;
       done += tiles.n;
       if (tiles.n > 0) {
-        if (!(ok = warp_wait(&bars.dq_full, dq_phase, stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.dq_full, dq_phase, stop, &p.watch))) break;
         dq_phase ^= 1;
         fence_after();
       }
@@ -753,7 +767,7 @@ __global__ void __launch_bounds__(threads_for(kQCols<DB>), 1) dq_tc_kernel(const
   fence_before();
   __syncthreads();
   fence_after();
-  if (threadIdx.x == 0 && *stop) drain(bars.full, kStages);
+  if (*stop) settle(bars.full, &bars.q_full, &bars.idle, bars.armed);
   __syncthreads();
   if (warp == 1) tmem_free(tmem, 512);
 }
@@ -814,7 +828,7 @@ void window_backward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s)
   const int64_t items = w.c.batch * heads * p.q_tiles;
   if (items > INT32_MAX / 2) fail(MSX_ERR_OVERFLOW, "window_attention has too many queries and heads for one call.");
   p.items = (int)items;
-  p.error = window_error_flag();
+  p.watch = window_watch();
   p.chunk = pick_chunk(w);
   p.n_chunks = p.chunk ? (int)ceil_div(w.c.q_len, p.chunk) : 0;
   p.far = w.c.delta + w.c.batch * heads * w.lse_row;

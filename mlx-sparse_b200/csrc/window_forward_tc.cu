@@ -27,6 +27,7 @@
 // side; beside a busy softmax a product takes about 700 clocks. 32768 tokens, window
 // 4096, 32 / 8 heads of 128, bf16: 2.0 ms, 1030 TFLOP/s.
 #include <algorithm>
+#include <atomic>
 
 #include "window_tc.cuh"
 
@@ -44,8 +45,8 @@ constexpr int kThreads = 64 + 2 * 128;  // loads, products, two softmax warpgrou
 
 struct Bars {
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
-  uint64_t kv_full[8], step[8];
-  uint32_t tmem;
+  uint64_t kv_full[8], step[8], idle;
+  uint32_t tmem, armed;  // armed: the last phases of kv_full (bits 0-7) and q_full (8, 9), see bar_settle
   int stop;
   float max1[kM], sum1[kM];  // the second slot's, where both share the queries
 };
@@ -60,7 +61,7 @@ struct Params {
   WindowProblem w;
   CUtensorMap q, k, v;
   int items, q_tiles, paired;
-  int *error;
+  Watch watch;
 };
 
 // One work item: the two slots' heads and first queries, and the keys of each
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
   const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int *stop = &bars.stop;
   if (smem_addr(sm) % 1024 != 0) {  // the swizzle's atoms would not lie where they are read
-    *p.error = 1;
+    *p.watch.error = 1;
     return;
   }
   if (threadIdx.x == 0) {
@@ -190,6 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
     }
     for (int s = 0; s < Sh::stages; ++s) bar_init(&bars.kv_full[s], 1);
     for (int s = 0; s < 8; ++s) bar_init(&bars.step[s], 1);
+    bar_init(&bars.idle, 1);
     bars.stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -202,6 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
     // ---- loads -------------------------------------------------------------
     if (lane == 0) {
       uint32_t q_phase[2] = {1, 1};  // an empty barrier's first wait passes
+      uint32_t armed = 0xff;
       // Step g of all tiles so far frees V of tile g, K of tile g + 1 and, where that
       // is an item's first, K of tile g: an item's entries of the ring, K and V in
       // turn, are free after the steps t - 1 (0 for the first) and t. `freed`: the
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           if (it.last[s] < 0) continue;
-          ok = ok && bar_wait(&bars.q_empty[s], q_phase[s], stop, p.error);
+          ok = ok && bar_wait(&bars.q_empty[s], q_phase[s], stop, &p.watch);
           if (!ok) break;
           q_phase[s] ^= 1;
           bar_expect(&bars.q_full[s], Sh::tile);
@@ -228,9 +231,10 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         for (int t = 0; ok && t < tiles.n; ++t) {
           for (int kv = 0; kv < 2; ++kv) {
             const int64_t g = freed[stage];
-            if (g >= 0 && !(ok = bar_wait(&bars.step[g & 7], (uint32_t)(g >> 3 & 1), stop, p.error))) break;
+            if (g >= 0 && !(ok = bar_wait(&bars.step[g & 7], (uint32_t)(g >> 3 & 1), stop, &p.watch))) break;
             freed[stage] = base + (kv || t == 0 ? t : t - 1);
             bar_expect(&bars.kv_full[stage], Sh::tile);
+            armed ^= 1u << stage;
             for (int x = 0; x < DB; ++x)
               tma_load_4d(kv_tile + stage * Sh::tile + x * kBox, kv ? &p.v : &p.k, &bars.kv_full[stage], x * 64,
                           tiles.first(t), it.hk, it.b);
@@ -239,6 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         }
         base += tiles.n;
       }
+      bars.armed = armed | q_phase[0] << 8 | q_phase[1] << 9;
     }
   } else if (warp == 1) {
     // ---- products ------------------------------------------------------------
@@ -267,11 +272,11 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
 #pragma unroll
       for (int s = 0; s < 2; ++s)
         if (it.last[s] >= 0) {
-          need(warp_wait(&bars.q_full[s], q_phase[s], stop, p.error));
+          need(warp_wait(&bars.q_full[s], q_phase[s], stop, &p.watch));
           q_phase[s] ^= 1;
         }
       // the stage of K_0 is now, V_t and K_{t+1} follow in turn
-      if (!need(warp_wait(&bars.kv_full[stage], phase, stop, p.error))) break;
+      if (!need(warp_wait(&bars.kv_full[stage], phase, stop, &p.watch))) break;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
         if (takes(s, 0)) scores(s, stage, it.last[s] == 0);
@@ -284,16 +289,16 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
           // the slots take turns: the other one's scores before this one's output
           next();
           if (more) {
-            if (!need(warp_wait(&bars.kv_full[stage], phase, stop, p.error))) break;
+            if (!need(warp_wait(&bars.kv_full[stage], phase, stop, &p.watch))) break;
 #pragma unroll
             for (int s = 0; s < 2; ++s)
               if ((t & 1) != s) scores(s, stage, it.last[s] == t + 1);
           }
-          need(warp_wait(&bars.kv_full[v_stage], v_phase, stop, p.error));
+          need(warp_wait(&bars.kv_full[v_stage], v_phase, stop, &p.watch));
 #pragma unroll
           for (int s = 0; s < 2; ++s)
             if ((t & 1) == s) {
-              need(warp_wait(&bars.p_full[s], p_phase[s], stop, p.error));
+              need(warp_wait(&bars.p_full[s], p_phase[s], stop, &p.watch));
               fence_after();
               mm.sums(tmem + 256 + s * 128, tmem + s * kN, kv_addr + v_stage * Sh::tile, started[s]);
               if (t == it.last[s]) mma_commit(mm.leader, &bars.o_full[s]);
@@ -304,21 +309,21 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
           if (more) next();
           continue;
         }
-        if (!need(warp_wait(&bars.kv_full[stage], phase, stop, p.error))) break;
+        if (!need(warp_wait(&bars.kv_full[stage], phase, stop, &p.watch))) break;
         next();
         const int k_stage = stage;
         const bool now[2] = {takes(0, t), takes(1, t)}, then[2] = {more && takes(0, t + 1), more && takes(1, t + 1)};
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           if (now[s]) {
-            need(warp_wait(&bars.p_full[s], p_phase[s], stop, p.error));
+            need(warp_wait(&bars.p_full[s], p_phase[s], stop, &p.watch));
             fence_after();
             mm.sums(tmem + 256 + s * 128, tmem + s * kN, kv_addr + v_stage * Sh::tile, started[s]);
             if (t == it.last[s]) mma_commit(mm.leader, &bars.o_full[s]);
             p_phase[s] ^= 1;
             started[s] = true;
           }
-          if (s == 0 && more) need(warp_wait(&bars.kv_full[k_stage], phase, stop, p.error));
+          if (s == 0 && more) need(warp_wait(&bars.kv_full[k_stage], phase, stop, &p.watch));
           if (then[s]) scores(s, k_stage, it.last[s] == t + 1);
         }
         mma_commit(mm.leader, &bars.step[steps++ & 7]);
@@ -346,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
       bool started = false;
       for (int t = 0; ok && t < tiles.n; ++t) {
         if (SPLIT ? (t & 1) != s : !p.paired && !range.touches(tiles.first(t), tiles.end(t))) continue;
-        if (!(ok = warp_wait(&bars.s_full[s], s_phase, stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.s_full[s], s_phase, stop, &p.watch))) break;
         fence_after();
         const int j0 = tiles.first(t), j1 = tiles.end(t);
         const bool masked = !(j0 >= all_low && j0 + kN <= all_end && j1 - j0 >= kN);
@@ -429,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (s == 1 || !ok) break;
         if (it.last[1] >= 0) {
-          if (!(ok = warp_wait(&bars.o_full[1], 0, stop, p.error))) break;
+          if (!(ok = warp_wait(&bars.o_full[1], 0, stop, &p.watch))) break;
           const float m1 = bars.max1[row], top = fmaxf(m, m1);
           keep0 = m == -INFINITY ? 0.f : exp2_fast((m - top) * c);
           keep1 = m1 == -INFINITY ? 0.f : exp2_fast((m1 - top) * c);
@@ -438,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
       }
       if (!ok) break;
       if (started) {
-        if (!(ok = warp_wait(&bars.o_full[s], o_phase, stop, p.error))) break;
+        if (!(ok = warp_wait(&bars.o_full[s], o_phase, stop, &p.watch))) break;
         o_phase ^= 1;
         fence_after();
       }
@@ -506,10 +511,13 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
   fence_before();
   __syncthreads();
   fence_after();
-  if (threadIdx.x == 0 && *stop)  // a wait gave up: let copies in flight land before the memory goes away
-    for (int s = 0; s < Sh::stages; ++s)
-      for (int x = 0; x < (1 << 16) && !bar_try(&bars.kv_full[s], 0) && !bar_try(&bars.kv_full[s], 1); ++x) {
-      }
+  if (*stop) {
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < Sh::stages; ++s) bar_settle(&bars.kv_full[s], bars.armed >> s & 1);
+      for (int s = 0; s < 2; ++s) bar_settle(&bars.q_full[s], bars.armed >> (8 + s) & 1);
+    }
+    if (warp == 1) mma_commit(lane == 0, &bars.idle), bar_settle(&bars.idle, 0);
+  }
   __syncthreads();
   if (warp == 1) tmem_free(tmem, 512);
 }
@@ -529,11 +537,17 @@ template <typename T, int DB> void launch(Params &p, bool split, cudaStream_t s)
 
 }  // namespace
 
-int *window_error_flag() {
-  int *ptr = nullptr;
-  MSX_CUDA(cudaGetSymbolAddress(reinterpret_cast<void **>(&ptr), g_window_error));
-  return ptr;
+static std::atomic<long long> g_wait_ns{kWaitNs};
+
+Watch window_watch() {
+  Watch w{};
+  MSX_CUDA(cudaGetSymbolAddress(reinterpret_cast<void **>(&w.error), g_window_error));
+  w.limit_ns = (unsigned long long)g_wait_ns.load(std::memory_order_relaxed);
+  w.polls = w.limit_ns ? 64 : 0;
+  return w;
 }
+
+void window_set_wait_limit(long long ns) { g_wait_ns.store(ns < 0 ? kWaitNs : ns, std::memory_order_relaxed); }
 
 bool window_take_error() {
   int v = 0;
@@ -568,7 +582,7 @@ void window_forward_tc(const WindowProblem &w, int value_dtype, cudaStream_t s) 
                                  : w.c.batch * w.c.q_heads * ((p.q_tiles + 1) / 2);
   if (items > INT32_MAX / 2) fail(MSX_ERR_OVERFLOW, "window_attention has too many queries and heads for one call.");
   p.items = (int)items;
-  p.error = window_error_flag();
+  p.watch = window_watch();
   if (bf16) {
     if (w.c.dim <= 64) launch<__nv_bfloat16, 1>(p, split, s); else launch<__nv_bfloat16, 2>(p, split, s);
   } else {

@@ -162,6 +162,8 @@ template <typename T> __device__ inline bool row_not_finite(const T *p, int64_t 
 }
 
 // ---- host ---------------------------------------------------------------------
+tc::Watch window_watch();  // the current device's error flag and the limit of waits (window_forward_tc.cu)
+
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void *f = nullptr;

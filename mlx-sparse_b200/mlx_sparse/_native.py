@@ -74,6 +74,7 @@ def extension():
         L.msx_csr_diagonal.argtypes = [c_int, c_int, p, p, p, i64, i64, i64, p, p]
         L.msx_check_device_errors.argtypes = [p]
         L.msx_debug_set_spmv_poll_limit.argtypes = [i64]
+        L.msx_debug_set_window_wait_limit.argtypes = [i64]
         L.msx_coo_tocsr.argtypes = [c_int, c_int, p, p, p, i64, i64, i64, c_int, p, p, p, p, p]
         L.msx_csr_transpose.argtypes = [c_int, c_int, p, p, p, i64, i64, i64, p, p, p, p, p]
         L.msx_csr_matvec_transpose.argtypes = [c_int, c_int, p, p, p, i64, p, p, i64, i64, p]
