@@ -37,6 +37,12 @@
 // A masked P or dS is 0, but 0 times an infinity or NaN in a hidden row of dO, Q
 // or K would reach the sums: rows that end not finite while something not finite
 // hides in their tiles are computed again pair by pair.
+//
+// float16: dS is beyond the type's range where loss-scaled gradients of a few
+// thousand meet few keys, while dQ and dK need not be. A row with such a dS ends
+// not finite with finite log-sum-exp and delta, and is computed again in fp32 like
+// those above. (A factor on dS before it is rounded would move the range's other
+// end: gradients of 1e-5 already have dS among float16's smallest steps.)
 #include <algorithm>
 
 #include "window_tc.cuh"
@@ -98,9 +104,16 @@ template <typename T> struct PairDots {
   }
   __device__ void weights(const WindowProblem &w, float lse, float delta, float &p, float &ds) const {
     float s = 0.f, dp = 0.f;
-    for (int d = 0; d < w.c.dim; ++d) {
-      s = fmaf(VT<T>::load(q[d]), VT<T>::load(k[d]), s);
-      dp = fmaf(VT<T>::load(g[d]), VT<T>::load(v[d]), dp);
+    for (int d = 0; d < w.c.dim; d += 8) {  // 16 bytes of each row
+      alignas(16) T x[4][8];
+      const T *rows[4] = {q, k, g, v};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) *reinterpret_cast<uint4 *>(x[r]) = *reinterpret_cast<const uint4 *>(rows[r] + d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s = fmaf(VT<T>::load(x[0][e]), VT<T>::load(x[1][e]), s);
+        dp = fmaf(VT<T>::load(x[2][e]), VT<T>::load(x[3][e]), dp);
+      }
     }
     p = exp2f(s * (w.c.scale * kLog2e) + lse);
     ds = p * (dp + delta);
@@ -120,6 +133,7 @@ __device__ __noinline__ void repair_dq(const WindowProblem &w, int b, int h, int
     for (int j0 = from; j0 < end; j0 += 32) {
       float p = 0.f, ds = 0.f;
       if (j0 + lane < end) PairDots<T>(w, b, h, i, j0 + lane).weights(w, lse, delta, p, ds);
+#pragma unroll 8  // loads in flight
       for (int x = 0; x < min(32, end - j0); ++x) {
         const float e = __shfl_sync(~0u, ds, x);
         const T *k = PairDots<T>(w, b, h, i, j0 + x).k;
@@ -149,6 +163,7 @@ __device__ __noinline__ void repair_dkv(const WindowProblem &w, int b, int hk, i
       float p = 0.f, ds = 0.f;
       if (i + lane < i1)
         PairDots<T>(w, b, h, i + lane, j).weights(w, w.c.lse[at + i + lane], w.c.delta[at + i + lane], p, ds);
+#pragma unroll 8  // loads in flight
       for (int x = 0; x < min(32, i1 - i); ++x) {
         const float e = __shfl_sync(~0u, keys ? ds : p, x);
         const PairDots<T> pair(w, b, h, i + x, j);
@@ -494,6 +509,14 @@ __global__ void __launch_bounds__(threads_for(kKvCols), 1) dkv_tc_kernel(const _
           for (int h = hk * w.group; h < (hk + 1) * w.group; ++h)
             look_at(h, (most - 1) / kT * kT, 0, stop_i > 0 ? stop_i - 1 : INT_MAX);
         if (stop_i > 0 && stop_i < most) hidden = true;
+        if (!BF16 && half && bad && inside && !hidden) {  // as in dQ, of all queries that see the key
+          hidden = true;
+          for (int h = hk * w.group; hidden && h < (hk + 1) * w.group; ++h) {
+            const int64_t at = ((int64_t)b * w.c.q_heads + h) * w.lse_row;
+            for (int i = max(0, first_i); hidden && i <= last_i; ++i)
+              hidden = isfinite(w.c.lse[at + i]) && isfinite(w.c.delta[at + i]);
+          }
+        }
         for (unsigned left = __ballot_sync(~0u, bad && inside && hidden); left; left &= left - 1)
           repair_dkv<T>(w, b, hk, key - lane + __ffs(left) - 1, half != 0, d0, d0 + DB * 32);
       }
@@ -746,7 +769,8 @@ __global__ void __launch_bounds__(threads_for(kQCols<DB>), 1) dq_tc_kernel(const
         bad = store32<T>(dq, (int64_t)w.c.q_heads * w.c.dim, o, w.c.scale, d, w.c.dim, (int)w.c.q_len - (i - lane)) || bad;
       }
       if (__any_sync(~0u, bad && inside)) {
-        bool hidden = false;
+        // float16: the row's own numbers are finite, a dS was beyond the type's range
+        bool hidden = !BF16 && isfinite(lse) && isfinite(delta);
         const PairDots<T> pair(w, b, h, 0, 0);
         for (int t = 0; t < tiles.n; ++t) {
           const int j0 = tiles.first(t);

@@ -38,10 +38,12 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, scale=None, indptr
     ``h // (q_heads // k_heads)``. float32, float16 or bfloat16, head sizes up
     to 256; sums and the softmax are held in float32. 16-bit inputs with a head
     size that is a multiple of 8 up to 128 run on the tensor cores; these round
-    the probabilities to the inputs' type before the second product. ``scale``
-    defaults to ``dim ** -0.5``. Inputs may be strided views; a view whose last
-    dimension is strided, or whose 16-bit rows do not start on 16-byte
-    boundaries, is copied first.
+    the probabilities ``p``, and in the backward pass ``p * (dp - delta)`` too, to
+    the inputs' type before the products that sum them (in float32). float16 rows
+    where the latter is beyond the type's range are computed again in float32, which
+    takes longer. ``scale`` defaults to ``dim ** -0.5``. Inputs may be strided
+    views; a view whose last dimension is strided, or whose 16-bit rows do not
+    start on 16-byte boundaries, is copied first.
 
     Differentiable (once) in ``q``, ``k`` and ``v``. A training step can be captured
     into a CUDA graph under torch's rule for it: no eager graph of the same leaves
