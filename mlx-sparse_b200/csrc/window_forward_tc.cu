@@ -336,6 +336,10 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const uint32_t t_s = tmem + s * kN + lanes, t_o = tmem + 256 + s * 128 + lanes;
     const float c = w.c.scale * kLog2e;
+    // What the exponents of a maximum are taken over. Weights of two maxima are
+    // joined by the difference of these rounded products, in which their rounding,
+    // |c m| 2^-24, cancels (as it would not in c times the difference).
+    auto over = [&](float max) { return __fmul_rn(max, c); };
     uint32_t s_phase = 0, o_phase = 0;
     bool ok = true;
     for (int n = blockIdx.x; ok && n < p.items; n += gridDim.x) {
@@ -359,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         // Scores of the tile: their maximum and, with EXP, their exponentials over the
         // maximum in use, packed, and their sum.
         auto tile = [&](auto exp, auto mask) {
-          const float base = m == -INFINITY ? 0.f : m * c;
+          const float base = m == -INFINITY ? 0.f : over(m);
           const float2 base2 = make_float2(-base, -base), c2 = make_float2(c, c);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         float2 r = !started ? tile(no, yes) : masked ? tile(yes, yes) : tile(yes, no);
         const bool raise = (r.x - m) * c > 8.f;
         if (!started || __any_sync(~0u, raise)) {
-          const float keep = raise ? (m == -INFINITY ? 0.f : exp2_fast((m - r.x) * c)) : 1.f;
+          const float keep = raise ? (m == -INFINITY ? 0.f : exp2_fast(over(m) - over(r.x))) : 1.f;
           l *= keep;
           if (raise) m = r.x;
           if (started) {  // the tiles before are in the output: these scores were computed after them
@@ -436,8 +440,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         if (it.last[1] >= 0) {
           if (!(ok = warp_wait(&bars.o_full[1], 0, stop, &p.watch))) break;
           const float m1 = bars.max1[row], top = fmaxf(m, m1);
-          keep0 = m == -INFINITY ? 0.f : exp2_fast((m - top) * c);
-          keep1 = m1 == -INFINITY ? 0.f : exp2_fast((m1 - top) * c);
+          keep0 = m == -INFINITY ? 0.f : exp2_fast(over(m) - over(top));
+          keep1 = m1 == -INFINITY ? 0.f : exp2_fast(over(m1) - over(top));
           l = l * keep0 + bars.sum1[row] * keep1, m = top;
         }
       }
@@ -485,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_tc_kernel(const __grid_co
         }
       }
       if (inside && w.c.lse)
-        w.c.lse[((int64_t)it.b * w.c.q_heads + h) * w.lse_row + i] = empty ? -INFINITY : -(m * c + log2f(l));
+        w.c.lse[((int64_t)it.b * w.c.q_heads + h) * w.lse_row + i] = empty ? -INFINITY : -(over(m) + log2f(l));
       if (__any_sync(~0u, bad && inside)) {
         // What the row sees may be at fault; recompute it only if something not
         // finite hides among the tiles' other keys.
