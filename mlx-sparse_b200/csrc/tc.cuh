@@ -69,6 +69,7 @@ static __device__ __noinline__ bool bar_wait_slow(uint64_t *bar, uint32_t parity
   return true;
 }
 __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile int *stop, const Watch *w) {
+  if (bar_test(bar, parity)) return true;
 #pragma unroll 1
   for (int i = 0; i < w->polls; ++i)
     if (bar_try(bar, parity)) return true;
