@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from mlx_sparse import _native
-from mlx_sparse._validation import check_index_dtype, check_rank1, ensure_array, validate_window_inputs
+from mlx_sparse._validation import check_index_dtype, check_rank1, ensure_array, refuse_tangents, validate_window_inputs
 
 
 def window_attention(q, k, v, *, window: int, sinks: int = 0, scale=None, indptr=None):
@@ -45,10 +45,12 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, scale=None, indptr
     views; a view whose last dimension is strided, or whose 16-bit rows do not
     start on 16-byte boundaries, is copied first.
 
-    Differentiable (once) in ``q``, ``k`` and ``v``. A training step can be captured
+    Differentiable (once, in reverse mode; inputs with forward-mode tangents are
+    refused) in ``q``, ``k`` and ``v``. A training step can be captured
     into a CUDA graph under torch's rule for it: no eager graph of the same leaves
     may be alive meanwhile.
     """
+    refuse_tangents("window_attention", q, k, v)
     q = ensure_array(q)
     k, v = ensure_array(k, device=q.device), ensure_array(v, device=q.device)
     if indptr is None:
@@ -83,12 +85,13 @@ def window_attention_decode(q, k_cache, v_cache, lengths, *, window: int, sinks:
     ``lengths`` (batch,) int32 or int64 is read on the device and clamped to
     ``[0, max_len]``; a sequence of length 0 gets zeros. Only the window and the
     sink tokens are read. Types, heads and scale as ``window_attention``. Not
-    differentiable: it refuses inputs that require a gradient.
+    differentiable: it refuses inputs that require a gradient or carry a tangent.
     """
+    name = "window_attention_decode"
+    refuse_tangents(name, q, k_cache, v_cache)
     q = ensure_array(q)
     k_cache, v_cache = ensure_array(k_cache, device=q.device), ensure_array(v_cache, device=q.device)
     lengths = ensure_array(lengths, device=q.device)
-    name = "window_attention_decode"
     if q.ndim != 3 or k_cache.ndim != 4 or v_cache.ndim != 4:
         raise ValueError(f"{name} expects q of rank 3 and caches of rank 4, got {q.ndim}, {k_cache.ndim} and "
                          f"{v_cache.ndim}.")

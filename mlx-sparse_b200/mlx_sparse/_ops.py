@@ -16,6 +16,7 @@ from mlx_sparse._coo import COOArray
 from mlx_sparse._csr import CSRArray
 from mlx_sparse._validation import (
     ensure_array,
+    refuse_tangents,
     validate_csr_matmul_inputs,
     validate_csr_matvec_inputs,
     validate_distillation_inputs,
@@ -214,13 +215,15 @@ def csr_distillation_loss(teacher: CSRArray, logits, *, temperature: float = 1.0
     terms of their own. Entries with ``-inf`` teacher logits add nothing. A
     column outside the vocabulary makes its row's loss NaN.
 
-    Differentiable (once) in ``logits``; the teacher is a constant. ``logits``
+    Differentiable (once, in reverse mode; forward-mode tangents are refused) in
+    ``logits``; the teacher is a constant. ``logits``
     may have any row stride; a stride other than 1 along the vocabulary is
     copied. Use ``csr_distillation_loss_and_grad`` where the losses' weights
     are known beforehand: it reads the logits once instead of twice.
     """
     if not isinstance(teacher, CSRArray):
         raise TypeError(f"csr_distillation_loss expects CSRArray, got {type(teacher).__name__}.")
+    refuse_tangents("csr_distillation_loss", teacher.data, logits)
     logits = ensure_array(logits, device=teacher.device)
     validate_distillation_inputs(teacher.data, teacher.indices, teacher.indptr, logits, teacher.shape, temperature)
     if _wants_grad(logits):
@@ -239,6 +242,7 @@ def csr_distillation_loss_and_grad(teacher: CSRArray, logits, *, cotangent=None,
     gradient 0 whatever its logits hold. No autograd graph is recorded."""
     if not isinstance(teacher, CSRArray):
         raise TypeError(f"csr_distillation_loss_and_grad expects CSRArray, got {type(teacher).__name__}.")
+    refuse_tangents("csr_distillation_loss_and_grad", teacher.data, logits, cotangent)
     logits = ensure_array(logits, device=teacher.device).detach()
     validate_distillation_inputs(teacher.data, teacher.indices, teacher.indptr, logits, teacher.shape, temperature)
     if cotangent is not None:

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 VALUE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 INDEX_DTYPES = (torch.int32, torch.int64)
@@ -151,6 +152,20 @@ def validate_csr_matmul_inputs(data, indices, indptr, rhs, shape) -> None:
             "csr_matmul requires sparse data and RHS to have the same dtype, "
             f"got {_dtype_name(data.dtype)} and {_dtype_name(rhs.dtype)}."
         )
+
+
+# The level of forward-mode differentiation, -1 where there is none: then no tensor
+# has a tangent, and none is asked for one.
+_NO_LEVEL = -1
+
+
+def refuse_tangents(name: str, *tensors) -> None:
+    """The kernels compute no forward-mode derivatives: a tangent would be lost without a word."""
+    if getattr(forward_ad, "_current_level", 0) == _NO_LEVEL:
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} has no forward-mode derivative; use the reverse mode, or pass the primal alone.")
 
 
 def validate_distillation_inputs(data, indices, indptr, logits, shape, temperature) -> None:
