@@ -229,49 +229,67 @@ template <typename T> struct SliceShape {
 // Subtracts the teacher's probabilities from the gradient of columns [c0, c1):
 // the gradient of every entry's column is recomputed and rounded once. `bits`
 // (a bit for each column) finds columns that occur twice; only then the
-// probabilities are added up in `table`, as integers of 2^-62 so that their
-// order does not matter, `table_n` columns at a time.
+// probabilities are added up in `table`, some columns at a time and only those near
+// a column that occurred twice: as integers, so that their order does not matter,
+// of a step that follows the largest probability of the column, 2^52 or so steps
+// for a thousand entries, so that sums of small ones keep fp32's accuracy.
+constexpr int kSumBytes = 12;  // of the table for each column: the sum and the largest term
+
 template <typename T, typename I>
 __device__ void subtract_teacher(const DistillArgs &a, const T *z, T *g, int64_t lo, int64_t hi, int64_t c0,
-                                 int64_t c1, const RowStats &st, float scale, uint32_t *bits,
-                                 unsigned long long *table, int64_t table_n) {
+                                 int64_t c1, const RowStats &st, float scale, uint32_t *bits, void *table,
+                                 int64_t table_bytes) {
+  __shared__ uint32_t near_twice[2];  // blocks of columns, modulo 64, with one that occurs twice
   const T *t = static_cast<const T *>(a.t_data);
   const I *idx = static_cast<const I *>(a.t_idx);
+  const int64_t n = table_bytes / kSumBytes;
+  unsigned long long *sum = static_cast<unsigned long long *>(table);
+  uint32_t *top = reinterpret_cast<uint32_t *>(sum + n);
   const int words = (int)((c1 - c0 + 31) / 32);
   for (int w = threadIdx.x; w < words; w += blockDim.x) bits[w] = 0;
+  if (threadIdx.x < 2) near_twice[threadIdx.x] = 0;
   __syncthreads();  // also: the gradient of this slice is written
+  auto p_of = [&](int64_t e) { return exp2_fast(fmaf(VT<T>::load(t[e]), a.c, -st.t_max)) * st.t_inv; };
+  auto put = [&](int64_t col, float p) {
+    const float q = exp2_fast(fmaf(VT<T>::load(z[col]), a.c, -st.z_max)) * st.z_inv;
+    g[col] = VT<T>::store((q - p) * scale);
+  };
   int twice = 0;
   for (int64_t e = lo + threadIdx.x; e < hi; e += blockDim.x) {
     const int64_t col = (int64_t)idx[e];
     if (col < c0 || col >= c1) continue;
     const uint32_t bit = 1u << ((col - c0) & 31);
-    twice |= (atomicOr(&bits[(col - c0) >> 5], bit) & bit) != 0;
-    const float p = exp2_fast(fmaf(VT<T>::load(t[e]), a.c, -st.t_max)) * st.t_inv;
-    const float q = exp2_fast(fmaf(VT<T>::load(z[col]), a.c, -st.z_max)) * st.z_inv;
-    g[col] = VT<T>::store((q - p) * scale);
+    if (atomicOr(&bits[(col - c0) >> 5], bit) & bit) {
+      const int64_t block = (col - c0) / n;
+      twice = 1;
+      atomicOr(&near_twice[block >> 5 & 1], 1u << (block & 31));
+    }
+    put(col, p_of(e));
   }
-  if (!__syncthreads_or(twice)) return;
-  for (int64_t b0 = c0; b0 < c1; b0 += table_n) {
-    const int64_t b1 = min(c1, b0 + table_n);
-    for (int64_t j = threadIdx.x; j < b1 - b0; j += blockDim.x) table[j] = 0;
+  if (!__syncthreads_or(twice) || !isfinite(st.t_inv)) return;  // a row of NaN keeps the NaN that is there
+  const int steps = 62 - (64 - __clzll(hi - lo));  // all entries' terms, each below 2^steps, fit 62 bits
+  int64_t block = 0;
+  for (int64_t b0 = c0; b0 < c1; b0 += n, ++block) {
+    if (!(near_twice[block >> 5 & 1] >> (block & 31) & 1)) continue;
+    const int64_t b1 = min(c1, b0 + n);
+    auto each = [&](auto f) {
+      for (int64_t e = lo + threadIdx.x; e < hi; e += blockDim.x) {
+        const int64_t col = (int64_t)idx[e];
+        if (col >= b0 && col < b1) f(col, (int)(col - b0), p_of(e));
+      }
+      __syncthreads();
+    };
+    for (int64_t j = threadIdx.x; j < b1 - b0; j += blockDim.x) sum[j] = 0, top[j] = 0;
     __syncthreads();
-    for (int64_t e = lo + threadIdx.x; e < hi; e += blockDim.x) {
-      const int64_t col = (int64_t)idx[e];
-      if (col < b0 || col >= b1) continue;
-      const float p = exp2_fast(fmaf(VT<T>::load(t[e]), a.c, -st.t_max)) * st.t_inv;
-      atomicAdd(&table[col - b0], __float2ull_rn(p * 4611686018427387904.f));
-    }
-    __syncthreads();
-    for (int64_t e = lo + threadIdx.x; e < hi; e += blockDim.x) {
-      const int64_t col = (int64_t)idx[e];
-      if (col < b0 || col >= b1) continue;
-      // a NaN teacher row keeps the NaN that the first pass wrote
-      const float p1 = exp2_fast(fmaf(VT<T>::load(t[e]), a.c, -st.t_max)) * st.t_inv;
-      const float p = isnan(p1) ? p1 : __ull2float_rn(table[col - b0]) * 2.1684043449710089e-19f;
-      const float q = exp2_fast(fmaf(VT<T>::load(z[col]), a.c, -st.z_max)) * st.z_inv;
-      g[col] = VT<T>::store((q - p) * scale);
-    }
-    __syncthreads();
+    each([&](int64_t, int j, float p) { atomicMax(&top[j], __float_as_uint(p)); });
+    each([&](int64_t, int j, float p) {
+      const float most = __uint_as_float(top[j]);  // below 2^(ilogb + 1)
+      if (most > 0.f) atomicAdd(&sum[j], __double2ull_rn(ldexp((double)p, steps - 1 - ilogbf(most))));
+    });
+    each([&](int64_t col, int j, float) {
+      const float most = __uint_as_float(top[j]);
+      put(col, most > 0.f ? (float)ldexp((double)sum[j], ilogbf(most) + 1 - steps) : 0.f);
+    });
   }
 }
 
@@ -314,7 +332,7 @@ constexpr int kGroups = 4;  // commit groups of a slice: the sums start when the
 // pass alone), or the gradient, from the slice in shared memory or from a second
 // read of it.
 enum class Grad { none, kept, reread };
-constexpr int kBackwardTable = 1024;  // columns at a time of repeated entries' sums
+constexpr int kTableBytes = 8192;  // for repeated entries' sums, where the slice does not leave its space to them
 
 // One cluster for each row, one slice of the row for each CTA. Registers are held to
 // what lets 48 warps run on an SM where the loads are waited for (forward alone: 0.33
@@ -451,9 +469,8 @@ __global__ void __launch_bounds__(TH, MODE == Grad::kept ? 1024 / TH : 1536 / TH
   if (has_loose) g[loose_col] = VT<T>::store(exp2_fast(fmaf(loose, a.c, -st.z_max)) * qs);
   __syncthreads();  // the slice in shared memory is done with: its space serves the teacher's entries
   const int64_t bits_bytes = (c1 - c0 + 127) / 128 * 16;
-  const int64_t table = KEEP ? (a.slice * (int64_t)sizeof(T) - bits_bytes) / 8 : kBackwardTable;
-  subtract_teacher<T, I>(a, z, g, lo, hi, c0, c1, st, scale, reinterpret_cast<uint32_t *>(dyn),
-                         reinterpret_cast<unsigned long long *>(dyn + bits_bytes), table);
+  subtract_teacher<T, I>(a, z, g, lo, hi, c0, c1, st, scale, reinterpret_cast<uint32_t *>(dyn), dyn + bits_bytes,
+                         KEEP ? a.slice * (int64_t)sizeof(T) - bits_bytes : kTableBytes);
 }
 
 // The backward pass from the forward's statistics: one CTA for each slice.
@@ -500,9 +517,8 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const Distil
     const int64_t col = tid < sh.head ? c0 + tid : c1 - 1 - (tid - sh.head);
     g[col] = VT<T>::store(exp2_fast(fmaf(VT<T>::load(z[col]), a.c, -st.z_max)) * qs);
   }
-  unsigned long long *table = reinterpret_cast<unsigned long long *>(dyn);
-  subtract_teacher<T, I>(a, z, g, lo, hi, c0, c1, st, scale, reinterpret_cast<uint32_t *>(table + kBackwardTable),
-                         table, kBackwardTable);
+  subtract_teacher<T, I>(a, z, g, lo, hi, c0, c1, st, scale, reinterpret_cast<uint32_t *>(dyn + kTableBytes), dyn,
+                         kTableBytes);
 }
 
 template <typename K>
@@ -549,7 +565,7 @@ template <typename T, typename I> void run_typed(const DistillCall &call, cudaSt
   auto backward = [&] {
     split(pick_slices(a.rows, row_bytes, 65536, 1 << 20));
     if (a.rows * a.n_slices > INT32_MAX) fail(MSX_ERR_OVERFLOW, "csr_distillation has too many rows for one call.");
-    const size_t smem = kBackwardTable * 8 + (size_t)(a.slice + 31) / 32 * 4;
+    const size_t smem = kTableBytes + (size_t)(a.slice + 31) / 32 * 4;
     distill_backward_kernel<T, I><<<(unsigned)(a.rows * a.n_slices), kThreads, smem, s>>>(a);
     MSX_CHECK_LAUNCH();
   };
@@ -564,7 +580,7 @@ template <typename T, typename I> void run_typed(const DistillCall &call, cudaSt
   split(pick_slices(a.rows, row_bytes, kRereadMost, 8));
   const int64_t kept = a.slice * (int64_t)sizeof(T);
   if (kept > kKeepMost) {
-    const int64_t smem = ceil_div(a.slice, 128) * 16 + kBackwardTable * 8;
+    const int64_t smem = ceil_div(a.slice, 128) * 16 + kTableBytes;
     if (smem <= kMaxKept)
       return launch_rows(distill_row_kernel<T, I, Grad::reread, kRereadThreads>, a, kRereadThreads, (size_t)smem, s);
     // a bit for each column of a slice does not fit (over 12 million columns): two passes
