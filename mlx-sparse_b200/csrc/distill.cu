@@ -11,14 +11,16 @@
 // gradient. Everything is computed in base 2 (c = log2(e) / T) and in fp32;
 // the gradient is rounded once, to the logits' type.
 //
-// Bound: HBM (8192 x 128000 bf16: forward 0.34 ms, backward 0.69 ms, both in one
-// pass 0.87 ms, where the special-function unit's two exponentials and a
-// conversion for each logit, 0.55 ms, are the next limit). Forward reads the logits once, the backward pass reads them
-// again and writes the gradient. The one-pass form reads HBM once and writes
+// Bound: HBM (8192 x 128000 bf16: forward 0.34 ms, backward 0.67 ms, both in one
+// pass 0.90 ms, where the special-function unit, with two exponentials and a
+// conversion for each logit, is busy 63% of the time and DRAM moves 72% of what a copy
+// does). Forward reads the logits once, the backward pass reads them
+// again and writes the gradient. The one-pass form reads HBM about once and writes
 // once, two thirds of the bytes of the two passes: a row's logits stay on chip
 // between the sum of the exponentials and the gradient, in shared memory where
 // they fit (spread over a cluster where there are too few rows to fill the SMs),
-// else in L2, from where the CTA that summed the row reads it again.
+// else in L2, from where the CTA that summed the row reads it again (2048 x 128000
+// bf16: 634 MB read from DRAM for 524 MB of logits, a fifth of the second reads miss).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -42,9 +44,9 @@ struct RowStats {
 constexpr int kMaxKept = 200 * 1024;  // dynamic shared memory, at most
 constexpr int kKeepMost = 64 * 1024;  // slices up to this are kept in shared memory
 // Longer ones are read again, in slices of 128 KB: four CTAs an SM then have few
-// enough bytes between their two reads for L2 (8192 x 128000 bf16: 860 us with a
-// cluster of two, 947 with whole rows, all of whose second reads miss, 1095 with
-// four slices and their waits).
+// enough bytes between their two reads for L2 (8192 x 128000 bf16, in one series of
+// runs: 860 us with a cluster of two, 947 with whole rows, all of whose second reads
+// miss, 1095 with four slices and their waits; 900 on other days).
 constexpr int kRereadMost = 128 * 1024;
 constexpr int kRereadThreads = 384;
 

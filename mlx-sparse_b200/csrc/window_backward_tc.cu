@@ -31,8 +31,9 @@
 // Bound: the tensor cores, 4 x 520 (3 x 520) clocks for each tile pair at head
 // size 128, against 128 x 128 / 16 = 1024 clocks of exponentials; the weights wait
 // for the scores and the scores for the sums of the tile before, which makes it
-// about 3700 (2900). 16384 tokens, window 2048, 32 / 8 heads of 128, bf16: dQ 0.80
-// ms, dK and dV 1.09 ms.
+// about 3700 (2900), with the tensor pipe busy 55% of the time. 16384 tokens, window
+// 2048, 32 / 8 heads of 128, bf16: dQ 0.74-0.80 ms, dK and dV 1.03-1.14 ms, as the
+// power cap lets the clock run.
 //
 // A masked P or dS is 0, but 0 times an infinity or NaN in a hidden row of dO, Q
 // or K would reach the sums: rows that end not finite while something not finite
